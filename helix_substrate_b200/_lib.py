@@ -40,6 +40,12 @@ class HxqDesc(C.Structure):
     ]
 
 
+class HxqKv8(C.Structure):
+    """Mirror of struct hxq_kv8 (include/hxq_b200.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail")] \
+        + [(n, C.c_int32) for n in ("slots", "nkv", "D", "max_len")]
+
+
 class HxqError(RuntimeError):
     def __init__(self, status: int, where: str):
         self.status = status
@@ -102,6 +108,22 @@ def lib() -> C.CDLL:
     L.hxq_attn_decode.argtypes = [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
                                   C.c_void_p, C.c_size_t, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                   C.c_float, C.c_void_p]
+    K = C.POINTER(HxqKv8)
+    L.hxq_rope_append_kv8.restype = C.c_int
+    L.hxq_rope_append_kv8.argtypes = [K, C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                      C.c_int64, C.c_int32, C.c_int32, C.c_void_p]
+    L.hxq_rope_append_prompt_kv8.restype = C.c_int
+    L.hxq_rope_append_prompt_kv8.argtypes = [K, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p,
+                                             C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                             C.c_int32, C.c_void_p]
+    L.hxq_attn_decode_kv8_workspace_bytes.restype = C.c_size_t
+    L.hxq_attn_decode_kv8_workspace_bytes.argtypes = [C.c_int32] * 5
+    L.hxq_attn_decode_kv8.restype = C.c_int
+    L.hxq_attn_decode_kv8.argtypes = [K, C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p,
+                                      C.c_size_t, C.c_int32, C.c_int32, C.c_float, C.c_void_p]
+    L.hxq_kv8_rows.restype = C.c_int
+    L.hxq_kv8_rows.argtypes = [K, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,
+                               C.c_int64, C.c_void_p]
     L.hxq_dense_gemv.restype = C.c_int
     L.hxq_dense_gemv.argtypes = [C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p,
                                  C.c_int, C.c_int64, C.c_void_p]

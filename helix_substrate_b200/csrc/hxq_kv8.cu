@@ -1,0 +1,824 @@
+// hxq_kv8: a key/value cache held in 8 bits - rotary embedding + append of new rows (one token a sequence, or packed
+// prompts), single-query grouped attention over it, and its rows back as bf16.  No counterpart in the reference,
+// whose decode loop keeps the framework's 16-bit cache (helix_substrate/basin_runtime.py:358-445).
+//
+// Per (sequence, KV head) the positions form blocks of 64.  A finished block holds codes x = s * code with
+//     s = max(up(max |x| / 127), 2^-126),   code = rint(x / s) in -127 .. 127,
+// up() rounding up to bf16.  x and s then both have 8 significant bits, so x / s is a tie exactly or at least
+// 1/510 off one: the fp32 division decides every code as exact arithmetic would.  A block with an infinity or a
+// NaN gets s = NaN and reads back as NaN.  The rows of the last, unfinished block stay bf16 in the tail
+// (row = position mod 64) and are quantised once, when the 64th arrives: no row is ever rounded twice, and what a
+// cache holds does not depend on how a prompt was cut into calls.
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <utility>
+
+#include "hxq_common.cuh"
+
+namespace hxq {
+namespace kv8 {
+
+constexpr int kBlock = HXQ_KV8_BLOCK;
+
+__device__ __forceinline__ void pdl_enter() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+template <typename... KArgs, typename... Args>
+static cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStream_t stream, Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+struct Cache {
+    int8_t *k, *v;
+    float *ks, *vs;
+    __nv_bfloat16 *kt, *vt;
+    int nkv, D, max_len;
+};
+static Cache cache_of(const hxq_kv8* c) {
+    return Cache{c->k, c->v, c->k_scale, c->v_scale, reinterpret_cast<__nv_bfloat16*>(c->k_tail),
+                 reinterpret_cast<__nv_bfloat16*>(c->v_tail), c->nkv, c->D, c->max_len};
+}
+
+__device__ __forceinline__ void unpack8(const uint4& q, float (&f)[8]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        f[2 * e] = __uint_as_float(w[e] << 16);
+        f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const __nv_bfloat162 h2 = __floats2bfloat162_rn(f[2 * e], f[2 * e + 1]);
+        w[e] = *reinterpret_cast<const uint32_t*>(&h2);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 ld16(const void* p) { return *reinterpret_cast<const uint4*>(p); }
+
+// x cos - y sin in 64 bits (the products are exact there), rounded to bf16: a value next to a border of bf16 lands on
+// the side it is on, whatever the order of the operations elsewhere.
+__device__ __forceinline__ float turn(float x, float c, float y, float s) {
+    return __bfloat162float(__float2bfloat16_rn(__double2float_rn((double)x * (double)c + (double)y * (double)s)));
+}
+// The rotated pair of eight-element pieces at d and d + D / 2 of one head, `row` being the table's row.
+__device__ __forceinline__ void rotate16(float (&lo)[8], float (&hi)[8], const float* cos_row, const float* sin_row, int d, int half) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const float4 c0 = *reinterpret_cast<const float4*>(cos_row + d + 4 * q), s0 = *reinterpret_cast<const float4*>(sin_row + d + 4 * q);
+        const float4 c1 = *reinterpret_cast<const float4*>(cos_row + d + half + 4 * q), s1 = *reinterpret_cast<const float4*>(sin_row + d + half + 4 * q);
+        const float ca[4] = {c0.x, c0.y, c0.z, c0.w}, sa[4] = {s0.x, s0.y, s0.z, s0.w};
+        const float cb[4] = {c1.x, c1.y, c1.z, c1.w}, sb[4] = {s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float x0 = lo[4 * q + e], x1 = hi[4 * q + e];
+            lo[4 * q + e] = turn(x0, ca[e], -x1, sa[e]);
+            hi[4 * q + e] = turn(x1, cb[e], x0, sb[e]);
+        }
+    }
+}
+
+// ---- append -----------------------------------------------------------------------------------------
+
+struct AppendArgs {
+    Cache c;
+    const __nv_bfloat16* qkv;
+    const int32_t* cu;       // rows of qkv per sequence, or nullptr: row s is sequence s's only token
+    const int64_t* pos;      // position of each sequence's first new row (< 0: the sequence is left alone)
+    const float *cos_t, *sin_t;
+    __nv_bfloat16 *q_out, *k_out;
+    int64_t ld_qkv, ld_q, ld_k;
+    int pos_stride, T, S, max_q, nq, n_blk, kv_ctas, q_tokens;
+};
+
+constexpr int kAppendThreads = 256;
+constexpr int kMaxD = 128;
+constexpr int kUnits = 4 * kMaxD / kAppendThreads;      // pairs of eight-element pieces a thread holds of a block
+
+// Sequence s: its first row of qkv, the number of its new rows that have a place in the cache, its first position.
+__device__ __forceinline__ int sequence(const AppendArgs& a, int s, int& row0, int64_t& p0) {
+    p0 = a.pos[(int64_t)s * a.pos_stride];
+    int r0 = s, r1 = s + 1;
+    if (a.cu != nullptr) {
+        r0 = a.cu[s];
+        r1 = a.cu[s + 1];
+    }
+    if (r0 < 0) r0 = 0;
+    if (r1 > a.T) r1 = a.T;
+    row0 = r0;
+    if (p0 < 0 || p0 >= a.c.max_len || r1 <= r0) return 0;       // (a position past the cache may be any number)
+    const int n = r1 - r0 < a.max_q ? r1 - r0 : a.max_q, room = a.c.max_len - (int)p0;
+    return n < room ? n : room;
+}
+
+// One block of one KV head's keys or values: rows from r_old on are new, rows before it stand in the tail.
+// A whole block is quantised, of an unfinished one the new rows go to the tail.
+__device__ void append_block(const AppendArgs& a, bool is_k, int s, int h, int blk, int row0, int64_t p0, int n, float* red) {
+    const int D = a.c.D, half = D >> 1, pieces = D >> 4;
+    const int64_t b0 = (int64_t)blk * kBlock;
+    const int r_old = p0 > b0 ? (int)(p0 - b0) : 0;
+    const int r_end = p0 + n - b0 < kBlock ? (int)(p0 + n - b0) : kBlock;
+    const bool whole = r_end == kBlock;
+    const int64_t head = (int64_t)s * a.c.nkv + h;
+    __nv_bfloat16* tail = (is_k ? a.c.kt : a.c.vt) + head * kBlock * D;
+    const int col = (a.nq + (is_k ? 0 : a.c.nkv) + h) * D;
+
+    float lo[kUnits][8], hi[kUnits][8];
+    float amax = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < kUnits; ++j) {
+        const int u = threadIdx.x + j * kAppendThreads;
+        const int r = u / pieces, d = (u - r * pieces) * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) lo[j][e] = hi[j][e] = 0.f;
+        if (r >= r_end || (!whole && r < r_old)) continue;
+        if (r < r_old) {
+            unpack8(ld16(tail + r * D + d), lo[j]);
+            unpack8(ld16(tail + r * D + d + half), hi[j]);
+        } else {
+            const int64_t p = b0 + r;
+            const int64_t t = row0 + (p - p0);
+            const __nv_bfloat16* src = a.qkv + t * a.ld_qkv + col;
+            unpack8(ld16(src + d), lo[j]);
+            unpack8(ld16(src + d + half), hi[j]);
+            if (is_k) {
+                rotate16(lo[j], hi[j], a.cos_t + p * D, a.sin_t + p * D, d, half);
+                if (a.k_out != nullptr) {
+                    __nv_bfloat16* dst = a.k_out + t * a.ld_k + h * D + d;
+                    *reinterpret_cast<uint4*>(dst) = pack8(lo[j]);
+                    *reinterpret_cast<uint4*>(dst + half) = pack8(hi[j]);
+                }
+            }
+            if (!whole) {
+                *reinterpret_cast<uint4*>(tail + r * D + d) = pack8(lo[j]);
+                *reinterpret_cast<uint4*>(tail + r * D + d + half) = pack8(hi[j]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            amax = fmaxf(amax, fmaxf(fabsf(lo[j][e]), fabsf(hi[j][e])));
+            bad |= !(fabsf(lo[j][e]) <= 3.4e38f) || !(fabsf(hi[j][e]) <= 3.4e38f);
+        }
+    }
+    if (!whole) return;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    bad = __any_sync(0xffffffffu, bad);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = bad ? INFINITY : amax;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, red[w]);
+    __syncthreads();                 // (red is used again, and the tail's rows have been read)
+    bad = amax == INFINITY;
+    float scale = __uint_as_float((__float_as_uint(__fdiv_rn(amax, 127.f)) + 0xffffu) & 0xffff0000u);
+    scale = fmaxf(scale, 1.17549435e-38f);
+    int8_t* codes = (is_k ? a.c.k : a.c.v) + (head * a.c.max_len + b0) * D;
+    if (threadIdx.x == 0) (is_k ? a.c.ks : a.c.vs)[head * (a.c.max_len / kBlock) + blk] = bad ? __uint_as_float(0x7fc00000u) : scale;
+#pragma unroll
+    for (int j = 0; j < kUnits; ++j) {
+        const int u = threadIdx.x + j * kAppendThreads;
+        const int r = u / pieces, d = (u - r * pieces) * 8;
+        if (r >= kBlock) continue;
+        uint32_t w[4] = {0u, 0u, 0u, 0u};
+        if (!bad) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                w[e >> 2] |= ((uint32_t)__float2int_rn(__fdiv_rn(lo[j][e], scale)) & 0xffu) << (8 * (e & 3));
+                w[2 + (e >> 2)] |= ((uint32_t)__float2int_rn(__fdiv_rn(hi[j][e], scale)) & 0xffu) << (8 * (e & 3));
+            }
+        }
+        *reinterpret_cast<uint2*>(codes + r * D + d) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2*>(codes + r * D + d + half) = make_uint2(w[2], w[3]);
+    }
+}
+
+// The first kv_ctas CTAs take one (sequence, KV head, keys or values, block) each, the others q_tokens rows of query
+// heads.  Bound by HBM for prompts, by one memory round trip and the launch for single tokens.
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
+    __shared__ float red[kAppendThreads / 32];
+    pdl_enter();
+    const int D = a.c.D;
+    if ((int)blockIdx.x < a.kv_ctas) {
+        int i = blockIdx.x;
+        const int j = i % a.n_blk;
+        i /= a.n_blk;
+        const bool is_k = (i & 1) == 0;
+        i >>= 1;
+        const int h = i % a.c.nkv, s = i / a.c.nkv;
+        int row0;
+        int64_t p0;
+        const int n = sequence(a, s, row0, p0);
+        if (n == 0) return;
+        const int first = (int)(p0 / kBlock), last = (int)((p0 + n - 1) / kBlock);
+        const int blk = first + j;
+        if (blk > last) return;
+        // An unfinished last block's rows take the place of the tail's rows that the first block takes in: where both
+        // happen, the first block's CTA does one after the other.
+        const bool waits = p0 % kBlock != 0 && last != first && (p0 + n) % kBlock != 0;
+        if (waits && blk == last) return;
+        append_block(a, is_k, s, h, blk, row0, p0, n, red);
+        if (waits && blk == first) append_block(a, is_k, s, h, last, row0, p0, n, red);
+        return;
+    }
+    // query heads: a thread takes the pair of pieces (d, d + D / 2) of one head and row
+    const int pieces = D >> 4, half = D >> 1;
+    const int t0 = ((int)blockIdx.x - a.kv_ctas) * a.q_tokens;
+    const int per_token = a.nq * pieces;
+    for (int u = threadIdx.x; u < a.q_tokens * per_token; u += kAppendThreads) {
+        const int t = t0 + u / per_token;
+        if (t >= a.T) break;
+        const int rem = u % per_token;
+        const int d = (rem % pieces) * 8;
+        int64_t p = -1;
+        if (a.cu == nullptr) {
+            p = a.pos[(int64_t)t * a.pos_stride];
+        } else {
+            int lo = 0, hi = a.S;          // the sequence with cu[s] <= t < cu[s + 1]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (a.cu[mid] <= t) lo = mid; else hi = mid;
+            }
+            const int64_t first = a.pos[(int64_t)lo * a.pos_stride];
+            const int i = t - a.cu[lo];
+            if (first >= 0 && i >= 0 && i < a.max_q && t < a.cu[lo + 1]) p = first + i;
+        }
+        if (p < 0 || p >= a.c.max_len) continue;
+        const __nv_bfloat16* src = a.qkv + (int64_t)t * a.ld_qkv + (rem / pieces) * D + d;
+        float lo8[8], hi8[8];
+        unpack8(ld16(src), lo8);
+        unpack8(ld16(src + half), hi8);
+        rotate16(lo8, hi8, a.cos_t + p * D, a.sin_t + p * D, d, half);
+        __nv_bfloat16* dst = a.q_out + (int64_t)t * a.ld_q + (rem / pieces) * D + d;
+        *reinterpret_cast<uint4*>(dst) = pack8(lo8);
+        *reinterpret_cast<uint4*>(dst + half) = pack8(hi8);
+    }
+}
+
+// ---- rows back as bf16 ------------------------------------------------------------------------------
+
+// One block of one KV head per CTA (keys and values): 16 codes in, 32 bytes out per thread and step.
+__global__ void __launch_bounds__(256) rows_kernel(const Cache c, const int64_t* __restrict__ len_p, int len_stride, int rows,
+                                                   __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out,
+                                                   int64_t ld_seq, int64_t ld_head, int64_t ld_row) {
+    const int blk = blockIdx.x, h = blockIdx.y, s = blockIdx.z;
+    pdl_enter();
+    int64_t len = len_p[(int64_t)s * len_stride];
+    if (len > rows) len = rows;
+    if (len > c.max_len) len = c.max_len;
+    const int64_t b0 = (int64_t)blk * kBlock;
+    if (b0 >= len) return;
+    const int64_t have = len_p[(int64_t)s * len_stride];
+    const bool whole = have - b0 >= kBlock;            // (rows may cut a finished block short)
+    const int n = (int)(len - b0 < kBlock ? len - b0 : kBlock);
+    const int pieces = c.D >> 4;
+    const int64_t head = (int64_t)s * c.nkv + h;
+    const int64_t out0 = s * ld_seq + h * ld_head + b0 * ld_row;
+    const float ks = whole ? c.ks[head * (c.max_len / kBlock) + blk] : 0.f, vs = whole ? c.vs[head * (c.max_len / kBlock) + blk] : 0.f;
+    for (int u = threadIdx.x; u < 2 * n * pieces; u += 256) {
+        const bool is_v = u >= n * pieces;
+        const int w = is_v ? u - n * pieces : u;
+        const int r = w / pieces, d = (w - r * pieces) * 16;
+        __nv_bfloat16* dst = (is_v ? v_out : k_out) + out0 + r * ld_row + d;
+        if (whole) {
+            const uint4 q = ld_stream_u4((is_v ? c.v : c.k) + (head * c.max_len + b0 + r) * c.D + d);
+            const uint32_t wd[4] = {q.x, q.y, q.z, q.w};
+            const float sc = is_v ? vs : ks;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = (float)(int8_t)(wd[2 * g + (e >> 2)] >> (8 * (e & 3))) * sc;
+                *reinterpret_cast<uint4*>(dst + 8 * g) = pack8(f);
+            }
+        } else {
+            const __nv_bfloat16* src = (is_v ? c.vt : c.kt) + (head * kBlock + r) * c.D + d;
+            const uint4 a = ld16(src), b = ld16(src + 8);
+            *reinterpret_cast<uint4*>(dst) = a;
+            *reinterpret_cast<uint4*>(dst + 8) = b;
+        }
+    }
+}
+
+// ---- single-query attention -------------------------------------------------------------------------
+
+constexpr int kWarps = 4;
+constexpr int kHeads = 8;           // query heads of a KV head: the used rows of an MMA's sixteen
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t bf2_of(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Two biased bytes (code + 128), picked by sel out of x, as two exact fp16 integers: 0x64nn is 1024 + nn.
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t codes2(uint32_t x) {
+    const uint32_t h = __byte_perm(x, 0x64646464u, SEL);
+    const uint32_t bias = 0x64806480u;      // 1152
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(bias));
+    return r;
+}
+__device__ __forceinline__ uint2 ld_stream_u2(const void* p) {
+    uint2 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ float quad_max(float v) {
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+    v += __shfl_xor_sync(0xffffffffu, v, 1);
+    return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+
+// Units of 64 positions (the last one the tail) of one sequence, and how many of them a CTA of the split takes.
+__device__ __forceinline__ int units_of(int64_t pos, int max_len) {
+    if (pos < 0 || pos >= max_len) return 0;
+    return (int)(pos / kBlock) + 1;
+}
+
+struct DecodeArgs {
+    Cache c;
+    const __nv_bfloat16* q;
+    const int64_t* pos;
+    __nv_bfloat16* out;
+    float* part;            // [B, nq, splits, D + 2]: maximum, sum, un-normalised output
+    int64_t ld_q, ld_out;
+    int pos_stride, nq, G, splits;
+    float scale_log2;       // scale * log2(e)
+};
+
+// One CTA: a contiguous share of one sequence's blocks, one KV head, all of its (up to eight) query heads; a warp takes
+// whole blocks of 64 positions in turn, 32 positions at a step.
+//
+// Bound by HBM: each code is read once, 2 D bytes a position and KV head.  On the CUDA cores G query heads cost G
+// multiply-adds a code, more than the cores have at the memory's pace from G = 5 on, so both products go through
+// mma.sync m16n8k16 in fp16 with fp32 sums (a tcgen05 tile would want 128 rows of queries; there are eight).
+//   * codes become fp16 exactly (two byte permutes and a subtraction for four); a query row is scaled by a power of two
+//     into fp16's range, which keeps bf16's eight bits; a block's scale multiplies sums in fp32.
+//   * the order of a contraction's index is free, so it is chosen such that every lane's operands are 16 consecutive
+//     bytes of a cache row: keys go from memory to registers to the MMA with no exchange, values with two byte permutes per
+//     two rows, and a warp's load covers whole 64- or 128-byte pieces.  The next 32 positions' keys are in flight while
+//     this step's values are used, and the other way round.
+//   * probabilities are rounded to fp16, 2^-12 relative, a sixteenth of the output's own rounding; the sum that divides
+//     takes them in fp32.
+//   * the tail's products run in bf16, with each probability as the sum of two bf16 numbers (2^-17).
+template <int DP>
+__global__ void __launch_bounds__(32 * kWarps) decode_kernel(const DecodeArgs a) {
+    constexpr int KS = DP / 16;        // k steps of Q K^T
+    constexpr int KC = DP / 64;        // 16-byte pieces of a key row per lane
+    constexpr int NT = DP / 8;         // n tiles of P V, and bytes of a value row per lane
+    const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int D = a.c.D;
+    pdl_enter();
+    const int64_t pos = a.pos[(int64_t)b * a.pos_stride];
+    const int units = units_of(pos, a.c.max_len);
+    const int span = (units + a.splits - 1) / a.splits;
+    const int u0 = split * span, u1 = u0 + span < units ? u0 + span : units;
+    if (u0 >= u1) {
+        if (a.splits == 1)          // nothing to see: zeros
+            for (int i = threadIdx.x; i < a.G * D; i += 32 * kWarps) a.out[(int64_t)b * a.ld_out + (int64_t)kvh * a.G * D + i] = __float2bfloat16_rn(0.f);
+        return;
+    }
+    const int tail_n = (int)((pos + 1) % kBlock);        // rows of the unfinished block
+    const int whole = tail_n ? units - 1 : units;        // units below this one are finished blocks
+    const int64_t head = (int64_t)b * a.c.nkv + kvh;
+    const __nv_bfloat16* q = a.q + (int64_t)b * a.ld_q + ((int64_t)kvh * a.G + (g < a.G ? g : 0)) * D;
+
+    float o[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = 0.f;
+    float m = -INFINITY, l = 0.f;           // of head g: m the same in its four lanes, l this lane's positions
+
+    // Running softmax of S scores; rescales o when the maximum moved.  Returns the probabilities in s.
+    auto softmax = [&](float* s, int S) {
+        float mx = m;
+#pragma unroll
+        for (int i = 0; i < S; ++i) mx = fmaxf(mx, s[i]);
+        mx = quad_max(mx);
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        const float corr = exp2f(m - ref);
+        l *= corr;
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            s[i] = exp2f(s[i] - ref);
+            l += s[i];
+        }
+        if (__any_sync(0xffffffffu, mx != m)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) { o[n][0] *= corr; o[n][1] *= corr; }
+        }
+        m = mx;
+    };
+
+    int u = u0 + warp;
+    if (u < u1 && u < whole) {
+        // query rows as fp16 A operands: lane (g, t) holds the dimensions of the key pieces it loads
+        uint32_t qa[KS][2];
+        float q_back;
+        {
+            float f[KC][2][8];
+            float amax = 0.f;
+#pragma unroll
+            for (int i = 0; i < KC; ++i)
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    const int d = 64 * i + 16 * t + 8 * hh;
+                    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                    if (d < D && g < a.G) w = ld16(q + d);
+                    unpack8(w, f[i][hh]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[i][hh][e]));
+                }
+            amax = quad_max(amax);
+            int ex = (int)(__float_as_uint(amax) >> 23);        // 0 .. 255
+            if (ex == 0 || ex == 255) ex = 137;                 // zeros, infinities: as they are
+            if (ex < 27) ex = 27;
+            const float up = __uint_as_float((uint32_t)(264 - ex) << 23);      // largest element into [2^10, 2^11)
+            q_back = __uint_as_float((uint32_t)(ex - 10) << 23);
+#pragma unroll
+            for (int i = 0; i < KC; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float* e = &f[i][j >> 1][4 * (j & 1)];
+                    qa[4 * i + j][0] = half2_of(e[0] * up, e[1] * up);
+                    qa[4 * i + j][1] = half2_of(e[2] * up, e[3] * up);
+                }
+            q_back *= a.scale_log2;
+        }
+        const int8_t* kp = a.c.k + head * a.c.max_len * D;
+        const int8_t* vp = a.c.v + head * a.c.max_len * D;
+        const float* ksp = a.c.ks + head * (a.c.max_len / kBlock);
+        const float* vsp = a.c.vs + head * (a.c.max_len / kBlock);
+        uint4 kr[4][KC];
+        uint4 vr[2][4];           // (eight-byte loads at DP = 64 use x and y)
+        auto load_k = [&](int unit, int half) {
+            const int8_t* p = kp + ((int64_t)unit * kBlock + half * 32 + g) * D + 16 * t;
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int i = 0; i < KC; ++i) kr[n][i] = 64 * i + 16 * t < D ? ld_stream_u4(p + n * 8 * D + 64 * i) : make_uint4(0u, 0u, 0u, 0u);
+        };
+        auto load_v = [&](int unit, int half) {
+            const int8_t* p = vp + ((int64_t)unit * kBlock + half * 32 + 2 * t) * D + NT * g;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int8_t* pr = p + (16 * j + (r & 1) + 8 * (r >> 1)) * D;
+                    vr[j][r] = make_uint4(0u, 0u, 0u, 0u);
+                    if (NT * g < D) {
+                        if constexpr (NT == 16) {
+                            vr[j][r] = ld_stream_u4(pr);
+                        } else {
+                            const uint2 w = ld_stream_u2(pr);
+                            vr[j][r].x = w.x;
+                            vr[j][r].y = w.y;
+                        }
+                    }
+                }
+        };
+        const int u_end = u1 < whole ? u1 : whole;
+        load_k(u, 0);
+        load_v(u, 0);
+        float ks = ksp[u], vs = vsp[u];
+        int half = 0;
+        while (true) {
+            int nu = u, nh = 1;
+            if (half == 1) { nu = u + kWarps; nh = 0; }
+            const bool more = nu < u_end;
+            float s[8], c4[4][4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) c4[n][0] = c4[n][1] = c4[n][2] = c4[n][3] = 0.f;
+#pragma unroll
+            for (int i = 0; i < KC; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {       // four independent sums
+                        const uint32_t w[4] = {kr[n][i].x, kr[n][i].y, kr[n][i].z, kr[n][i].w};
+                        const uint32_t x = w[j] ^ 0x80808080u;
+                        mma_f16(c4[n], qa[4 * i + j][0], qa[4 * i + j][1], codes2<0x4140>(x), codes2<0x4342>(x));
+                    }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                s[2 * n] = c4[n][0] * (ks * q_back);
+                s[2 * n + 1] = c4[n][1] * (ks * q_back);
+            }
+            if (more) load_k(nu, nh);
+            softmax(s, 8);
+#pragma unroll
+            for (int n0 = 0; n0 < NT; n0 += 4) {
+                float c[4][4];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t p0 = half2_of(s[4 * j], s[4 * j + 1]), p1 = half2_of(s[4 * j + 2], s[4 * j + 3]);
+                    uint32_t w[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const uint32_t v4[4] = {vr[j][r].x, vr[j][r].y, vr[j][r].z, vr[j][r].w};
+                        w[r] = v4[n0 >> 2] ^ 0x80808080u;
+                    }
+                    const uint32_t a01 = __byte_perm(w[0], w[1], 0x5140), a23 = __byte_perm(w[0], w[1], 0x7362);
+                    const uint32_t b01 = __byte_perm(w[2], w[3], 0x5140), b23 = __byte_perm(w[2], w[3], 0x7362);
+                    mma_f16(c[0], p0, p1, codes2<0x4140>(a01), codes2<0x4140>(b01));
+                    mma_f16(c[1], p0, p1, codes2<0x4342>(a01), codes2<0x4342>(b01));
+                    mma_f16(c[2], p0, p1, codes2<0x4140>(a23), codes2<0x4140>(b23));
+                    mma_f16(c[3], p0, p1, codes2<0x4342>(a23), codes2<0x4342>(b23));
+                }
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    o[n0 + n][0] = fmaf(vs, c[n][0], o[n0 + n][0]);
+                    o[n0 + n][1] = fmaf(vs, c[n][1], o[n0 + n][1]);
+                }
+            }
+            if (!more) break;
+            load_v(nu, nh);
+            if (nh == 0) { ks = ksp[nu]; vs = vsp[nu]; }
+            u = nu;
+            half = nh;
+        }
+    }
+
+    // the unfinished block: bf16 rows, sixteen positions at a step
+    if (tail_n && u1 == units && (units - 1 - u0) % kWarps == warp) {
+        const __nv_bfloat16* kt = a.c.kt + head * kBlock * D;
+        const __nv_bfloat16* vt = a.c.vt + head * kBlock * D;
+        uint32_t qb[KS][2];
+#pragma unroll
+        for (int i = 0; i < KS / 2; ++i) {
+            uint4 w = make_uint4(0u, 0u, 0u, 0u);
+            if (32 * i + 8 * t < D && g < a.G) w = ld16(q + 32 * i + 8 * t);
+            qb[2 * i][0] = w.x; qb[2 * i][1] = w.y;
+            qb[2 * i + 1][0] = w.z; qb[2 * i + 1][1] = w.w;
+        }
+        for (int p = 0; p < tail_n; p += 16) {
+            float s[4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int row = p + 8 * n + g;
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < KS / 2; ++i) {
+                    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                    if (32 * i + 8 * t < D && row < tail_n) w = ld16(kt + row * D + 32 * i + 8 * t);
+                    mma_bf16(c, qb[2 * i][0], qb[2 * i][1], w.x, w.y);
+                    mma_bf16(c, qb[2 * i + 1][0], qb[2 * i + 1][1], w.z, w.w);
+                }
+                const int col = p + 8 * n + 2 * t;
+                s[2 * n] = col < tail_n ? c[0] * a.scale_log2 : -INFINITY;
+                s[2 * n + 1] = col + 1 < tail_n ? c[1] * a.scale_log2 : -INFINITY;
+            }
+            softmax(s, 4);
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const float h0 = __bfloat162float(__float2bfloat16_rn(s[2 * n])), h1 = __bfloat162float(__float2bfloat16_rn(s[2 * n + 1]));
+                hi[n] = bf2_of(h0, h1);
+                lo[n] = bf2_of(s[2 * n] - h0, s[2 * n + 1] - h1);
+            }
+#pragma unroll
+            for (int n0 = 0; n0 < NT; n0 += 8) {          // eight dimensions of four rows at a time
+                uint4 w[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = p + 2 * t + (r & 1) + 8 * (r >> 1);
+                    w[r] = make_uint4(0u, 0u, 0u, 0u);
+                    if (NT * g + n0 < D && row < tail_n) w[r] = ld16(vt + row * D + NT * g + n0);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t x0 = (&w[0].x)[e], x1 = (&w[1].x)[e], x2 = (&w[2].x)[e], x3 = (&w[3].x)[e];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t b0 = __byte_perm(x0, x1, k ? 0x7632 : 0x5410), b1 = __byte_perm(x2, x3, k ? 0x7632 : 0x5410);
+                        float c[4] = {o[n0 + 2 * e + k][0], o[n0 + 2 * e + k][1], 0.f, 0.f};
+                        mma_bf16(c, hi[0], hi[1], b0, b1);
+                        mma_bf16(c, lo[0], lo[1], b0, b1);
+                        o[n0 + 2 * e + k][0] = c[0];
+                        o[n0 + 2 * e + k][1] = c[1];
+                    }
+                }
+            }
+        }
+    }
+
+    // ---- the four warps' (m, l, o) meet; lane (g, t) owns dimensions 2 NT t .. of head g
+    __shared__ float o_s[kWarps][kHeads][DP];
+    __shared__ float m_s[kWarps][kHeads], l_s[kWarps][kHeads];
+    l = quad_sum(l);
+    if (t == 0) { m_s[warp][g] = m; l_s[warp][g] = l; }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        o_s[warp][g][2 * NT * t + n] = o[n][0];
+        o_s[warp][g][2 * NT * t + NT + n] = o[n][1];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.G * D; i += 32 * kWarps) {
+        const int hd = i / D, d = i - hd * D;
+        float mx = m_s[0][hd];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, m_s[w][hd]);
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        float ov = 0.f, lv = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float e = exp2f(m_s[w][hd] - ref);
+            ov += e * o_s[w][hd][d];
+            lv += e * l_s[w][hd];
+        }
+        if (a.splits == 1) {
+            a.out[(int64_t)b * a.ld_out + ((int64_t)kvh * a.G + hd) * D + d] = __float2bfloat16_rn(ov / lv);
+        } else {
+            float* dst = a.part + (((int64_t)b * a.nq + kvh * a.G + hd) * a.splits + split) * (D + 2);
+            dst[2 + d] = ov;
+            if (d == 0) { dst[0] = mx; dst[1] = lv; }
+        }
+    }
+}
+
+// out[b, head] = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over the CTAs that had blocks to look at.
+__global__ void __launch_bounds__(kMaxD) combine_kernel(const DecodeArgs a) {
+    const int head = blockIdx.x, b = blockIdx.y, d = threadIdx.x, D = a.c.D;
+    pdl_enter();
+    const int units = units_of(a.pos[(int64_t)b * a.pos_stride], a.c.max_len);
+    if (d >= D) return;
+    __nv_bfloat16* out = a.out + (int64_t)b * a.ld_out + (int64_t)head * D;
+    if (units == 0) {
+        out[d] = __float2bfloat16_rn(0.f);
+        return;
+    }
+    const int span = (units + a.splits - 1) / a.splits, nc = (units + span - 1) / span;
+    const float* src = a.part + ((int64_t)b * a.nq + head) * a.splits * (D + 2);
+    float mx = -INFINITY;
+    for (int c = 0; c < nc; ++c) mx = fmaxf(mx, src[(int64_t)c * (D + 2)]);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float o = 0.f, l = 0.f;
+    for (int c = 0; c < nc; ++c) {
+        const float* p = src + (int64_t)c * (D + 2);
+        const float e = exp2f(p[0] - ref);
+        l += e * p[1];
+        o += e * p[2 + d];
+    }
+    out[d] = __float2bfloat16_rn(o / l);
+}
+
+// ---- host side --------------------------------------------------------------------------------------
+
+static int check_cache(const hxq_kv8* c) {
+    if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale || !c->k_tail || !c->v_tail) return HXQ_E_ARG;
+    if (c->slots <= 0 || c->nkv <= 0 || c->nkv > 65535 || c->D < 16 || c->D > kMaxD || c->D % 16 != 0 || c->max_len <= 0 || c->max_len % kBlock != 0)
+        return HXQ_E_SHAPE;
+    if (!aligned_to(c->k, 16) || !aligned_to(c->v, 16) || !aligned_to(c->k_tail, 16) || !aligned_to(c->v_tail, 16) ||
+        !aligned_to(c->k_scale, 4) || !aligned_to(c->v_scale, 4))
+        return HXQ_E_ALIGN;
+    return HXQ_OK;
+}
+
+static int run_append(const hxq_kv8* c, const void* qkv, int64_t ld_qkv, int32_t T, const int32_t* cu, int32_t S, int32_t max_q,
+                      const int64_t* pos, int32_t pos_stride, const float* cos_table, const float* sin_table, void* q_out, int64_t ld_q,
+                      void* k_out, int64_t ld_k, int32_t nq, cudaStream_t stream) {
+    if (!qkv || !pos || !cos_table || !sin_table || !q_out || T < 0 || S <= 0 || max_q < 0 || nq <= 0) return HXQ_E_ARG;
+    const int st = check_cache(c);
+    if (st != HXQ_OK) return st;
+    const int64_t width = (int64_t)(nq + 2 * c->nkv) * c->D;
+    if (S > c->slots || nq % c->nkv != 0 || (pos_stride != 0 && pos_stride != 1)) return HXQ_E_SHAPE;
+    if (ld_qkv < width || ld_q < (int64_t)nq * c->D || (k_out && ld_k < (int64_t)c->nkv * c->D)) return HXQ_E_SHAPE;
+    if (!aligned_to(qkv, 16) || !aligned_to(q_out, 16) || !aligned_to(cos_table, 16) || !aligned_to(sin_table, 16) || ld_qkv % 8 != 0 ||
+        ld_q % 8 != 0 || (k_out && (!aligned_to(k_out, 16) || ld_k % 8 != 0)))
+        return HXQ_E_ALIGN;
+    if (T == 0 || max_q == 0) return HXQ_OK;
+    AppendArgs a;
+    a.c = cache_of(c);
+    a.qkv = reinterpret_cast<const __nv_bfloat16*>(qkv);
+    a.cu = cu;
+    a.pos = pos;
+    a.cos_t = cos_table;
+    a.sin_t = sin_table;
+    a.q_out = reinterpret_cast<__nv_bfloat16*>(q_out);
+    a.k_out = reinterpret_cast<__nv_bfloat16*>(k_out);
+    a.ld_qkv = ld_qkv; a.ld_q = ld_q; a.ld_k = ld_k;
+    a.pos_stride = pos_stride; a.T = T; a.S = S; a.nq = nq;
+    a.max_q = max_q < c->max_len ? max_q : c->max_len;
+    a.n_blk = cu ? (a.max_q + 2 * kBlock - 2) / kBlock : 1;          // blocks that max_q rows can touch, wherever they start
+    // rows of query heads per CTA: about two steps of its threads
+    const int per_token = nq * (c->D / 16);
+    a.q_tokens = 2 * kAppendThreads / per_token > 0 ? 2 * kAppendThreads / per_token : 1;
+    const int64_t kv = (int64_t)S * c->nkv * 2 * a.n_blk, qc = ((int64_t)T + a.q_tokens - 1) / a.q_tokens;
+    if (kv + qc > 0x7fffffffLL) return HXQ_E_SHAPE;
+    a.kv_ctas = (int)kv;
+    const cudaError_t e = launch_pdl(append_kernel, dim3((unsigned)(kv + qc)), dim3(kAppendThreads), stream, a);
+    return e == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
+}
+
+// CTAs that share one sequence and KV head.
+static int decode_splits(int B, int nkv, int max_len) {
+    const int64_t units = max_len / kBlock, pairs = (int64_t)B * nkv;
+    int64_t n = (148 * 8 + pairs - 1) / pairs;          // about eight CTAs of four warps per SM in all
+    const int64_t most = (units + kWarps - 1) / kWarps; // a block for each warp
+    if (n > most) n = most;
+    return (int)(n < 1 ? 1 : n);
+}
+
+}  // namespace kv8
+}  // namespace hxq
+
+using namespace hxq::kv8;
+
+extern "C" int hxq_rope_append_kv8(const hxq_kv8* cache, const void* qkv, int64_t ld_qkv, const int64_t* pos, int32_t pos_stride,
+                                   const float* cos_table, const float* sin_table, void* q_out, int64_t ld_q, int32_t B, int32_t nq,
+                                   hxq_stream_t stream) {
+    if (B <= 0) return HXQ_E_ARG;
+    return run_append(cache, qkv, ld_qkv, B, nullptr, B, 1, pos, pos_stride, cos_table, sin_table, q_out, ld_q, nullptr, 0, nq,
+                      reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int hxq_rope_append_prompt_kv8(const hxq_kv8* cache, const void* qkv, int64_t ld_qkv, int32_t T, const int32_t* cu, int32_t S,
+                                          int32_t max_q, const int64_t* pos, int32_t pos_stride, const float* cos_table, const float* sin_table,
+                                          void* q_out, int64_t ld_q, void* k_out, int64_t ld_k, int32_t nq, hxq_stream_t stream) {
+    if (!cu) return HXQ_E_ARG;
+    return run_append(cache, qkv, ld_qkv, T, cu, S, max_q, pos, pos_stride, cos_table, sin_table, q_out, ld_q, k_out, ld_k, nq,
+                      reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int hxq_kv8_rows(const hxq_kv8* cache, const int64_t* len, int32_t len_stride, int32_t S, int32_t rows, void* k_out, void* v_out,
+                            int64_t ld_seq, int64_t ld_head, int64_t ld_row, hxq_stream_t stream) {
+    if (!len || !k_out || !v_out || S <= 0 || rows < 0) return HXQ_E_ARG;
+    const int st = check_cache(cache);
+    if (st != HXQ_OK) return st;
+    if (S > cache->slots || S > 65535 || (len_stride != 0 && len_stride != 1) || ld_row < cache->D) return HXQ_E_SHAPE;
+    if (!hxq::aligned_to(k_out, 16) || !hxq::aligned_to(v_out, 16) || ld_seq % 8 != 0 || ld_head % 8 != 0 || ld_row % 8 != 0) return HXQ_E_ALIGN;
+    const int n = rows < cache->max_len ? rows : cache->max_len;
+    if (n == 0) return HXQ_OK;
+    const cudaError_t e = launch_pdl(rows_kernel, dim3((n + kBlock - 1) / kBlock, cache->nkv, S), dim3(256), reinterpret_cast<cudaStream_t>(stream),
+                                     cache_of(cache), len, (int)len_stride, n, reinterpret_cast<__nv_bfloat16*>(k_out),
+                                     reinterpret_cast<__nv_bfloat16*>(v_out), ld_seq, ld_head, ld_row);
+    return e == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
+}
+
+extern "C" size_t hxq_attn_decode_kv8_workspace_bytes(int32_t B, int32_t nq, int32_t nkv, int32_t D, int32_t max_len) {
+    if (B <= 0 || nq <= 0 || nkv <= 0 || D <= 0 || max_len <= 0) return 0;
+    const int n = decode_splits(B, nkv, max_len);
+    return n == 1 ? 0 : (size_t)B * nq * n * (D + 2) * sizeof(float);
+}
+
+extern "C" int hxq_attn_decode_kv8(const hxq_kv8* cache, const void* q, int64_t ld_q, const int64_t* pos, int32_t pos_stride, void* out,
+                                   int64_t ld_out, void* workspace, size_t workspace_bytes, int32_t B, int32_t nq, float scale,
+                                   hxq_stream_t stream_) {
+    if (!q || !pos || !out || B <= 0 || nq <= 0) return HXQ_E_ARG;
+    const int st = check_cache(cache);
+    if (st != HXQ_OK) return st;
+    if (B > cache->slots || B > 65535 || nq % cache->nkv != 0 || nq / cache->nkv > kHeads || (pos_stride != 0 && pos_stride != 1)) return HXQ_E_SHAPE;
+    if (ld_q < (int64_t)nq * cache->D || ld_out < (int64_t)nq * cache->D) return HXQ_E_SHAPE;
+    if (!hxq::aligned_to(q, 16) || ld_q % 8 != 0) return HXQ_E_ALIGN;
+    DecodeArgs a;
+    a.splits = decode_splits(B, cache->nkv, cache->max_len);
+    if (a.splits > 1 && (!workspace || !hxq::aligned_to(workspace, 4) ||
+                         workspace_bytes < hxq_attn_decode_kv8_workspace_bytes(B, nq, cache->nkv, cache->D, cache->max_len)))
+        return HXQ_E_WORKSPACE;
+    a.c = cache_of(cache);
+    a.q = reinterpret_cast<const __nv_bfloat16*>(q);
+    a.pos = pos;
+    a.out = reinterpret_cast<__nv_bfloat16*>(out);
+    a.part = reinterpret_cast<float*>(workspace);
+    a.ld_q = ld_q; a.ld_out = ld_out;
+    a.pos_stride = pos_stride; a.nq = nq; a.G = nq / cache->nkv;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+    const dim3 grid(a.splits, cache->nkv, B);
+    cudaError_t e = cache->D <= 64 ? launch_pdl(decode_kernel<64>, grid, dim3(32 * kWarps), stream, a)
+                                   : launch_pdl(decode_kernel<128>, grid, dim3(32 * kWarps), stream, a);
+    if (e == cudaSuccess && a.splits > 1) e = launch_pdl(combine_kernel, dim3(nq, B), dim3(kMaxD), stream, a);
+    return e == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
+}

@@ -236,6 +236,58 @@ int hxq_attn_decode(const void* q, int64_t ld_q, const void* k_cache, const void
  * cache are few, more as they grow.  Needs no device. */
 int32_t hxq_attn_decode_span(int32_t B, int32_t nkv, int32_t max_len);
 
+/*
+ * ---- key/value cache held in 8 bits (no counterpart in the reference, which keeps the framework's
+ * 16-bit cache: helix_substrate/basin_runtime.py:358-445) ----
+ * Positions form blocks of HXQ_KV8_BLOCK.  A finished block of one (sequence, KV head) holds int8 codes and
+ * one fp32 scale for its keys and one for its values, x = scale * code:  scale = max(|x|) / 127 rounded up to
+ * bf16, at least 2^-126; code = x / scale rounded to nearest even.  A block that holds an infinity or a NaN gets
+ * the scale NaN (codes 0).  The rows of a sequence's last, unfinished block stay bf16 in the tail, row =
+ * position mod HXQ_KV8_BLOCK.  D % 16 == 0, 16 <= D <= 128, max_len % HXQ_KV8_BLOCK == 0; buffers contiguous,
+ * codes and tails 16-byte aligned.
+ */
+#define HXQ_KV8_BLOCK 64
+typedef struct hxq_kv8 {
+    int8_t* k;           /* [slots, nkv, max_len, D]                    */
+    int8_t* v;
+    float* k_scale;      /* [slots, nkv, max_len / HXQ_KV8_BLOCK]       */
+    float* v_scale;
+    void* k_tail;        /* bf16 [slots, nkv, HXQ_KV8_BLOCK, D]         */
+    void* v_tail;
+    int32_t slots, nkv, D, max_len;
+} hxq_kv8;
+
+/* hxq_rope_append for an 8-bit cache.  qkv[b, :] is one new token of the sequence in slot b at position pos[b]
+ * (int64 on the DEVICE; pos_stride 1: one per sequence, 0: pos[0] for all).  q and k are rotated (products and sum
+ * in fp64, rounded once to bf16), q goes to q_out, k and v to the tail, or, when their row is the 64th of its block,
+ * the block's codes and scales are written from the tail and that row.  A position < 0 or >= max_len leaves that
+ * sequence's q_out and cache as they are.  Rows of qkv and q_out 16-byte aligned, tables [max_len, D] too. */
+int hxq_rope_append_kv8(const hxq_kv8* cache, const void* qkv, int64_t ld_qkv, const int64_t* pos, int32_t pos_stride,
+                        const float* cos_table, const float* sin_table, void* q_out, int64_t ld_q, int32_t B, int32_t nq,
+                        hxq_stream_t stream);
+
+/* The same for S packed prompts: rows cu[s] .. cu[s + 1] - 1 of qkv (cu: int32 [S + 1] on the device, ascending, within
+ * 0 .. T) are the tokens of the sequence in slot s at positions pos[s], pos[s] + 1, ...; none of them longer than max_q
+ * (rows past that are not looked at).  pos[s] is the number of positions slot s holds already.  k_out (bf16 [T, ld_k],
+ * may be NULL) gets the rotated keys.  Rows that belong to no sequence, and positions from max_len on, are left out. */
+int hxq_rope_append_prompt_kv8(const hxq_kv8* cache, const void* qkv, int64_t ld_qkv, int32_t T, const int32_t* cu,
+                               int32_t S, int32_t max_q, const int64_t* pos, int32_t pos_stride, const float* cos_table,
+                               const float* sin_table, void* q_out, int64_t ld_q, void* k_out, int64_t ld_k, int32_t nq,
+                               hxq_stream_t stream);
+
+/* hxq_attn_decode over an 8-bit cache: positions 0 .. pos[b] of slot b, the finished blocks from their codes, the
+ * last one from the tail.  A position < 0 or >= max_len gives zeros.  nq / nkv <= 8.  workspace:
+ * hxq_attn_decode_kv8_workspace_bytes() of plain scratch (0: none needed). */
+size_t hxq_attn_decode_kv8_workspace_bytes(int32_t B, int32_t nq, int32_t nkv, int32_t D, int32_t max_len);
+int hxq_attn_decode_kv8(const hxq_kv8* cache, const void* q, int64_t ld_q, const int64_t* pos, int32_t pos_stride,
+                        void* out, int64_t ld_out, void* workspace, size_t workspace_bytes, int32_t B, int32_t nq,
+                        float scale, hxq_stream_t stream);
+
+/* Rows 0 .. len[s] - 1 (len_stride as pos_stride) of slots 0 .. S - 1 as bf16, scale * code rounded once; at most
+ * `rows` of them.  k_out, v_out: element (s, head, row, d) at s * ld_seq + head * ld_head + row * ld_row + d. */
+int hxq_kv8_rows(const hxq_kv8* cache, const int64_t* len, int32_t len_stride, int32_t S, int32_t rows, void* k_out,
+                 void* v_out, int64_t ld_seq, int64_t ld_head, int64_t ld_row, hxq_stream_t stream);
+
 /* out[b, i] = silu(gate[b, i]) * up[b, i], i < n (the MLP between gate/up and down). */
 int hxq_swiglu(const void* gate, const void* up, void* out, int32_t B, int32_t n, int64_t ld_gate,
                int64_t ld_up, int64_t ld_out, hxq_stream_t stream);
