@@ -46,6 +46,14 @@ class HxqKv8(C.Structure):
         + [(n, C.c_int32) for n in ("slots", "nkv", "D", "max_len")]
 
 
+class HxqAttn(C.Structure):
+    """Mirror of struct hxq_attn (include/hxq_b200.h)."""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out")] \
+        + [(n, C.c_int64) for n in ("q_tok", "q_head", "k_seq", "k_head", "k_row", "v_seq", "v_head", "v_row", "o_tok", "o_head")] \
+        + [(n, C.c_void_p) for n in ("cu_q", "cu_k", "k_len")] \
+        + [(n, C.c_int32) for n in ("Tq", "Tk", "S", "max_q", "nq", "nkv", "D", "causal")] + [("scale", C.c_float)]
+
+
 class HxqError(RuntimeError):
     def __init__(self, status: int, where: str):
         self.status = status
@@ -108,6 +116,8 @@ def lib() -> C.CDLL:
     L.hxq_attn_decode.argtypes = [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
                                   C.c_void_p, C.c_size_t, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                   C.c_float, C.c_void_p]
+    L.hxq_attn_prompt.restype = C.c_int
+    L.hxq_attn_prompt.argtypes = [C.POINTER(HxqAttn), C.c_void_p, C.c_void_p]
     K = C.POINTER(HxqKv8)
     L.hxq_rope_append_kv8.restype = C.c_int
     L.hxq_rope_append_kv8.argtypes = [K, C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,

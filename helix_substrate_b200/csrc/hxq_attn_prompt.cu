@@ -1,0 +1,540 @@
+// hxq_attn_prompt: attention of whole prompts - causal, grouped heads, packed sequences of different lengths, keys
+// and values packed like the queries or in the slabs of a cache (a later piece of a prompt over the rows before it).
+// The reference leaves this to the framework's attention inside its HF models
+// (helix_substrate/basin_runtime.py:281-330).
+//
+//     out[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h / G]) v[j, h / G],   j < count(i),
+//     count(i) = lk - lq + i + 1 (causal) or lk;  a row with count(i) <= 0 is zero.
+//
+// One CTA takes two tiles of 128 rows.  A row is (token, head of the group): the G query heads of a KV head share
+// its keys, so a tile spans 128 / G tokens, the causal edge wastes that much less, and a short prompt fills its
+// tiles G times better than with a head per CTA.  Per 128 keys and tile, all on the tensor cores (tcgen05):
+//
+//     S = Q K^T       both operands in shared memory (TMA, 128-byte swizzle), S in tensor memory
+//     P = 2^(scale' S - m)      one thread per row, in registers: running maximum m and sum; P goes back to tensor
+//                               memory as bf16, over S
+//     O += P V        A operand from tensor memory, V as it lies in memory (its rows are the contraction), O in
+//                     tensor memory for the whole row
+//
+// Roles: warps 0-3 and 4-7 are the two tiles' softmax (and epilogue), warp 8 feeds K and V through a ring of
+// 128-row tiles, warp 9 issues the MMAs (while one tile's softmax runs, the other tile's products do), warps 10 and 11
+// clean V tiles.  P is rounded to bf16, V's type (the MMA takes no other beside it): 2^-9 at most per weight, as much as
+// the output's own rounding; the sum that divides takes the weights before rounding.
+//
+// The reference point m moves only when the maximum has grown by more than 2^8: weights stay below 256, nothing
+// overflows, the result is the same, and O is rarely rescaled.
+//
+// What a row does not see must not reach it, whatever it holds: scores are replaced, not added to; a V tile with rows past
+// the sequence's end, or past what some row of the CTA sees, is looked at before its product: rows past the end become
+// zero, infinities and NaNs in rows that only some see are taken out and, in the epilogue, given back to the rows that do.
+//
+// Every mbarrier wait is bounded and raises the status word.  No multicast loads.
+
+#include <cuda.h>
+
+#include "hxq_common.cuh"
+#include "hxq_sm100.cuh"
+
+namespace hxq {
+namespace gemm {
+bool make_map_nd(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* base, const uint64_t* dims,
+                 const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle sw);
+}  // namespace gemm
+
+namespace attnp {
+
+constexpr int BM = 128;                     // rows of a tile
+constexpr int BN = 128;                     // keys of a step
+constexpr int NUM_THREADS = 384;
+constexpr int kMaxStages = 8;
+constexpr int kBarBytes = 512;
+
+template <int DP>
+struct Sizes {
+    static constexpr int kTile = BM * DP * 2;                 // a Q, K or V tile
+    static constexpr int kStages = DP == 128 ? 5 : 8;
+    static constexpr int kSmem = (2 + kStages) * kTile + kBarBytes + 1024;
+};
+
+struct Args {
+    const int32_t *cu_q, *cu_k;
+    const int64_t* k_len;
+    const __nv_bfloat16* v;
+    __nv_bfloat16* out;
+    int32_t* status;
+    int64_t v_seq, v_head, v_row, o_tok, o_head;
+    int32_t Tq, Tk, S, nkv, G, D, tpg, n_ct, causal;
+    float scale_log2;
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(sm100::smem_u32(bar)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(sm100::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+          "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t bf2(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// V's descriptor: the contraction's index (keys) is the row, 64 elements of N a 128-byte swizzled row, 8 rows 1024 B
+// apart, the next 64 elements of N a whole half tile on.
+__device__ __forceinline__ uint64_t make_desc_mn_sw128(uint32_t smem_addr, uint32_t half_bytes) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)(half_bytes >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+template <int DP>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v, const Args a) {
+    using Z = Sizes<DP>;
+    constexpr int NS = Z::kStages, TILE = Z::kTile, HALF = BM * 128;      // HALF: 64 of the dimensions of a tile
+    extern __shared__ char smem_raw[];
+    char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    char* ring = smem + 2 * TILE;
+    uint64_t* full = reinterpret_cast<uint64_t*>(ring + NS * TILE);     // [NS] a tile has landed, ready for its product
+    uint64_t* empty = full + kMaxStages;        // [NS] its products have retired
+    uint64_t* raw = empty + kMaxStages;         // [NS] a V tile that is to be cleaned has landed (full is not signalled) ...
+    uint64_t* clean = raw + kMaxStages;         // [NS] ... and has been cleaned
+    uint64_t* q_full = clean + kMaxStages;
+    uint64_t* s_full = q_full + 1;              // [2] S of a tile is complete (and the product before it)
+    uint64_t* p_ready = s_full + 2;             // [2] P is written, O is rescaled
+    uint64_t* o_done = p_ready + 2;             // [2] the last product of a tile has retired
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* odd_v = abort_flag + 1;       // a V tile held an infinity or a NaN that some row does not see
+    static_assert((4 * kMaxStages + 7) * 8 + 12 <= kBarBytes, "barrier area");
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    // ---- what this CTA is for (every thread works it out): longest work first
+    const int hs = blockIdx.x % (a.nkv * a.S), ct = a.n_ct - 1 - blockIdx.x / (a.nkv * a.S);
+    const int kvh = hs % a.nkv, s = hs / a.nkv;
+    int q0 = a.cu_q[s], q1 = a.cu_q[s + 1];
+    q0 = q0 < 0 ? 0 : q0;
+    q1 = q1 > a.Tq ? a.Tq : q1;
+    const int lq = q1 - q0, i0 = ct * 2 * a.tpg;
+    if (i0 >= lq) return;
+    int k0 = 0, lk;
+    if (a.cu_k != nullptr) {
+        int k1 = a.cu_k[s + 1];
+        k0 = a.cu_k[s];
+        k0 = k0 < 0 ? 0 : k0;
+        k1 = k1 > a.Tk ? a.Tk : k1;
+        lk = k1 > k0 ? k1 - k0 : 0;
+    } else {
+        const int64_t n = a.k_len[s];
+        lk = n < 0 ? 0 : (n > a.Tk ? a.Tk : (int)n);
+    }
+    auto count = [&](int i) {           // keys that token i sees
+        if (!a.causal || i >= lq) return lk;
+        const int n = lk - lq + i + 1;
+        return n > 0 ? n : 0;
+    };
+    auto steps = [&](int x) {           // key tiles of Q tile x
+        const int first = i0 + x * a.tpg;
+        if (first >= lq) return 0;
+        return (count(first + a.tpg < lq ? first + a.tpg - 1 : lq - 1) + BN - 1) / BN;
+    };
+    const int n0 = steps(0), n1 = steps(1), n = n0 > n1 ? n0 : n1;
+    const int seen_by_all = count(i0);          // keys that every token of this CTA sees
+    const int jc = seen_by_all / BN;            // V tiles from here on are looked at
+    const int rows = a.G * a.tpg;               // of a tile; the rest is zero
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < NS; ++i) {
+            sm100::mbar_init(&full[i], 1);
+            sm100::mbar_init(&empty[i], 1);
+            sm100::mbar_init(&raw[i], 1);
+            sm100::mbar_init(&clean[i], 2);
+        }
+        sm100::mbar_init(q_full, 1);
+        for (int x = 0; x < 2; ++x) {
+            sm100::mbar_init(&s_full[x], 1);
+            sm100::mbar_init(&p_ready[x], 4);
+            sm100::mbar_init(&o_done[x], 1);
+        }
+        *abort_flag = 0;
+        *odd_v = 0;
+        sm100::fence_barrier_init();
+        sm100::prefetch_tensormap(&map_q);
+        sm100::prefetch_tensormap(&map_k);
+        sm100::prefetch_tensormap(&map_v);
+    }
+    if (warp == 9) {
+        sm100::tmem_alloc(tmem_slot, 512);
+        sm100::tmem_relinquish();
+    }
+    // rows of the Q tiles that no token fills
+    for (int i = threadIdx.x; i < 2 * (DP / 64) * (BM - rows) * 8; i += NUM_THREADS) {
+        const int part = i / ((BM - rows) * 8), rem = i - part * (BM - rows) * 8;
+        *reinterpret_cast<uint4*>(smem + part * HALF + (rows + (rem >> 3)) * 128 + (rem & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    sm100::fence_proxy_async_smem();
+    sm100::tc_fence_before_sync();
+    __syncthreads();
+    sm100::tc_fence_after_sync();
+    // The next kernel may come in only now: one that took tensor memory before this CTA did would keep it waiting.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;       // S0 | S1 | O0 | O1, 128 columns each
+    bool ok = true;
+
+    if (warp == 8) {
+        // ------------------------------------------------------------ loads
+        if (lane == 0 && n > 0) {
+            sm100::mbar_arrive_expect_tx(q_full, 2u * (DP / 64) * (uint32_t)rows * 128u);
+            for (int x = 0; x < 2; ++x)
+                for (int h = 0; h < DP / 64; ++h)
+                    tma_load_3d(sm100::smem_u32(smem + x * TILE + h * HALF), &map_q, q_full, 64 * h, kvh * a.G, q0 + i0 + x * a.tpg);
+            int slot = 0;
+            uint32_t ph = 1;
+            for (int it = 0; it < 2 * n && ok; ++it) {
+                ok = sm100::mbar_wait(&empty[slot], ph, abort_flag);
+                if (!ok) break;
+                uint64_t* bar = (it & 1) && (it >> 1) >= jc ? &raw[slot] : &full[slot];
+                sm100::mbar_arrive_expect_tx(bar, TILE);
+                const uint32_t dst = sm100::smem_u32(ring + slot * TILE);
+                for (int h = 0; h < DP / 64; ++h)
+                    tma_load_4d(dst + h * HALF, (it & 1) ? &map_v : &map_k, bar, 64 * h, k0 + (it >> 1) * BN, kvh, a.cu_k != nullptr ? 0 : s);
+                if (++slot == NS) { slot = 0; ph ^= 1u; }
+            }
+        }
+    } else if (warp == 9) {
+        // ------------------------------------------------------------ MMAs
+        if (lane == 0 && n > 0) {
+            const uint32_t idesc_s = sm100::make_idesc_bf16(BM, BN);
+            const uint32_t idesc_o = sm100::make_idesc_bf16(BM, DP) | (1u << 16);      // B is N-major
+            int slot = 0;
+            uint32_t full_ph = 0, clean_ph = 0;       // parity of each slot's next phase: not every round signals both
+            auto next = [&]() { if (++slot == NS) slot = 0; };
+            auto wait = [&](uint64_t* bars, uint32_t& phases, int sl) {
+                const bool done = sm100::mbar_wait(&bars[sl], (phases >> sl) & 1u, abort_flag);
+                phases ^= 1u << sl;
+                return done;
+            };
+            auto scores = [&](int x, int sl) {
+                const uint32_t qa = sm100::smem_u32(smem + x * TILE), ka = sm100::smem_u32(ring + sl * TILE);
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k)
+                    sm100::umma_bf16(tmem + 128u * x, sm100::make_desc_k_sw128(qa + (k >> 2) * HALF) + 2 * (k & 3),
+                                     sm100::make_desc_k_sw128(ka + (k >> 2) * HALF) + 2 * (k & 3), idesc_s, k > 0);
+                sm100::umma_commit(&s_full[x]);
+            };
+            ok = sm100::mbar_wait(q_full, 0, abort_flag) && wait(full, full_ph, 0);
+            if (ok) {
+                sm100::tc_fence_after_sync();
+                if (n0 > 0) scores(0, 0);
+                if (n1 > 0) scores(1, 0);
+                sm100::umma_commit(&empty[0]);
+                next();
+            }
+            for (int j = 0; j < n && ok; ++j) {
+                const int v_slot = slot;
+                ok = j >= jc ? wait(clean, clean_ph, v_slot) : wait(full, full_ph, v_slot);
+                if (!ok) break;
+                sm100::tc_fence_after_sync();
+                next();
+                const int k_slot = slot;
+                bool have_k = false;
+                for (int x = 0; x < 2 && ok; ++x) {
+                    const int nx = x ? n1 : n0;
+                    if (j < nx) {
+                        ok = sm100::mbar_wait(&p_ready[x], (uint32_t)j & 1u, abort_flag);
+                        if (!ok) break;
+                        sm100::tc_fence_after_sync();
+                        const uint64_t dv = make_desc_mn_sw128(sm100::smem_u32(ring + v_slot * TILE), HALF);
+#pragma unroll
+                        for (int k = 0; k < BN / 16; ++k)
+                            umma_ts(tmem + 256u + 128u * x, tmem + 128u * x + 8 * k, dv + k * (2048 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+                        if (j == nx - 1) sm100::umma_commit(&o_done[x]);
+                    }
+                    if (j + 1 < nx) {
+                        if (!have_k) {
+                            ok = wait(full, full_ph, k_slot);
+                            if (!ok) break;
+                            sm100::tc_fence_after_sync();
+                            have_k = true;
+                        }
+                        scores(x, k_slot);       // over P, which the product before it reads: issued in order
+                    }
+                }
+                if (!ok) break;
+                sm100::umma_commit(&empty[v_slot]);
+                if (j + 1 < n) {
+                    sm100::umma_commit(&empty[k_slot]);
+                    next();
+                }
+            }
+        }
+    } else if (warp >= 10) {
+        // ------------------------------------------------------------ V tiles that some row sees only in part
+        uint32_t raw_ph = 0;
+        for (int j = jc; j < n; ++j) {
+            const int slot = (2 * j + 1) % NS;
+            ok = __all_sync(0xffffffffu, sm100::mbar_wait(&raw[slot], (raw_ph >> slot) & 1u, abort_flag));
+            raw_ph ^= 1u << slot;
+            if (!ok) break;
+            char* tile = ring + slot * TILE;
+            const int from = seen_by_all - j * BN > 0 ? seen_by_all - j * BN : 0;         // rows before it are everybody's
+            bool odd = false;
+            for (int i = (warp - 10) * 32 + lane; i < (DP / 64) * (BN - from) * 8; i += 64) {
+                const int part = i / ((BN - from) * 8), rem = i - part * (BN - from) * 8;
+                const int row = from + (rem >> 3);
+                uint4* p = reinterpret_cast<uint4*>(tile + part * HALF + row * 128 + (rem & 7) * 16);
+                if (j * BN + row >= lk) {
+                    *p = make_uint4(0u, 0u, 0u, 0u);
+                } else {
+                    uint4 w = *p;
+                    uint32_t* e = &w.x;
+                    bool hit = false;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {        // exponent of all ones
+                        if ((e[c] & 0x7f80u) == 0x7f80u) { e[c] &= 0xffff0000u; hit = true; }
+                        if ((e[c] & 0x7f800000u) == 0x7f800000u) { e[c] &= 0xffffu; hit = true; }
+                    }
+                    if (hit) { *p = w; odd = true; }
+                }
+            }
+            if (odd) *odd_v = 1;
+            sm100::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(&clean[slot]);
+        }
+    } else {
+        // ------------------------------------------------------------ softmax and epilogue: TMEM lane == row
+        const int x = warp >> 2, row = 32 * (warp & 3) + lane;
+        const int nx = x ? n1 : n0;
+        const int tok = i0 + x * a.tpg + row / a.G;
+        const int cnt = count(tok);
+        const int seen = nx > 0 ? count(i0 + x * a.tpg) : 0;        // keys that every row of the tile sees
+        const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        const uint32_t ts = t_lane + 128u * x, to = t_lane + 256u + 128u * x;
+        const float sc = a.scale_log2;
+        float ref = -INFINITY, l = 0.f;         // in units of S
+        for (int j = 0; j < nx; ++j) {
+            ok = __all_sync(0xffffffffu, sm100::mbar_wait(&s_full[x], (uint32_t)j & 1u, abort_flag));
+            if (!ok) break;
+            sm100::tc_fence_after_sync();
+            const bool edge = (j + 1) * BN > seen;
+            const int lim = cnt - j * BN;
+            float mx = -INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < BN; c += 32) {
+                uint32_t r[32];
+                sm100::tmem_ld_32x32(ts + c, r);
+                sm100::tmem_ld_wait();
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) if (c + e >= lim) r[e] = 0xff800000u;
+                }
+#pragma unroll
+                for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(r[e]));
+            }
+            // a new reference point where the maximum has grown by more than 2^8
+            const bool move = (mx - ref) * sc > 8.f;        // (-inf - -inf is NaN: no)
+            const float old = ref;
+            if (move) ref = mx;
+            if (__any_sync(0xffffffffu, move)) {
+                const float corr = move ? ex2((old - ref) * sc) : 1.f;
+                l *= corr;
+                if (j > 0) {
+#pragma unroll 1
+                    for (int c = 0; c < DP; c += 16) {
+                        uint32_t r[16];
+                        asm volatile(
+                            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                              "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(to + c) : "memory");
+                        sm100::tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * corr);
+                        tmem_st_32x16(to + c, r);
+                    }
+                }
+            }
+            // 2^(S sc - ref sc) in one multiply-add: the rounding of ref sc shifts a whole row and divides out, unless
+            // scores are so large that it is itself large; then the difference is taken first
+            const bool far = __any_sync(0xffffffffu, ref != -INFINITY && fabsf(ref * sc) > 65536.f);
+            const float bias = ref == -INFINITY || far ? 0.f : -ref * sc;
+            const float first = ref == -INFINITY ? 0.f : ref;
+#pragma unroll 1
+            for (int c = 0; c < BN; c += 32) {
+                uint32_t r[32], p[16];
+                sm100::tmem_ld_32x32(ts + c, r);
+                sm100::tmem_ld_wait();
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) if (c + e >= lim) r[e] = 0xff800000u;
+                }
+                if (far) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) - first);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float p0 = ex2(fmaf(__uint_as_float(r[2 * e]), sc, bias)), p1 = ex2(fmaf(__uint_as_float(r[2 * e + 1]), sc, bias));
+                    l += p0 + p1;
+                    p[e] = bf2(p0, p1);
+                }
+                tmem_st_32x16(ts + c / 2, p);
+            }
+            tmem_st_wait();
+            sm100::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(&p_ready[x]);
+        }
+        if (ok && nx > 0) ok = __all_sync(0xffffffffu, sm100::mbar_wait(&o_done[x], 0, abort_flag));
+        if (ok) {
+            sm100::tc_fence_after_sync();
+            const bool live = row < rows && tok < lq;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            __nv_bfloat16* dst = a.out + (int64_t)(q0 + tok) * a.o_tok + (int64_t)(kvh * a.G + row % a.G) * a.o_head;
+            const bool odd = nx > 0 && *odd_v != 0;
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 32) {
+                uint32_t r[32];
+                if (nx > 0) {
+                    sm100::tmem_ld_32x32(to + c, r);
+                    sm100::tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) r[e] = 0u;
+                }
+                if (live) {
+                    float f[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) f[e] = inv == 0.f ? 0.f : __uint_as_float(r[e]) * inv;
+                    if (odd) {      // infinities and NaNs that were taken out of V, back to the rows that see them
+                        const __nv_bfloat16* vp = a.v + (a.cu_k != nullptr ? 0 : (int64_t)s * a.v_seq) + (int64_t)kvh * a.v_head + (int64_t)k0 * a.v_row;
+                        for (int kk = seen_by_all; kk < cnt; ++kk)
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                const float y = c + e < a.D ? __bfloat162float(vp[(int64_t)kk * a.v_row + c + e]) : 0.f;
+                                if (!(fabsf(y) <= 3.4e38f)) f[e] += y;
+                            }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c + 8 * e < a.D)
+                            *reinterpret_cast<uint4*>(dst + c + 8 * e) = make_uint4(bf2(f[8 * e], f[8 * e + 1]), bf2(f[8 * e + 2], f[8 * e + 3]),
+                                                                                   bf2(f[8 * e + 4], f[8 * e + 5]), bf2(f[8 * e + 6], f[8 * e + 7]));
+                }
+            }
+        }
+    }
+
+    if (!ok && (warp == 8 || warp == 9)) {     // gave up: let copies and products already in flight land
+        const long long t0 = clock64();
+        while (clock64() - t0 < 20000000LL) { }
+    }
+    sm100::tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 9) {
+        sm100::tc_fence_after_sync();
+        sm100::tmem_dealloc(tmem, 512);
+    }
+    if (threadIdx.x == 0 && *abort_flag != 0 && a.status != nullptr) atomicExch(a.status, HXQ_E_TIMEOUT);
+}
+
+// ---- host side ---------------------------------------------------------------------
+
+template <int DP>
+static int run(const hxq_attn* p, int32_t* status, cudaStream_t stream) {
+    using Z = Sizes<DP>;
+    Args a;
+    a.cu_q = p->cu_q; a.cu_k = p->cu_k; a.k_len = p->k_len;
+    a.v = reinterpret_cast<const __nv_bfloat16*>(p->v);
+    a.out = reinterpret_cast<__nv_bfloat16*>(p->out);
+    a.status = status;
+    a.v_seq = p->v_seq; a.v_head = p->v_head; a.v_row = p->v_row; a.o_tok = p->o_tok; a.o_head = p->o_head;
+    a.Tq = p->Tq; a.Tk = p->Tk; a.S = p->S; a.nkv = p->nkv; a.G = p->nq / p->nkv; a.D = p->D; a.causal = p->causal != 0;
+    a.tpg = BM / a.G;
+    a.scale_log2 = p->scale * 1.4426950408889634f;
+    const int64_t max_q = p->max_q < p->Tq ? p->max_q : p->Tq;
+    a.n_ct = (int)((max_q + 2 * a.tpg - 1) / (2 * a.tpg));
+    const int64_t grid = (int64_t)a.n_ct * a.nkv * a.S;
+    if (grid > 0x7fffffffLL) return HXQ_E_SHAPE;
+
+    CUtensorMap mq, mk, mv;
+    // (the stride of a dimension of one element is never used, but has to be a valid one)
+    auto st = [](int64_t elements, int64_t extent) { return extent > 1 ? (uint64_t)elements * 2 : (uint64_t)16; };
+    const uint64_t qd[3] = {(uint64_t)p->D, (uint64_t)p->nq, (uint64_t)p->Tq}, qs[2] = {st(p->q_head, p->nq), st(p->q_tok, p->Tq)};
+    const uint32_t qb[3] = {64, (uint32_t)a.G, (uint32_t)a.tpg};
+    const uint64_t slabs = p->cu_k ? 1 : (uint64_t)p->S;
+    const uint64_t kd[4] = {(uint64_t)p->D, (uint64_t)p->Tk, (uint64_t)p->nkv, slabs};
+    const uint64_t ks[3] = {st(p->k_row, p->Tk), st(p->k_head, p->nkv), st(p->k_seq, (int64_t)slabs)};
+    const uint64_t vs[3] = {st(p->v_row, p->Tk), st(p->v_head, p->nkv), st(p->v_seq, (int64_t)slabs)};
+    const uint32_t kb[4] = {64, BN, 1, 1};
+    const CUtensorMapDataType dt = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    if (!gemm::make_map_nd(&mq, dt, 3, p->q, qd, qs, qb, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !gemm::make_map_nd(&mk, dt, 4, p->k, kd, ks, kb, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !gemm::make_map_nd(&mv, dt, 4, p->v, kd, vs, kb, CU_TENSOR_MAP_SWIZZLE_128B))
+        return HXQ_E_DEVICE;
+    static bool attr_set[64] = {false};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return HXQ_E_DEVICE;
+    if (!attr_set[dev]) {
+        if (cudaFuncSetAttribute(attn_prompt_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::kSmem) != cudaSuccess) return HXQ_E_DEVICE;
+        attr_set[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.dynamicSmemBytes = Z::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attn_prompt_kernel<DP>, mq, mk, mv, a) == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
+}
+
+}  // namespace attnp
+}  // namespace hxq
+
+extern "C" int hxq_attn_prompt(const hxq_attn* p, int32_t* status_word, hxq_stream_t stream) {
+    if (!p || !p->q || !p->k || !p->v || !p->out || !p->cu_q || (!p->cu_k) == (!p->k_len)) return HXQ_E_ARG;
+    if (p->Tq < 0 || p->Tk < 0 || p->S <= 0 || p->max_q < 0 || !(p->scale > 0.f) || !(p->scale <= 3.4e38f)) return HXQ_E_ARG;
+    if (p->nq <= 0 || p->nkv <= 0 || p->nq % p->nkv != 0 || p->nq / p->nkv > 64) return HXQ_E_SHAPE;
+    if (p->D < 8 || p->D > 128 || p->D % 8 != 0) return HXQ_E_SHAPE;
+    const int64_t strides[10] = {p->q_tok, p->q_head, p->k_seq, p->k_head, p->k_row, p->v_seq, p->v_head, p->v_row, p->o_tok, p->o_head};
+    for (int64_t s : strides)
+        if (s < 0 || s >= (int64_t(1) << 38) || s % 8 != 0) return HXQ_E_ALIGN;
+    if (!hxq::aligned_to(p->q, 16) || !hxq::aligned_to(p->k, 16) || !hxq::aligned_to(p->v, 16) || !hxq::aligned_to(p->out, 16)) return HXQ_E_ALIGN;
+    if (p->Tq == 0 || p->max_q == 0) return HXQ_OK;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    return p->D <= 64 ? hxq::attnp::run<64>(p, status_word, st) : hxq::attnp::run<128>(p, status_word, st);
+}

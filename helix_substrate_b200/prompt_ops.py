@@ -1,0 +1,67 @@
+"""Attention of whole prompts: causal, grouped heads, packed sequences of different lengths, keys and values
+packed like the queries or in a cache's slabs.  A thin bf16 wrapper over the C ABI, one launch; no counterpart in
+the reference, whose HF models use the framework's attention (helix_substrate/basin_runtime.py:281-330)."""
+
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .kv8 import _call, _ints
+from .packed import _status_word
+
+
+def _heads(t: torch.Tensor, name: str, dev: torch.device, shape: tuple) -> None:
+    if not (t.dtype is torch.bfloat16 and t.device == dev and t.is_cuda and t.ndim == len(shape) and t.stride(-1) == 1
+            and all(w is None or n == w for n, w in zip(t.shape, shape))):
+        raise TypeError(f"{name}: expected a CUDA bf16 tensor {tuple('*' if w is None else w for w in shape)} on {dev}, contiguous along "
+                        f"its last dimension, got {t.dtype} {tuple(t.shape)} {t.stride()} on {t.device}")
+
+
+def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, cu_q: torch.Tensor, max_q: int,
+                scale: float, *, cu_k: Optional[torch.Tensor] = None, k_len: Optional[torch.Tensor] = None,
+                causal: bool = True) -> torch.Tensor:
+    """Sequence s has the queries ``q[cu_q[s]: cu_q[s + 1]]`` of q [T, nq, D] (int32 offsets on the device, none longer
+    than ``max_q``).  Its keys and values are the same rows of k, v [T, nkv, D]; or rows ``cu_k[s]`` .. of k, v [Tk, nkv,
+    D]; or rows 0 .. ``k_len[s] - 1`` (int64) of slab s of k, v [S, nkv, rows, D].  Causal attention is aligned at the end:
+    with more keys than queries the queries are the last ones.  A query that sees no key gets zeros, rows of ``out``
+    [T, nq, D] of no sequence are left as they are, and what a query does not see may hold anything.  q, k, v and out may be
+    views (strides of whole 16 bytes)."""
+    dev = q.device
+    slabs = k_len is not None
+    if slabs and cu_k is not None:
+        raise ValueError("keys lie packed (cu_k) or in slabs (k_len), not both")
+    _heads(q, "q", dev, (None, None, None))
+    T, nq, D = q.shape
+    S = cu_q.shape[0] - 1 if cu_q.ndim == 1 else -1
+    if S < 1 or max_q < 0:
+        raise ValueError(f"cu_q of shape {tuple(cu_q.shape)}, max_q {max_q}")
+    _ints(cu_q, "cu_q", dev, torch.int32, S + 1)
+    _heads(k, "k", dev, (S, None, None, D) if slabs else (None, None, D))
+    _heads(v, "v", dev, tuple(k.shape))
+    _heads(out, "out", dev, (T, nq, D))
+    nkv, rows = (k.shape[1], k.shape[2]) if slabs else (k.shape[1], k.shape[0])
+    if nkv < 1 or nq % nkv:
+        raise ValueError(f"{nq} query heads over {nkv} KV heads")
+    if slabs:
+        _ints(k_len, "k_len", dev, torch.int64, S)
+    elif cu_k is not None:
+        _ints(cu_k, "cu_k", dev, torch.int32, S + 1)
+    elif rows != T:
+        raise ValueError(f"{T} rows of q and {rows} of k: cu_k says where each sequence's keys lie")
+    else:
+        cu_k = cu_q
+    if T == 0 or max_q == 0:
+        return out
+    if rows == 0:
+        raise ValueError("k and v have no rows")
+    ks, vs = k.stride(), v.stride()
+    k3, v3 = ((ks[0], ks[1], ks[2]), (vs[0], vs[1], vs[2])) if slabs else ((0, ks[1], ks[0]), (0, vs[1], vs[0]))
+    p = _lib.HxqAttn(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), *k3, *v3, out.stride(0),
+                     out.stride(1), cu_q.data_ptr(), None if slabs else cu_k.data_ptr(), k_len.data_ptr() if slabs else None,
+                     T, rows, S, min(max_q, T), nq, nkv, D, int(causal), scale)
+    _call(dev, "hxq_attn_prompt", C.byref(p), _status_word(dev).data_ptr())
+    return out

@@ -237,6 +237,32 @@ int hxq_attn_decode(const void* q, int64_t ld_q, const void* k_cache, const void
 int32_t hxq_attn_decode_span(int32_t B, int32_t nkv, int32_t max_len);
 
 /*
+ * Attention of whole prompts (no counterpart in the reference, whose HF models use the framework's:
+ * helix_substrate/basin_runtime.py:281-330), bf16: for sequence s, queries are rows cu_q[s] .. cu_q[s + 1] - 1 of
+ * q [Tq, nq, D]; its lk keys and values are rows cu_k[s] .. cu_k[s + 1] - 1 of k, v [Tk, nkv, D] (packed), or rows
+ * 0 .. k_len[s] - 1 of slab s of k, v [S, nkv, Tk, D] (a cache).  causal: query i of lq sees keys 0 .. lk - lq + i, so the
+ * last query sees all; a query that sees none gets zeros.  What a query does not see may hold anything, NaN too.
+ * cu_q, cu_k (int32 [S + 1], ascending) and k_len (int64 [S]) are DEVICE arrays, exactly one of cu_k and k_len given;
+ * max_q: no sequence has more queries (those past it are not computed).  Rows of out that belong to no sequence are
+ * left as they are.  Strides in elements, multiples of 8; pointers 16-byte aligned; D % 8 == 0, 8 <= D <= 128;
+ * nq / nkv <= 64; scale > 0.  status_word as in hxq_gemm.
+ */
+typedef struct hxq_attn {
+    const void *q, *k, *v;
+    void* out;                              /* [Tq, nq, D] by o_tok, o_head          */
+    int64_t q_tok, q_head;
+    int64_t k_seq, k_head, k_row;           /* k_seq, v_seq: slabs only              */
+    int64_t v_seq, v_head, v_row;
+    int64_t o_tok, o_head;
+    const int32_t* cu_q;
+    const int32_t* cu_k;
+    const int64_t* k_len;
+    int32_t Tq, Tk, S, max_q, nq, nkv, D, causal;
+    float scale;
+} hxq_attn;
+int hxq_attn_prompt(const hxq_attn* p, int32_t* status_word, hxq_stream_t stream);
+
+/*
  * ---- key/value cache held in 8 bits (no counterpart in the reference, which keeps the framework's
  * 16-bit cache: helix_substrate/basin_runtime.py:358-445) ----
  * Positions form blocks of HXQ_KV8_BLOCK.  A finished block of one (sequence, KV head) holds int8 codes and

@@ -1,0 +1,220 @@
+"""Attention of whole prompts against plain 64-bit arithmetic: packed sequences, slabs of a cache, lengths around
+the tiles, grouped heads that do not divide them, rows that see nothing, NaNs where nobody looks."""
+
+import pytest
+import torch
+
+from conftest import rel_l2
+from kv8_ref import attention
+
+pytestmark = pytest.mark.gpu
+
+# Each weight is rounded to bf16 (2^-9 of it at most half an ulp: eps / 2 = 2^-8 as a bound), the output once more: the two
+# together stay below 2^-7; rms over random mantissas, sqrt(2) * 2^-9.2.  Bound of rel-L2: 2^-8.
+TOL = 2.0 ** -8
+
+
+def _dev():
+    return torch.device("cuda:0")
+
+
+def _want(q, k, v, scale, causal):
+    lq, lk = q.shape[0], k.shape[0]
+    seen = torch.ones(lq, lk, dtype=torch.bool, device=q.device)
+    if causal:
+        seen = seen.tril(lk - lq)
+    return attention(q.transpose(0, 1), k.transpose(0, 1), v.transpose(0, 1), scale, seen).transpose(0, 1)
+
+
+def _compare(got, want, what):
+    nan = want.isnan()
+    assert torch.equal(nan, got.isnan()), what
+    inf = want.isinf()
+    assert torch.equal(got[inf], want[inf].to(got.dtype)), what
+    fine = ~(nan | inf)
+    got, want = got.double()[fine], want[fine]
+    if not want.numel() or not bool(want.any()):
+        assert not bool(got.any()), what
+        return
+    assert rel_l2(got.cpu(), want.cpu()) < TOL, (what, rel_l2(got.cpu(), want.cpu()))
+    big = (got - want).abs() / want.abs().clamp_min(float(want.pow(2).mean().sqrt()))
+    assert float(big.max()) < 2.0 ** -5, (what, float(big.max()))
+
+
+@pytest.mark.parametrize("nq,nkv,D", [(28, 4, 128), (4, 2, 64), (40, 8, 128), (3, 3, 128), (8, 1, 64), (5, 1, 80), (6, 2, 16), (64, 1, 128), (9, 3, 72), (2, 1, 8)])
+@pytest.mark.parametrize("lens", [[1], [37, 0, 1, 256, 129], [700, 3], [127, 128, 300]])
+def test_packed(nq, nkv, D, lens):
+    """Views of one projection's output, sequences of every kind, two rows that belong to none."""
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, T = _dev(), sum(lens)
+    g = torch.Generator(device=dev).manual_seed(T + nq)
+    qkv = torch.randn(T + 2, nq + 2 * nkv, D, device=dev, generator=g).bfloat16()
+    qkv[T:] = float("nan")
+    q, k, v = qkv.split([nq, nkv, nkv], 1)
+    cu = [sum(lens[:s]) for s in range(len(lens) + 1)]
+    for causal in (True, False):
+        out = torch.full((T + 2, nq, D), 7.0, device=dev, dtype=torch.bfloat16)
+        attn_prompt(q, k, v, out, torch.tensor(cu, dtype=torch.int32, device=dev), max(lens), D ** -0.5, causal=causal)
+        for a, b in zip(cu, cu[1:]):
+            if b > a:
+                _compare(out[a:b], _want(q[a:b], k[a:b], v[a:b], D ** -0.5, causal), (causal, a, b))
+        assert bool((out[T:] == 7).all())
+        again = torch.full_like(out, 7.0)
+        attn_prompt(q, k, v, again, torch.tensor(cu, dtype=torch.int32, device=dev), max(lens) + 500, D ** -0.5, causal=causal)
+        assert torch.equal(out, again), "the same bits, whatever max_q"
+
+
+@pytest.mark.parametrize("nq,nkv,D", [(28, 4, 128), (4, 2, 64), (3, 1, 40)])
+@pytest.mark.parametrize("lens,keys", [([5, 64, 1, 130], [1000, 64, 513, 131]), ([300, 10], [299, 4]), ([20], [0]), ([256, 3], [2048, 1])])
+def test_slabs_and_more_or_fewer_keys_than_queries(nq, nkv, D, lens, keys):
+    """Keys in a cache's slabs, rows past each length NaN; fewer keys than queries leave the first queries nothing to see."""
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, T, S, rows = _dev(), sum(lens), len(lens), max(keys) + 70
+    g = torch.Generator(device=dev).manual_seed(T + D)
+    q = torch.randn(T, nq + 1, D, device=dev, generator=g).bfloat16()[:, :nq]
+    kc = torch.randn(S, nkv, rows, D, device=dev, generator=g).bfloat16()
+    vc = torch.randn(S, nkv + 2, rows, D, device=dev, generator=g).bfloat16()[:, 1: nkv + 1]
+    for s, n in enumerate(keys):
+        kc[s, :, n:] = float("nan")
+        vc[s, :, n:] = float("inf")
+    cu = [sum(lens[:s]) for s in range(S + 1)]
+    cu_d, len_d = torch.tensor(cu, dtype=torch.int32, device=dev), torch.tensor(keys, device=dev)
+    for causal in (True, False):
+        out = torch.empty(T, nq, D, device=dev, dtype=torch.bfloat16)
+        attn_prompt(q, kc, vc, out, cu_d, max(lens), 0.3, k_len=len_d, causal=causal)
+        for s, (a, b) in enumerate(zip(cu, cu[1:])):
+            n = keys[s]
+            _compare(out[a:b], _want(q[a:b], kc[s, :, :n].transpose(0, 1), vc[s, :, :n].transpose(0, 1), 0.3, causal), (causal, s))
+        # the same keys, packed
+        if sum(keys):
+            kp = torch.cat([kc[s, :, :n].transpose(0, 1) for s, n in enumerate(keys)]).contiguous()
+            vp = torch.cat([vc[s, :, :n].transpose(0, 1) for s, n in enumerate(keys)]).contiguous()
+            cu_k = torch.tensor([sum(keys[:s]) for s in range(S + 1)], dtype=torch.int32, device=dev)
+            packed = torch.empty_like(out)
+            attn_prompt(q, kp, vp, packed, cu_d, max(lens), 0.3, cu_k=cu_k, causal=causal)
+            assert torch.equal(out, packed)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("at", [0, 5, 127, 128, 200, 299])
+def test_infinities_and_nans_reach_only_the_rows_that_see_them(D, at):
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, nq, nkv, T = _dev(), 14, 2, 300
+    g = torch.Generator(device=dev).manual_seed(at)
+    q, k, v = (torch.randn(T, n, D, device=dev, generator=g).bfloat16() for n in (nq, nkv, nkv))
+    v[at, 0, 3], v[at, 0, 4], v[at, 1, 0] = float("inf"), float("nan"), float("-inf")
+    cu = torch.tensor([0, T], dtype=torch.int32, device=dev)
+    out = torch.empty(T, nq, D, device=dev, dtype=torch.bfloat16)
+    attn_prompt(q, k, v, out, cu, T, D ** -0.5)
+    _compare(out, _want(q, k, v, D ** -0.5, True), at)
+    v.nan_to_num_(0.0, 0.0, 0.0)
+    k[at, 1, 2] = float("nan")
+    attn_prompt(q, k, v, out, cu, T, D ** -0.5)
+    want = _want(q, k, v, D ** -0.5, True)
+    want[at:, 7:] = float("nan")
+    _compare(out, want, ("key", at))
+
+
+@pytest.mark.parametrize("case", ["growing", "peaked", "huge scores", "equal", "lowest"])
+def test_running_softmax(case):
+    """Scores that grow along the sequence (the reference point moves at every tile), one key that takes all, scores of 1e5, equal
+    keys, and rows whose scores are the type's lowest."""
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, nq, nkv, T, D = _dev(), 6, 2, 1000, 64
+    g = torch.Generator(device=dev).manual_seed(1)
+    q, k, v = (torch.randn(T, n, D, device=dev, generator=g) for n in (nq, nkv, nkv))
+    scale = D ** -0.5
+    if case == "growing":
+        q, k = q.abs(), k.abs() * torch.linspace(0.1, 12, T, device=dev)[:, None, None]
+    elif case == "peaked":
+        k[333] = 20 * k[333].sign()
+        q = 4 * k[333, :1].sign() + 0.1 * q
+    elif case == "huge scores":
+        q, k = q * 200, k * 200
+    elif case == "equal":
+        k = torch.ones_like(k)
+    else:
+        q, k, scale = torch.full_like(q, 1e18), torch.full_like(k, -3e18), 1.0
+    q, k, v = q.bfloat16(), k.bfloat16(), v.bfloat16()
+    out = torch.empty(T, nq, D, device=dev, dtype=torch.bfloat16)
+    attn_prompt(q, k, v, out, torch.tensor([0, T], dtype=torch.int32, device=dev), T, scale)
+    _compare(out, _want(q, k, v, scale, True), case)
+
+
+def test_offsets_past_32_bits_and_a_stream_of_its_own():
+    """Slabs whose second one lies past 2^31 elements; a call on another stream than the one the inputs were made on."""
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, nq, nkv, D, rows = _dev(), 4, 2, 128, 1 << 22
+    kc = torch.empty(3, nkv, rows, D, device=dev, dtype=torch.bfloat16)
+    vc = torch.empty_like(kc)
+    g = torch.Generator(device=dev).manual_seed(4)
+    n = 200
+    for c in (kc, vc):
+        c[:, :, :n] = torch.randn(3, nkv, n, D, device=dev, generator=g).bfloat16()
+    q = torch.randn(3 * 40, nq, D, device=dev, generator=g).bfloat16()
+    cu = torch.tensor([0, 40, 80, 120], dtype=torch.int32, device=dev)
+    out = torch.empty_like(q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        attn_prompt(q, kc, vc, out, cu, 40, D ** -0.5, k_len=torch.tensor([n, n, n], device=dev))
+    torch.cuda.current_stream().wait_stream(side)
+    for s in range(3):
+        _compare(out[40 * s: 40 * s + 40], _want(q[40 * s: 40 * s + 40], kc[s, :, :n].transpose(0, 1), vc[s, :, :n].transpose(0, 1), D ** -0.5, True), s)
+
+
+def test_captured_and_replayed():
+    """Lengths are read on the device: a captured call follows them."""
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, nq, nkv, D, T = _dev(), 28, 4, 128, 400
+    g = torch.Generator(device=dev).manual_seed(6)
+    q, k, v = (torch.randn(T, n, D, device=dev, generator=g).bfloat16() for n in (nq, nkv, nkv))
+    cu = torch.tensor([0, 100, T], dtype=torch.int32, device=dev)
+    out = torch.zeros(T, nq, D, device=dev, dtype=torch.bfloat16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        attn_prompt(q, k, v, out, cu, T, D ** -0.5)
+        side.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            attn_prompt(q, k, v, out, cu, T, D ** -0.5)
+    for mid in (100, 0, 333):
+        cu[1] = mid
+        graph.replay()
+        want = torch.zeros_like(out)
+        attn_prompt(q, k, v, want, cu, T, D ** -0.5)
+        assert torch.equal(out, want)
+
+
+def test_prompt_refuses():
+    from helix_substrate_b200 import _lib
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, T, nq, nkv, D = _dev(), 10, 4, 2, 64
+    bf = lambda *s: torch.zeros(*s, device=dev, dtype=torch.bfloat16)       # noqa: E731
+    q, k, v, out = bf(T, nq, D), bf(T, nkv, D), bf(T, nkv, D), bf(T, nq, D)
+    cu = torch.tensor([0, T], dtype=torch.int32, device=dev)
+    n1 = torch.tensor([5], device=dev)
+    bad = [
+        (TypeError, lambda: attn_prompt(q.half(), k, v, out, cu, T, 0.1)),
+        (TypeError, lambda: attn_prompt(q.cpu(), k, v, out, cu, T, 0.1)),
+        (TypeError, lambda: attn_prompt(q, k.transpose(0, 2), v, out, cu, T, 0.1)),
+        (TypeError, lambda: attn_prompt(q, k, v[:, :1], out, cu, T, 0.1)),
+        (TypeError, lambda: attn_prompt(q, k, v, out[:5], cu, T, 0.1)),
+        (TypeError, lambda: attn_prompt(q, k, v, out, cu.long(), T, 0.1)),
+        (TypeError, lambda: attn_prompt(q, k, v, out, cu, T, 0.1, k_len=n1)),
+        (ValueError, lambda: attn_prompt(q, k, v, out, cu, T, 0.1, cu_k=cu, k_len=n1)),
+        (ValueError, lambda: attn_prompt(q, k[:5], v[:5], out, cu, T, 0.1)),
+        (ValueError, lambda: attn_prompt(q[:, :3], k, v, out[:, :3], cu, T, 0.1)),
+        (ValueError, lambda: attn_prompt(q, k, v, out, cu[:1], T, 0.1)),
+        (ValueError, lambda: attn_prompt(q, k, v, out, cu, -1, 0.1)),
+        (_lib.HxqError, lambda: attn_prompt(q, k, v, out, cu, T, 0.0)),
+        (_lib.HxqError, lambda: attn_prompt(q, k, v, out, cu, T, float("nan"))),
+        (_lib.HxqError, lambda: attn_prompt(bf(T, nq, 136), bf(T, nkv, 136), bf(T, nkv, 136), bf(T, nq, 136), cu, T, 0.1)),
+        (_lib.HxqError, lambda: attn_prompt(bf(T, nq, D + 4)[..., :D], k, v, out, cu, T, 0.1)),
+        (_lib.HxqError, lambda: attn_prompt(bf(T, 65, D), bf(T, 1, D), bf(T, 1, D), bf(T, 65, D), cu, T, 0.1)),
+    ]
+    for kind, call in bad:
+        with pytest.raises(kind):
+            call()
+    assert attn_prompt(q[:0], k[:0], v[:0], out[:0], torch.zeros(2, dtype=torch.int32, device=dev), 0, 0.1).shape[0] == 0
