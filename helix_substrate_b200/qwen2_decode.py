@@ -13,6 +13,10 @@ ranks outnumber the KV heads (Qwen2.5-7B on 8 GPUs: 28 query / 4 KV heads) each 
 on two ranks and its seven query heads are dealt 4 + 3; the MLP is cut on whole 128-column
 affine groups.
 
+``prompt_attn="fused"`` runs the prompt's attention as one kernel (prompt_ops) instead of the framework's operator;
+``kv_bits=8`` holds the cache in 8 bits with a scale per 64 positions and head (kv8), the prompt's attention
+then being the fused one.
+
 Weights are random-init (N(0, 0.02)) and compressed on the GPU; lm_head and the
 embedding stay dense bf16, as in the reference's policy (tensor_policy.py:199-208).
 """
@@ -26,7 +30,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import decode_ops
+from . import decode_ops, kv8, prompt_ops
 from .helix_linear import HelixLinear
 from .hxq_writer_gpu import compress_weight
 from .tp import head_partition, shard_bounds, take_cols, take_rows
@@ -177,8 +181,15 @@ class Qwen2HxqDecoder(nn.Module):
 
     def __init__(self, shp: Qwen2Shape, device, batch: int, max_len: int, group_size: int = 128,
                  rank: int = 0, world: int = 1, group=None, fuse_proj: bool = True, p2p_allreduce: bool = False,
-                 build: str = "local"):
+                 build: str = "local", kv_bits: int = 16, prompt_attn: str = "torch"):
         super().__init__()
+        if kv_bits not in (8, 16):
+            raise ValueError(f"kv_bits must be 8 or 16, got {kv_bits!r}")
+        if prompt_attn not in ("torch", "fused"):
+            raise ValueError(f"prompt_attn must be 'torch' or 'fused', got {prompt_attn!r}")
+        self.kv_bits, self.prompt_attn = kv_bits, ("fused" if kv_bits == 8 else prompt_attn)
+        if kv_bits == 8:
+            max_len = (max_len + kv8.BLOCK - 1) // kv8.BLOCK * kv8.BLOCK
         self.shp, self.device, self.world, self.group = shp, device, world, group
         self.p2p = bool(p2p_allreduce) and world > 1   # one-shot peer-memory sum instead of NCCL in the fused step
         self.layers = nn.ModuleList(Qwen2Layer(shp, i, device, group_size, rank, world, fuse_proj, build)
@@ -188,8 +199,12 @@ class Qwen2HxqDecoder(nn.Module):
         self.lm_head = (torch.randn(shp.vocab, shp.hidden, device=device, generator=g) * 0.02).bfloat16()
         self.norm = torch.ones(shp.hidden, device=device, dtype=torch.bfloat16)
         n_kv = self.layers[0].n_kv
-        self.k_cache = torch.zeros(shp.layers, batch, n_kv, max_len, shp.head_dim, device=device, dtype=torch.bfloat16)
-        self.v_cache = torch.zeros_like(self.k_cache)
+        if kv_bits == 8:
+            self.k_cache = self.v_cache = None
+            self.kv8 = [kv8.Kv8Cache.empty(batch, n_kv, max_len, shp.head_dim, device) for _ in range(shp.layers)]
+        else:
+            self.k_cache = torch.zeros(shp.layers, batch, n_kv, max_len, shp.head_dim, device=device, dtype=torch.bfloat16)
+            self.v_cache = torch.zeros_like(self.k_cache)
         inv = 1.0 / (shp.rope_theta ** (torch.arange(0, shp.head_dim, 2, device=device, dtype=torch.float32)
                                         / shp.head_dim))
         ang = torch.arange(max_len, device=device, dtype=torch.float32)[:, None] * inv[None, :]
@@ -215,7 +230,8 @@ class Qwen2HxqDecoder(nn.Module):
                        attn_len: Optional[int]) -> torch.Tensor:
         """ids [B, T]; positions [T] (absolute); the new K/V go to cache rows
         ``cache_rows`` [T]; attention spans cache[:attn_len] (None = whole cache
-        with a position mask, which is what the captured one-token step uses)."""
+        with a position mask, which is what the captured one-token step uses).  With fused prompt
+        attention (always with an 8-bit cache) positions and cache rows are consecutive and the same."""
         return _drive(self.blocks_tokens(ids, positions, cache_rows, attn_len), lambda part, key, *_: self._allreduce(part))
 
     def blocks_tokens(self, ids: torch.Tensor, positions: torch.Tensor, cache_rows: torch.Tensor,
@@ -226,8 +242,13 @@ class Qwen2HxqDecoder(nn.Module):
         D = self.shp.head_dim
         h = self.embed[ids]
         cos, sin = self.cos[positions][None, None], self.sin[positions][None, None]
+        fused = self._prompt_plan(B, T, positions, cache_rows, attn_len) if self.prompt_attn == "fused" else None
         for li, L in enumerate(self.layers):
             x = self._rms(h, L.ln1)
+            if fused is not None:
+                h = h + (yield L.o_proj(self._prompt_attention(li, L, x, cos, sin, fused)), "d1")
+                h = h + (yield self._mlp(L, self._rms(h, L.ln2)), "d2")
+                continue
             if L.fused:
                 q, k, v = L.qkv_proj(x).split([L.n_q * D, L.n_kv * D, L.n_kv * D], -1)
             else:
@@ -247,14 +268,61 @@ class Qwen2HxqDecoder(nn.Module):
             a = F.scaled_dot_product_attention(q, kk, vv, attn_mask=mask, enable_gqa=True)
             a = a.transpose(1, 2).reshape(B, T, L.n_q * D)
             h = h + (yield L.o_proj(a), "d1")
-            x = self._rms(h, L.ln2)
-            if L.fused:
-                gt, up = L.gate_up_proj(x).split([L.inter_local, L.inter_local], -1)
-            else:
-                gt, up = L.gate_proj(x), L.up_proj(x)
-            h = h + (yield L.down_proj(F.silu(gt) * up), "d2")
+            h = h + (yield self._mlp(L, self._rms(h, L.ln2)), "d2")
         h = self._rms(h[:, -1], self.norm)
         return h @ self.lm_head.t()
+
+    @staticmethod
+    def _mlp(L, x):
+        if L.fused:
+            gt, up = L.gate_up_proj(x).split([L.inter_local, L.inter_local], -1)
+        else:
+            gt, up = L.gate_proj(x), L.up_proj(x)
+        return L.down_proj(F.silu(gt) * up)
+
+    def _prompt_plan(self, B, T, positions, cache_rows, attn_len):
+        """What every layer's fused prompt attention needs: where each sequence's tokens lie, and, for an 8-bit cache that
+        holds earlier rows, scratch in which they stand beside the new ones as bf16."""
+        L0, D, dev = self.layers[0], self.shp.head_dim, positions.device
+        plan = dict(B=B, T=T, positions=positions, rows=cache_rows, attn_len=self.max_len if attn_len is None else attn_len,
+                    cu=torch.arange(0, B * T + 1, T, device=dev, dtype=torch.int32), scratch=None,
+                    k_len=(positions[-1:] + 1).expand(B).contiguous())
+        if self.kv_bits == 8 and plan["attn_len"] != T:
+            plan["scratch"] = torch.empty(2, B, L0.n_kv, plan["attn_len"], D, device=dev, dtype=torch.bfloat16)
+        return plan
+
+    def _prompt_attention(self, li, L, x, cos, sin, plan):
+        """Projections, rotary embedding, append and attention of T tokens a sequence -> [B, T, n_q D]."""
+        B, T, D, nq, nkv = plan["B"], plan["T"], self.shp.head_dim, L.n_q, L.n_kv
+        if L.fused:
+            qkv = L.qkv_proj(x)
+        else:
+            qkv = torch.cat([L.q_proj(x), L.k_proj(x), L.v_proj(x)], -1)
+        qkv = qkv.reshape(B * T, (nq + 2 * nkv) * D)
+        heads = qkv.view(B * T, nq + 2 * nkv, D)
+        out = torch.empty(B * T, nq, D, device=qkv.device, dtype=torch.bfloat16)
+        if self.kv_bits == 16:
+            turned = self._rope(heads[:, : nq + nkv].unflatten(0, (B, T)), cos[0, 0][None, :, None], sin[0, 0][None, :, None])
+            self.k_cache[li].index_copy_(2, plan["rows"], turned[:, :, nq:].transpose(1, 2))
+            self.v_cache[li].index_copy_(2, plan["rows"], heads[:, nq + nkv:].unflatten(0, (B, T)).transpose(1, 2))
+            n = plan["attn_len"]
+            prompt_ops.attn_prompt(turned.flatten(0, 1)[:, :nq], self.k_cache[li][:, :, :n], self.v_cache[li][:, :, :n], out, plan["cu"], T,
+                                   D ** -0.5, k_len=plan["k_len"])
+            return out.view(B, T, nq * D)
+        q = torch.empty(B * T, nq * D, device=qkv.device, dtype=torch.bfloat16)
+        k = torch.empty(B * T, nkv, D, device=qkv.device, dtype=torch.bfloat16)
+        v = heads[:, nq + nkv:]
+        start, cache = plan["positions"][:1], self.kv8[li][:B]
+        if plan["scratch"] is not None:      # the rows that the cache held before these tokens
+            kv8.kv8_rows(cache, start, *plan["scratch"])
+        kv8.rope_append_prompt_kv8(qkv, plan["cu"], T, start, self.cos, self.sin, q, k, cache, nq)
+        if plan["scratch"] is None:
+            prompt_ops.attn_prompt(q.view(B * T, nq, D), k, v, out, plan["cu"], T, D ** -0.5)
+        else:
+            for rows, new in zip(plan["scratch"], (k, v)):
+                rows.index_copy_(2, plan["rows"], new.unflatten(0, (B, T)).transpose(1, 2))
+            prompt_ops.attn_prompt(q.view(B * T, nq, D), *plan["scratch"], out, plan["cu"], T, D ** -0.5, k_len=plan["k_len"])
+        return out.view(B, T, nq * D)
 
     def _step_buffers(self, B: int):
         sb = getattr(self, "_sb", None)
@@ -316,8 +384,13 @@ class Qwen2HxqDecoder(nn.Module):
                 L.q_proj.packed().matmul(x, bf, out=qkv[:, : nq * D])
                 L.k_proj.packed().matmul(x, bf, out=qkv[:, nq * D: (nq + nkv) * D])
                 L.v_proj.packed().matmul(x, bf, out=qkv[:, (nq + nkv) * D:])
-            decode_ops.rope_append(qkv, pos, self.cos, self.sin, sb["q"], self.k_cache[li], self.v_cache[li], nq, nkv)
-            decode_ops.attn_decode(sb["q"], self.k_cache[li], self.v_cache[li], pos, sb["a"], nq, D ** -0.5)
+            if self.kv_bits == 8:
+                cache = self.kv8[li] if self.kv8[li].slots == B else self.kv8[li][:B]
+                kv8.rope_append_kv8(qkv, pos, self.cos, self.sin, sb["q"], cache, nq)
+                kv8.attn_decode_kv8(sb["q"], cache, pos, sb["a"], nq, D ** -0.5)
+            else:
+                decode_ops.rope_append(qkv, pos, self.cos, self.sin, sb["q"], self.k_cache[li], self.v_cache[li], nq, nkv)
+                decode_ops.attn_decode(sb["q"], self.k_cache[li], self.v_cache[li], pos, sb["a"], nq, D ** -0.5)
             # the exchange is handed the weight of the norm that follows it: a driver that folds the
             # residual add and that norm into the sum answers None
             delta = yield (*row_parallel(L.o_proj, sb["a"], "d1"), L.ln2)
@@ -352,8 +425,11 @@ class Qwen2HxqDecoder(nn.Module):
         """Capture the one-token step.  Returns (run, tok, pos): write the
         current tokens into ``tok`` [B, 1] and the position into ``pos`` [1],
         call ``run()``, read the next tokens from its result."""
+        if self.kv_bits == 8 and not fused:
+            raise ValueError("an 8-bit cache is decoded with the fused step")
         tok = torch.zeros(batch, 1, device=self.device, dtype=torch.long)
-        pos = torch.zeros(1, device=self.device, dtype=torch.long)
+        # (an 8-bit cache's warm-up runs at position -1, which leaves the cache as it is)
+        pos = torch.full((1,), -1 if self.kv_bits == 8 else 0, device=self.device, dtype=torch.long)
 
         def body():
             if fused:
@@ -403,7 +479,8 @@ class Qwen2HxqDecoder(nn.Module):
 
 def run_decode(shape: str, batches, prompt: int, new_tokens: int, device, rank: int = 0, world: int = 1, *,
                layers: int = 0, build: str = "local", allreduce: str = "p2p", fuse_proj: bool = True,
-               graph: bool = True, torch_glue: bool = False, fill_cache: bool = False):
+               graph: bool = True, torch_glue: bool = False, fill_cache: bool = False, kv_bits: int = 16,
+               prompt_attn: str = "torch"):
     """Build ONE random-init HXQ decoder of the named shape and, for every batch size in ``batches``,
     prefill ``prompt`` tokens per sequence and time ``new_tokens - 1`` greedy steps (CUDA events, max
     over ranks).  ``fill_cache`` replaces the prefill by random K/V rows (decode speed at a given
@@ -417,14 +494,19 @@ def run_decode(shape: str, batches, prompt: int, new_tokens: int, device, rank: 
         shp.layers = layers
     t0 = time.perf_counter()
     model = Qwen2HxqDecoder(shp, device, max(batches), prompt + new_tokens + 8, rank=rank, world=world,
-                            fuse_proj=fuse_proj, p2p_allreduce=(allreduce == "p2p"), build=build)
+                            fuse_proj=fuse_proj, p2p_allreduce=(allreduce == "p2p"), build=build, kv_bits=kv_bits,
+                            prompt_attn=prompt_attn)
     torch.cuda.synchronize(device)
     build_s = time.perf_counter() - t0
     k_full, v_full = model.k_cache, model.v_cache
+    kv8_full = model.kv8 if kv_bits == 8 else None
     hxq_mods = [m for m in model.modules() if isinstance(m, HelixLinear)]
     out = []
     for batch in batches:
-        model.k_cache, model.v_cache = k_full[:, :batch], v_full[:, :batch]
+        if kv8_full is not None:
+            model.kv8 = [c[:batch] for c in kv8_full]
+        else:
+            model.k_cache, model.v_cache = k_full[:, :batch], v_full[:, :batch]
         for name in ("_graph", "_sb"):
             if hasattr(model, name):
                 delattr(model, name)
@@ -434,7 +516,12 @@ def run_decode(shape: str, batches, prompt: int, new_tokens: int, device, rank: 
         with torch.no_grad():
             if fill_cache:
                 g = torch.Generator(device=device).manual_seed(1 + rank)
-                for li in range(shp.layers):   # layer by layer: the fp32 temporaries stay small
+                for c in (model.kv8 if kv_bits == 8 else ()):
+                    for codes, scale, tail in ((c.k, c.k_scale, c.k_tail), (c.v, c.v_scale, c.v_tail)):
+                        codes.copy_((torch.randn(codes.shape, device=device, generator=g) * 32).clamp_(-127, 127))
+                        scale.fill_(0.5 / 32)
+                        tail.copy_(torch.randn(tail.shape, device=device, generator=g) * 0.5)
+                for li in range(shp.layers if kv_bits == 16 else 0):   # layer by layer: the fp32 temporaries stay small
                     for cache in (model.k_cache, model.v_cache):
                         view = cache[li][:, :, :prompt]
                         view.copy_(torch.randn(view.shape, device=device, generator=g) * 0.5)
@@ -481,7 +568,7 @@ def run_decode(shape: str, batches, prompt: int, new_tokens: int, device, rank: 
             ar_status = model._ar.check_status()
         out.append({
             "tok_s": batch * 1000.0 / ms_dec, "ms_per_step": ms_dec, "batch": batch, "context": prompt,
-            "new_tokens": new_tokens, "shape": shape, "layers": shp.layers, "n_gpus": world,
+            "new_tokens": new_tokens, "kv_bits": kv_bits, "prompt_attn": model.prompt_attn, "shape": shape, "layers": shp.layers, "n_gpus": world,
             "launch": "python" if run is None else "cuda_graph", "glue": "torch" if torch_glue else "fused",
             "projections": "qkv,o,gate_up,down" if fuse_proj else "q,k,v,o,gate,up,down",
             "allreduce": (allreduce if world > 1 else None), "allreduce_status": ar_status,
@@ -496,7 +583,7 @@ def run_decode(shape: str, batches, prompt: int, new_tokens: int, device, rank: 
     for name in ("_graph", "_ar", "_sb"):
         if hasattr(model, name):
             delattr(model, name)
-    del model, k_full, v_full, hxq_mods
+    del model, k_full, v_full, kv8_full, hxq_mods
     gc.collect()
     torch.cuda.empty_cache()
     return out
@@ -522,6 +609,9 @@ def main(argv=None):
     ap.add_argument("--build", default="local", choices=["local", "global"],
                     help="local: each rank compresses matrices of its shard's shape; global: full matrices, then sharded")
     ap.add_argument("--fill-cache", action="store_true", help="random K/V rows instead of a prefill")
+    ap.add_argument("--kv-bits", type=int, default=16, choices=[8, 16], help="bits of the key/value cache")
+    ap.add_argument("--prompt-attn", default="torch", choices=["torch", "fused"],
+                    help="the prompt's attention: the framework's operator, or the fused kernel (always with --kv-bits 8)")
     ap.add_argument("--separate-proj", action="store_true",
                     help="q, k, v and gate, up as separate compressed matrices (7 products per layer instead of 4)")
     args = ap.parse_args(argv)
@@ -533,7 +623,8 @@ def main(argv=None):
         init_tensor_parallel(dev)
     res = run_decode(args.shape, [args.batch], args.prompt, args.new, dev, rank, world, layers=args.layers,
                      build=args.build, allreduce=args.allreduce, fuse_proj=not args.separate_proj,
-                     graph=not args.no_graph, torch_glue=args.torch_glue, fill_cache=args.fill_cache)[0]
+                     graph=not args.no_graph, torch_glue=args.torch_glue, fill_cache=args.fill_cache, kv_bits=args.kv_bits,
+                     prompt_attn=args.prompt_attn)[0]
     if rank == 0:
         print(json.dumps({"metric": "decode_tokens_per_s", "value": res["tok_s"], "unit": "tok/s", **res,
                           "data": "synthetic: N(0,0.02) weights, uniform random prompt ids"}), flush=True)
