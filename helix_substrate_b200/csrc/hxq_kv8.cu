@@ -28,11 +28,12 @@ __device__ __forceinline__ void pdl_enter() {
 }
 
 template <typename... KArgs, typename... Args>
-static cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStream_t stream, Args&&... args) {
+static cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStream_t stream, size_t smem, Args&&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.stream = stream;
+    cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -318,15 +319,21 @@ __global__ void __launch_bounds__(256) rows_kernel(const Cache c, const int64_t*
 // ---- single-query attention -------------------------------------------------------------------------
 
 constexpr int kWarps = 4;
+constexpr int kDecodeCtas = 3;      // per SM
 constexpr int kHeads = 8;           // query heads of a KV head: the used rows of an MMA's sixteen
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1));
+// d (+)= a * b, one warp: int8 with 32 dimensions, fp16 and bf16 with 16.
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(0u), "r"(a2), "r"(0u), "r"(b0), "r"(b1));
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
@@ -345,11 +352,6 @@ __device__ __forceinline__ uint32_t codes2(uint32_t x) {
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(bias));
     return r;
 }
-__device__ __forceinline__ uint2 ld_stream_u2(const void* p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
 __device__ __forceinline__ float quad_max(float v) {
     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
     return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
@@ -359,7 +361,13 @@ __device__ __forceinline__ float quad_sum(float v) {
     return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
 
-// Units of 64 positions (the last one the tail) of one sequence, and how many of them a CTA of the split takes.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Units of 64 positions of one sequence, the unfinished block among them.
 __device__ __forceinline__ int units_of(int64_t pos, int max_len) {
     if (pos < 0 || pos >= max_len) return 0;
     return (int)(pos / kBlock) + 1;
@@ -370,231 +378,337 @@ struct DecodeArgs {
     const __nv_bfloat16* q;
     const int64_t* pos;
     __nv_bfloat16* out;
-    float* part;            // [B, nq, splits, D + 2]: maximum, sum, un-normalised output
+    float* part;            // [CTAs, 2, G, D + 2]: maximum, sum, un-normalised output
     int64_t ld_q, ld_out;
-    int pos_stride, nq, G, splits;
+    int pos_stride, B, nq, G, ctas;
     float scale_log2;       // scale * log2(e)
 };
 
-// One CTA: a contiguous share of one sequence's blocks, one KV head, all of its (up to eight) query heads; a warp takes
-// whole blocks of 64 positions in turn, 32 positions at a step.
+// The units of all (sequence, KV head) pairs in a row, sequence by sequence, head by head: where the share of a CTA starts.
+// Every warp works it out for itself from the positions.
+struct Share {
+    int64_t per;        // units per CTA
+    int64_t before;     // units of the sequences before b, of one head
+    int b, units;       // the sequence that holds the given unit (or sequence `at`), and its units
+};
+// Where flat unit `flat` (>= 0) lies, or, with flat < 0, sequence `at`.
+__device__ __forceinline__ Share find(const DecodeArgs& a, int cta, int at, int64_t& total) {
+    const int lane = threadIdx.x & 31;
+    Share r;
+    int64_t sum = 0;
+    if (a.pos_stride == 0) {            // all alike
+        r.units = units_of(a.pos[0], a.c.max_len);
+        sum = (int64_t)r.units * a.B;
+    } else {
+        for (int b0 = 0; b0 < a.B; b0 += 32) {
+            int u = b0 + lane < a.B ? units_of(a.pos[b0 + lane], a.c.max_len) : 0;
+            sum += __reduce_add_sync(0xffffffffu, u);
+        }
+    }
+    total = sum * a.c.nkv;
+    r.per = (total + a.ctas - 1) / a.ctas;
+    if (r.per < kWarps) r.per = kWarps;       // a unit for each warp at least
+    const int64_t flat = at < 0 ? r.per * cta : 0;
+    if (at < 0 && flat >= total) { r.b = -1; r.before = 0; r.units = 0; return r; }
+    if (a.pos_stride == 0) {
+        r.b = at < 0 ? (int)(flat / ((int64_t)r.units * a.c.nkv)) : at;
+        r.before = (int64_t)r.b * r.units;
+        return r;
+    }
+    int64_t before = 0;
+    for (int b0 = 0;; b0 += 32) {
+        const int u = b0 + lane < a.B ? units_of(a.pos[b0 + lane], a.c.max_len) : 0;
+        int incl = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        const uint32_t hit = at < 0 ? __ballot_sync(0xffffffffu, (before + incl) * a.c.nkv > flat)
+                                    : (at - b0 < 32 ? 1u << (at - b0) : 0u);
+        if (hit != 0u || b0 + 32 >= a.B) {
+            const int l = hit != 0u ? __ffs(hit) - 1 : 31;
+            r.b = b0 + l;
+            r.units = __shfl_sync(0xffffffffu, u, l);
+            r.before = before + __shfl_sync(0xffffffffu, incl, l) - r.units;
+            return r;
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+}
+
+// Every CTA takes the same number of units, whatever the sequences' lengths: a contiguous share of the row of all
+// units, i.e. a few segments, each of one sequence and KV head with all of its (up to eight) query heads.  In a segment a
+// warp takes units of 64 positions in turn, 32 positions at a step.  A segment that is a whole pair writes the output, the
+// others partial results, which the next launch joins.
 //
 // Bound by HBM: each code is read once, 2 D bytes a position and KV head.  On the CUDA cores G query heads cost G
 // multiply-adds a code, more than the cores have at the memory's pace from G = 5 on, so both products go through
-// mma.sync m16n8k16 in fp16 with fp32 sums (a tcgen05 tile would want 128 rows of queries; there are eight).
-//   * codes become fp16 exactly (two byte permutes and a subtraction for four); a query row is scaled by a power of two
-//     into fp16's range, which keeps bf16's eight bits; a block's scale multiplies sums in fp32.
+// mma.sync (a tcgen05 tile would want 128 rows of queries; there are eight).
+//   * Q K^T runs in int8, the codes as they are.  A query row is rounded to 16 bits, a step of 2^-16 of its largest element
+//     (bf16 itself has steps of 2^-9 of each), as two int8 planes q = 256 hi + lo: heads' high parts are rows 0-7 of the
+//     MMA, low parts rows 8-15, and both sums of a score end in one lane.  They are exact; scales multiply in fp32.
+//   * P V runs in fp16 with fp32 sums: codes become fp16 exactly (two byte permutes and a subtraction for two), dimensions
+//     are the MMA's rows and heads its columns, which is how the scores' layout already holds P.  Probabilities are scaled by
+//     2^10 and rounded to fp16: 2^-12 relative (a sixteenth of the output's own rounding) down to 2^-24 of the largest, 2^-35
+//     of it absolute below that; the sum that divides takes them in fp32.
 //   * the order of a contraction's index is free, so it is chosen such that every lane's operands are 16 consecutive
-//     bytes of a cache row: keys go from memory to registers to the MMA with no exchange, values with two byte permutes per
-//     two rows, and a warp's load covers whole 64- or 128-byte pieces.  The next 32 positions' keys are in flight while
-//     this step's values are used, and the other way round.
-//   * probabilities are rounded to fp16, 2^-12 relative, a sixteenth of the output's own rounding; the sum that divides
-//     takes them in fp32.
-//   * the tail's products run in bf16, with each probability as the sum of two bf16 numbers (2^-17).
+//     bytes of a cache row: no lane needs another's bytes.  They pass through a ring in shared memory that each lane
+//     fills (asynchronous copies) and reads back for itself: a step of 8 KB a warp is in flight while one is used, nothing
+//     but its own copies is waited for, and there are no bank conflicts (a slot of 16 bytes per lane).
+//   * the tail's products run in bf16, 16 positions to a warp, with each probability as the sum of two bf16 numbers (2^-17).
+constexpr int kStages = 2;
 template <int DP>
-__global__ void __launch_bounds__(32 * kWarps) decode_kernel(const DecodeArgs a) {
-    constexpr int KS = DP / 16;        // k steps of Q K^T
+struct DecodeSmem { static constexpr int bytes = kWarps * kStages * 64 * DP; };
+
+template <int DP>
+__global__ void __launch_bounds__(32 * kWarps, kDecodeCtas) decode_kernel(const DecodeArgs a) {
+    constexpr int KS = DP / 32;        // k steps of Q K^T
+    constexpr int MT = DP / 16;        // m tiles of P V
     constexpr int KC = DP / 64;        // 16-byte pieces of a key row per lane
-    constexpr int NT = DP / 8;         // n tiles of P V, and bytes of a value row per lane
-    const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+    constexpr int NT = DP / 8;         // bytes of a value row per lane
+    constexpr int STAGE = 64 * DP;     // a step's bytes: 32 positions of keys, then of values
+    extern __shared__ __align__(16) char ring_smem[];
+    float (*o_s)[kHeads][DP] = reinterpret_cast<float (*)[kHeads][DP]>(ring_smem);      // at a segment's end, in the rings' place
+    static_assert(sizeof(float) * kWarps * kHeads * DP <= DecodeSmem<DP>::bytes, "the sums fit");
+    __shared__ float m_s[kWarps][kHeads], l_s[kWarps][kHeads];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int D = a.c.D;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(ring_smem) + (uint32_t)(warp * kStages * STAGE);
     pdl_enter();
-    const int64_t pos = a.pos[(int64_t)b * a.pos_stride];
-    const int units = units_of(pos, a.c.max_len);
-    const int span = (units + a.splits - 1) / a.splits;
-    const int u0 = split * span, u1 = u0 + span < units ? u0 + span : units;
-    if (u0 >= u1) {
-        if (a.splits == 1)          // nothing to see: zeros
-            for (int i = threadIdx.x; i < a.G * D; i += 32 * kWarps) a.out[(int64_t)b * a.ld_out + (int64_t)kvh * a.G * D + i] = __float2bfloat16_rn(0.f);
-        return;
-    }
-    const int tail_n = (int)((pos + 1) % kBlock);        // rows of the unfinished block
-    const int whole = tail_n ? units - 1 : units;        // units below this one are finished blocks
-    const int64_t head = (int64_t)b * a.c.nkv + kvh;
-    const __nv_bfloat16* q = a.q + (int64_t)b * a.ld_q + ((int64_t)kvh * a.G + (g < a.G ? g : 0)) * D;
+    int64_t total;
+    const Share at = find(a, blockIdx.x, -1, total);
+    if (at.b < 0) return;
+    int64_t flat = at.per * blockIdx.x;
+    const int64_t flat_end = flat + at.per < total ? flat + at.per : total;
+    int b = at.b, units = at.units;
+    int64_t pair0 = at.before * a.c.nkv;           // flat unit at which head kvh of sequence b starts
+    int kvh = (int)((flat - pair0) / units);
+    pair0 += (int64_t)kvh * units;
+    int slot = 0;
 
-    float o[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = 0.f;
-    float m = -INFINITY, l = 0.f;           // of head g: m the same in its four lanes, l this lane's positions
-
-    // Running softmax of S scores; rescales o when the maximum moved.  Returns the probabilities in s.
-    auto softmax = [&](float* s, int S) {
-        float mx = m;
-#pragma unroll
-        for (int i = 0; i < S; ++i) mx = fmaxf(mx, s[i]);
-        mx = quad_max(mx);
-        const float ref = mx == -INFINITY ? 0.f : mx;
-        const float corr = exp2f(m - ref);
-        l *= corr;
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-            s[i] = exp2f(s[i] - ref);
-            l += s[i];
-        }
-        if (__any_sync(0xffffffffu, mx != m)) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n) { o[n][0] *= corr; o[n][1] *= corr; }
-        }
-        m = mx;
-    };
-
-    int u = u0 + warp;
-    if (u < u1 && u < whole) {
-        // query rows as fp16 A operands: lane (g, t) holds the dimensions of the key pieces it loads
-        uint32_t qa[KS][2];
-        float q_back;
-        {
-            float f[KC][2][8];
-            float amax = 0.f;
-#pragma unroll
-            for (int i = 0; i < KC; ++i)
-#pragma unroll
-                for (int hh = 0; hh < 2; ++hh) {
-                    const int d = 64 * i + 16 * t + 8 * hh;
-                    uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                    if (d < D && g < a.G) w = ld16(q + d);
-                    unpack8(w, f[i][hh]);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(f[i][hh][e]));
-                }
-            amax = quad_max(amax);
-            int ex = (int)(__float_as_uint(amax) >> 23);        // 0 .. 255
-            if (ex == 0 || ex == 255) ex = 137;                 // zeros, infinities: as they are
-            if (ex < 27) ex = 27;
-            const float up = __uint_as_float((uint32_t)(264 - ex) << 23);      // largest element into [2^10, 2^11)
-            q_back = __uint_as_float((uint32_t)(ex - 10) << 23);
-#pragma unroll
-            for (int i = 0; i < KC; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float* e = &f[i][j >> 1][4 * (j & 1)];
-                    qa[4 * i + j][0] = half2_of(e[0] * up, e[1] * up);
-                    qa[4 * i + j][1] = half2_of(e[2] * up, e[3] * up);
-                }
-            q_back *= a.scale_log2;
-        }
-        const int8_t* kp = a.c.k + head * a.c.max_len * D;
-        const int8_t* vp = a.c.v + head * a.c.max_len * D;
+    while (true) {          // segments
+        const int64_t pos = a.pos[(int64_t)b * a.pos_stride];
+        const int u0 = (int)(flat - pair0);
+        const int u1 = flat_end - pair0 < units ? (int)(flat_end - pair0) : units;
+        const int tail_n = (int)((pos + 1) % kBlock);        // rows of the unfinished block
+        const int whole = tail_n ? units - 1 : units;        // units below this one are finished blocks
+        const int u_end = u1 < whole ? u1 : whole;
+        const int64_t head = (int64_t)b * a.c.nkv + kvh;
+        const __nv_bfloat16* q = a.q + (int64_t)b * a.ld_q + ((int64_t)kvh * a.G + (g < a.G ? g : 0)) * D;
+        const int8_t* kp = a.c.k + head * a.c.max_len * D + g * D + 16 * t;
+        const int8_t* vp = a.c.v + head * a.c.max_len * D + 2 * t * D + NT * g;
         const float* ksp = a.c.ks + head * (a.c.max_len / kBlock);
         const float* vsp = a.c.vs + head * (a.c.max_len / kBlock);
-        uint4 kr[4][KC];
-        uint4 vr[2][4];           // (eight-byte loads at DP = 64 use x and y)
-        auto load_k = [&](int unit, int half) {
-            const int8_t* p = kp + ((int64_t)unit * kBlock + half * 32 + g) * D + 16 * t;
+        const int first = u0 + warp;
+        const int steps = first < u_end ? 2 * ((u_end - first + kWarps - 1) / kWarps) : 0;       // of 32 positions
+        auto fetch = [&](int step, uint32_t st) {       // always one group
+            if (step < steps) {
+                const int64_t row = (int64_t)(first + (step >> 1) * kWarps) * kBlock + (step & 1) * 32;
+                const int8_t* k = kp + row * D;
+                const int8_t* v = vp + row * D;
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+                for (int n = 0; n < 4; ++n)
 #pragma unroll
-                for (int i = 0; i < KC; ++i) kr[n][i] = 64 * i + 16 * t < D ? ld_stream_u4(p + n * 8 * D + 64 * i) : make_uint4(0u, 0u, 0u, 0u);
+                    for (int i = 0; i < KC; ++i) {
+                        const uint32_t bytes = 64 * i + 16 * t < D ? 16u : 0u;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                                     :: "r"(st + (uint32_t)((n * KC + i) * 512 + lane * 16)), "l"(bytes ? k + n * 8 * D + 64 * i : kp), "r"(bytes) : "memory");
+                    }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {       // rows 16 (j / 4) + 8 (j / 2 % 2) + 2 t + j % 2
+                    const int8_t* vr = v + (16 * (j >> 2) + 8 * ((j >> 1) & 1) + (j & 1)) * D;
+                    const uint32_t bytes = NT * g < D ? (uint32_t)NT : 0u;
+                    const uint32_t dst = st + (uint32_t)(32 * DP + j * 32 * NT + lane * NT);
+                    if constexpr (NT == 16)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(bytes ? vr : vp - NT * g), "r"(bytes) : "memory");
+                    else
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" :: "r"(dst), "l"(bytes ? vr : vp - NT * g), "r"(bytes) : "memory");
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        auto load_v = [&](int unit, int half) {
-            const int8_t* p = vp + ((int64_t)unit * kBlock + half * 32 + 2 * t) * D + NT * g;
+        auto take = [&](uint32_t addr) {
+            uint4 v;
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+            return v;
+        };
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+        for (int k = 0; k < kStages - 1; ++k) fetch(k, ring + k * STAGE);
+
+        float o[MT][4];        // dimensions 16 g + 2 i and + 1 (rows g, g + 8) of heads 2 t and 2 t + 1
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int8_t* pr = p + (16 * j + (r & 1) + 8 * (r >> 1)) * D;
-                    vr[j][r] = make_uint4(0u, 0u, 0u, 0u);
-                    if (NT * g < D) {
-                        if constexpr (NT == 16) {
-                            vr[j][r] = ld_stream_u4(pr);
-                        } else {
-                            const uint2 w = ld_stream_u2(pr);
-                            vr[j][r].x = w.x;
-                            vr[j][r].y = w.y;
+        for (int i = 0; i < MT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        float m = -INFINITY, l = 0.f;           // of head g: m the same in its four lanes, l this lane's positions
+
+        // Running softmax of S scores; rescales o when the maximum moved.  Returns the probabilities in s.
+        auto softmax = [&](float* s, int S) {
+            float mx = m;
+#pragma unroll
+            for (int i = 0; i < S; ++i) mx = fmaxf(mx, s[i]);
+            mx = quad_max(mx);
+            const float ref = mx == -INFINITY ? 0.f : mx;
+            const float corr = ex2(m - ref);
+            l *= corr;
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                s[i] = ex2(s[i] - ref);
+                l += s[i];
+            }
+            if (__any_sync(0xffffffffu, mx != m)) {
+                const float c0 = __shfl_sync(0xffffffffu, corr, 8 * t), c1 = __shfl_sync(0xffffffffu, corr, 8 * t + 4);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) { o[i][0] *= c0; o[i][1] *= c1; o[i][2] *= c0; o[i][3] *= c1; }
+            }
+            m = mx;
+        };
+
+        if (steps > 0) {
+            float ks = ksp[first], vs = vsp[first], ks_next = 0.f, vs_next = 0.f;
+            // query rows as int8 A operands: lane (g, t) holds the dimensions of the key pieces it loads
+            uint32_t qa[KS][4];
+            float q_back;
+            {
+                float f[KC][2][8];
+                float amax = 0.f;
+                bool bad = false;
+#pragma unroll
+                for (int i = 0; i < KC; ++i)
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh) {
+                        const int d = 64 * i + 16 * t + 8 * hh;
+                        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                        if (d < D && g < a.G) w = ld16(q + d);
+                        unpack8(w, f[i][hh]);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            amax = fmaxf(amax, fabsf(f[i][hh][e]));
+                            bad |= !(fabsf(f[i][hh][e]) <= 3.4e38f);
                         }
                     }
-                }
-        };
-        const int u_end = u1 < whole ? u1 : whole;
-        load_k(u, 0);
-        load_v(u, 0);
-        float ks = ksp[u], vs = vsp[u];
-        int half = 0;
-        while (true) {
-            int nu = u, nh = 1;
-            if (half == 1) { nu = u + kWarps; nh = 0; }
-            const bool more = nu < u_end;
-            float s[8], c4[4][4];
+                bad = (__ballot_sync(0xffffffffu, bad) >> (lane & 28) & 15u) != 0u;      // in any of the head's four lanes
+                amax = quad_max(amax);
+                int ex = (int)(__float_as_uint(amax) >> 23);
+                if (ex == 0 || bad) { ex = 127; amax = 0.f; }       // zeros (or less than a normal number)
+                if (ex > 253) ex = 253;
+                const float up = __uint_as_float((uint32_t)(254 - ex) << 23);          // largest element into [1, 4)
+                const float to16 = amax > 0.f ? 32512.f / (amax * up) : 0.f;
+                q_back = __uint_as_float((uint32_t)ex << 23) * (amax * up / 32512.f) * a.scale_log2;
+                if (bad) q_back = __uint_as_float(0x7fc00000u);
 #pragma unroll
-            for (int n = 0; n < 4; ++n) c4[n][0] = c4[n][1] = c4[n][2] = c4[n][3] = 0.f;
+                for (int i = 0; i < KC; ++i)
 #pragma unroll
-            for (int i = 0; i < KC; ++i)
+                    for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                        for (int w = 0; w < 2; ++w) {
+                            uint32_t hi = 0u, lo = 0u;
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {       // four independent sums
-                        const uint32_t w[4] = {kr[n][i].x, kr[n][i].y, kr[n][i].z, kr[n][i].w};
-                        const uint32_t x = w[j] ^ 0x80808080u;
-                        mma_f16(c4[n], qa[4 * i + j][0], qa[4 * i + j][1], codes2<0x4140>(x), codes2<0x4342>(x));
-                    }
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                s[2 * n] = c4[n][0] * (ks * q_back);
-                s[2 * n + 1] = c4[n][1] * (ks * q_back);
+                            for (int e = 0; e < 4; ++e) {
+                                const int v = __float2int_rn(f[i][hh][4 * w + e] * up * to16);
+                                const int h = (v + 128) >> 8;
+                                hi |= ((uint32_t)h & 0xffu) << (8 * e);
+                                lo |= ((uint32_t)(v - 256 * h) & 0xffu) << (8 * e);
+                            }
+                            qa[2 * i + hh][2 * w] = hi;
+                            qa[2 * i + hh][2 * w + 1] = lo;
+                        }
             }
-            if (more) load_k(nu, nh);
-            softmax(s, 8);
-#pragma unroll
-            for (int n0 = 0; n0 < NT; n0 += 4) {
-                float c[4][4];
-#pragma unroll
-                for (int n = 0; n < 4; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const uint32_t p0 = half2_of(s[4 * j], s[4 * j + 1]), p1 = half2_of(s[4 * j + 2], s[4 * j + 3]);
-                    uint32_t w[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const uint32_t v4[4] = {vr[j][r].x, vr[j][r].y, vr[j][r].z, vr[j][r].w};
-                        w[r] = v4[n0 >> 2] ^ 0x80808080u;
-                    }
-                    const uint32_t a01 = __byte_perm(w[0], w[1], 0x5140), a23 = __byte_perm(w[0], w[1], 0x7362);
-                    const uint32_t b01 = __byte_perm(w[2], w[3], 0x5140), b23 = __byte_perm(w[2], w[3], 0x7362);
-                    mma_f16(c[0], p0, p1, codes2<0x4140>(a01), codes2<0x4140>(b01));
-                    mma_f16(c[1], p0, p1, codes2<0x4342>(a01), codes2<0x4342>(b01));
-                    mma_f16(c[2], p0, p1, codes2<0x4140>(a23), codes2<0x4140>(b23));
-                    mma_f16(c[3], p0, p1, codes2<0x4342>(a23), codes2<0x4342>(b23));
+            uint32_t st = ring;
+#pragma unroll 1
+            for (int step = 0; step < steps; ++step) {
+                asm volatile("cp.async.wait_group %0;" :: "n"(kStages - 2) : "memory");      // this step has landed
+                fetch(step + kStages - 1, st == ring ? ring + (kStages - 1) * STAGE : st - STAGE);      // where the step before was
+                if ((step & 1) == 0) {
+                    const int next = first + ((step >> 1) + 1) * kWarps;
+                    if (next < u_end) { ks_next = ksp[next]; vs_next = vsp[next]; }
                 }
+                float s[8];
+                int c4[4][4];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) c4[n][0] = c4[n][1] = c4[n][2] = c4[n][3] = 0;
+#pragma unroll
+                for (int i = 0; i < KC; ++i) {
+                    uint4 kr[4];
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) kr[n] = take(st + (uint32_t)((n * KC + i) * 512 + lane * 16));
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) mma_s8(c4[n], qa[2 * i], kr[n].x, kr[n].y);
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) mma_s8(c4[n], qa[2 * i + 1], kr[n].z, kr[n].w);
+                }
+                const float back = ks * q_back;
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
-                    o[n0 + n][0] = fmaf(vs, c[n][0], o[n0 + n][0]);
-                    o[n0 + n][1] = fmaf(vs, c[n][1], o[n0 + n][1]);
+                    s[2 * n] = (float)(c4[n][0] * 256 + c4[n][2]) * back;
+                    s[2 * n + 1] = (float)(c4[n][1] * 256 + c4[n][3]) * back;
                 }
-            }
-            if (!more) break;
-            load_v(nu, nh);
-            if (nh == 0) { ks = ksp[nu]; vs = vsp[nu]; }
-            u = nu;
-            half = nh;
-        }
-    }
-
-    // the unfinished block: bf16 rows, sixteen positions at a step
-    if (tail_n && u1 == units && (units - 1 - u0) % kWarps == warp) {
-        const __nv_bfloat16* kt = a.c.kt + head * kBlock * D;
-        const __nv_bfloat16* vt = a.c.vt + head * kBlock * D;
-        uint32_t qb[KS][2];
+                softmax(s, 8);
+                uint32_t p[4];
 #pragma unroll
-        for (int i = 0; i < KS / 2; ++i) {
-            uint4 w = make_uint4(0u, 0u, 0u, 0u);
-            if (32 * i + 8 * t < D && g < a.G) w = ld16(q + 32 * i + 8 * t);
-            qb[2 * i][0] = w.x; qb[2 * i][1] = w.y;
-            qb[2 * i + 1][0] = w.z; qb[2 * i + 1][1] = w.w;
+                for (int n = 0; n < 4; ++n) p[n] = half2_of(s[2 * n] * 1024.f, s[2 * n + 1] * 1024.f);
+                const float vb = vs * (1.f / 1024.f);
+                uint4 vr[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t src = st + (uint32_t)(32 * DP + j * 32 * NT + lane * NT);
+                    if constexpr (NT == 16) {
+                        vr[j] = take(src);
+                    } else {
+                        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(vr[j].x), "=r"(vr[j].y) : "r"(src) : "memory");
+                        vr[j].z = vr[j].w = 0u;
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < NT / 4; ++w) {            // four dimensions: two m tiles
+                    float c[2][4];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {             // sixteen positions
+                        uint32_t x[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t v4[4] = {vr[4 * j + k].x, vr[4 * j + k].y, vr[4 * j + k].z, vr[4 * j + k].w};
+                            x[k] = v4[w] ^ 0x80808080u;
+                        }
+                        const uint32_t a01 = __byte_perm(x[0], x[1], 0x5140), a23 = __byte_perm(x[0], x[1], 0x7362);
+                        const uint32_t b01 = __byte_perm(x[2], x[3], 0x5140), b23 = __byte_perm(x[2], x[3], 0x7362);
+                        mma_f16(c[0], codes2<0x4140>(a01), codes2<0x4342>(a01), codes2<0x4140>(b01), codes2<0x4342>(b01), p[2 * j], p[2 * j + 1]);
+                        mma_f16(c[1], codes2<0x4140>(a23), codes2<0x4342>(a23), codes2<0x4140>(b23), codes2<0x4342>(b23), p[2 * j], p[2 * j + 1]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[2 * w + i][e] = fmaf(vb, c[i][e], o[2 * w + i][e]);
+                }
+                st = st + STAGE == ring + kStages * STAGE ? ring : st + STAGE;
+                if (step & 1) { ks = ks_next; vs = vs_next; }
+            }
         }
-        for (int p = 0; p < tail_n; p += 16) {
+
+        // the unfinished block: bf16 rows, sixteen positions to a warp
+        if (u1 == units && 16 * warp < tail_n) {
+            const __nv_bfloat16* kt = a.c.kt + head * kBlock * D;
+            const __nv_bfloat16* vt = a.c.vt + head * kBlock * D;
+            const int p = 16 * warp;
             float s[4];
+            uint32_t qb[KC * 2][4];
+#pragma unroll
+            for (int i = 0; i < 2 * KC; ++i) {
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (32 * i + 8 * t < D && g < a.G) w = ld16(q + 32 * i + 8 * t);
+                qb[i][0] = w.x; qb[i][1] = w.y; qb[i][2] = w.z; qb[i][3] = w.w;
+            }
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const int row = p + 8 * n + g;
                 float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < KS / 2; ++i) {
+                for (int i = 0; i < 2 * KC; ++i) {
                     uint4 w = make_uint4(0u, 0u, 0u, 0u);
                     if (32 * i + 8 * t < D && row < tail_n) w = ld16(kt + row * D + 32 * i + 8 * t);
-                    mma_bf16(c, qb[2 * i][0], qb[2 * i][1], w.x, w.y);
-                    mma_bf16(c, qb[2 * i + 1][0], qb[2 * i + 1][1], w.z, w.w);
+                    mma_bf16(c, qb[i][0], 0u, qb[i][1], 0u, w.x, w.y);
+                    mma_bf16(c, qb[i][2], 0u, qb[i][3], 0u, w.z, w.w);
                 }
                 const int col = p + 8 * n + 2 * t;
                 s[2 * n] = col < tail_n ? c[0] * a.scale_log2 : -INFINITY;
@@ -612,86 +726,126 @@ __global__ void __launch_bounds__(32 * kWarps) decode_kernel(const DecodeArgs a)
             for (int n0 = 0; n0 < NT; n0 += 8) {          // eight dimensions of four rows at a time
                 uint4 w[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = p + 2 * t + (r & 1) + 8 * (r >> 1);
-                    w[r] = make_uint4(0u, 0u, 0u, 0u);
-                    if (NT * g + n0 < D && row < tail_n) w[r] = ld16(vt + row * D + NT * g + n0);
+                for (int k = 0; k < 4; ++k) {
+                    const int row = p + 2 * t + (k & 1) + 8 * (k >> 1);
+                    w[k] = make_uint4(0u, 0u, 0u, 0u);
+                    if (NT * g + n0 < D && row < tail_n) w[k] = ld16(vt + row * D + NT * g + n0);
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+                for (int e = 0; e < 4; ++e) {             // a word is two dimensions: rows g and g + 8 of an m tile
                     const uint32_t x0 = (&w[0].x)[e], x1 = (&w[1].x)[e], x2 = (&w[2].x)[e], x3 = (&w[3].x)[e];
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const uint32_t b0 = __byte_perm(x0, x1, k ? 0x7632 : 0x5410), b1 = __byte_perm(x2, x3, k ? 0x7632 : 0x5410);
-                        float c[4] = {o[n0 + 2 * e + k][0], o[n0 + 2 * e + k][1], 0.f, 0.f};
-                        mma_bf16(c, hi[0], hi[1], b0, b1);
-                        mma_bf16(c, lo[0], lo[1], b0, b1);
-                        o[n0 + 2 * e + k][0] = c[0];
-                        o[n0 + 2 * e + k][1] = c[1];
-                    }
+                    const uint32_t a0 = __byte_perm(x0, x1, 0x5410), a1 = __byte_perm(x0, x1, 0x7632);
+                    const uint32_t a2 = __byte_perm(x2, x3, 0x5410), a3 = __byte_perm(x2, x3, 0x7632);
+                    mma_bf16(o[n0 / 2 + e], a0, a1, a2, a3, hi[0], hi[1]);
+                    mma_bf16(o[n0 / 2 + e], a0, a1, a2, a3, lo[0], lo[1]);
                 }
             }
         }
-    }
 
-    // ---- the four warps' (m, l, o) meet; lane (g, t) owns dimensions 2 NT t .. of head g
-    __shared__ float o_s[kWarps][kHeads][DP];
-    __shared__ float m_s[kWarps][kHeads], l_s[kWarps][kHeads];
-    l = quad_sum(l);
-    if (t == 0) { m_s[warp][g] = m; l_s[warp][g] = l; }
+        // ---- the four warps' (m, l, o) meet
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        l = quad_sum(l);
+        __syncthreads();              // every warp is through with its ring
+        if (t == 0) { m_s[warp][g] = m; l_s[warp][g] = l; }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        o_s[warp][g][2 * NT * t + n] = o[n][0];
-        o_s[warp][g][2 * NT * t + NT + n] = o[n][1];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < a.G * D; i += 32 * kWarps) {
-        const int hd = i / D, d = i - hd * D;
-        float mx = m_s[0][hd];
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, m_s[w][hd]);
-        const float ref = mx == -INFINITY ? 0.f : mx;
-        float ov = 0.f, lv = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float e = exp2f(m_s[w][hd] - ref);
-            ov += e * o_s[w][hd][d];
-            lv += e * l_s[w][hd];
+        for (int i = 0; i < MT; ++i) {
+            *reinterpret_cast<float2*>(&o_s[warp][2 * t][NT * g + 2 * i]) = make_float2(o[i][0], o[i][2]);
+            *reinterpret_cast<float2*>(&o_s[warp][2 * t + 1][NT * g + 2 * i]) = make_float2(o[i][1], o[i][3]);
         }
-        if (a.splits == 1) {
-            a.out[(int64_t)b * a.ld_out + ((int64_t)kvh * a.G + hd) * D + d] = __float2bfloat16_rn(ov / lv);
-        } else {
-            float* dst = a.part + (((int64_t)b * a.nq + kvh * a.G + hd) * a.splits + split) * (D + 2);
-            dst[2 + d] = ov;
-            if (d == 0) { dst[0] = mx; dst[1] = lv; }
+        __syncthreads();
+        const bool all = u0 == 0 && u1 == units;
+        for (int i = threadIdx.x; i < a.G * D; i += 32 * kWarps) {
+            const int hd = i / D, d = i - hd * D;
+            float mx = m_s[0][hd];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, m_s[w][hd]);
+            const float ref = mx == -INFINITY ? 0.f : mx;
+            float ov = 0.f, lv = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float e = ex2(m_s[w][hd] - ref);
+                ov += e * o_s[w][hd][d];
+                lv += e * l_s[w][hd];
+            }
+            if (all) {
+                a.out[(int64_t)b * a.ld_out + ((int64_t)kvh * a.G + hd) * D + d] = __float2bfloat16_rn(ov / lv);
+            } else {
+                float* dst = a.part + (((int64_t)blockIdx.x * 2 + slot) * a.G + hd) * (D + 2);
+                dst[2 + d] = ov;
+                if (d == 0) { dst[0] = mx; dst[1] = lv; }
+            }
+        }
+        slot = 1;
+        flat = pair0 + u1;
+        if (flat >= flat_end) return;
+        __syncthreads();              // the sums have been read
+        pair0 = flat;                 // the next pair
+        if (++kvh == a.c.nkv) {
+            kvh = 0;
+            do units = units_of(a.pos[(int64_t)(++b) * a.pos_stride], a.c.max_len); while (units == 0);
         }
     }
 }
 
-// out[b, head] = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over the CTAs that had blocks to look at.
-__global__ void __launch_bounds__(kMaxD) combine_kernel(const DecodeArgs a) {
-    const int head = blockIdx.x, b = blockIdx.y, d = threadIdx.x, D = a.c.D;
+// Joins the partial results of the pairs that more than one CTA had a segment of:
+// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c; sequences with nothing to see get zeros.  A long context has a
+// hundred partial results and more: four groups of threads take every fourth, several loads in flight each.
+constexpr int kJoin = 4;
+__global__ void __launch_bounds__(kJoin * kMaxD) combine_kernel(const DecodeArgs a) {
+    __shared__ float w_s[kDecodeCtas * 148 + 1], o_s[kJoin][kMaxD], red[2][kJoin * kMaxD / 32];
+    const int kvh = blockIdx.x, hd = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, D = a.c.D;
+    const int d = tid & (kMaxD - 1), j = tid / kMaxD, lane = tid & 31, warp = tid >> 5;
     pdl_enter();
-    const int units = units_of(a.pos[(int64_t)b * a.pos_stride], a.c.max_len);
-    if (d >= D) return;
-    __nv_bfloat16* out = a.out + (int64_t)b * a.ld_out + (int64_t)head * D;
-    if (units == 0) {
-        out[d] = __float2bfloat16_rn(0.f);
+    int64_t total;
+    const Share at = find(a, 0, b, total);
+    __nv_bfloat16* out = a.out + (int64_t)b * a.ld_out + ((int64_t)kvh * a.G + hd) * D;
+    if (at.units == 0) {
+        if (tid < D) out[tid] = __float2bfloat16_rn(0.f);
         return;
     }
-    const int span = (units + a.splits - 1) / a.splits, nc = (units + span - 1) / span;
-    const float* src = a.part + ((int64_t)b * a.nq + head) * a.splits * (D + 2);
+    const int64_t s = at.before * a.c.nkv + (int64_t)kvh * at.units, e = s + at.units;
+    const int c0 = (int)(s / at.per), n = (int)((e - 1) / at.per) - c0 + 1;
+    if (n == 1) return;           // one CTA had it all and wrote it
+    // the CTA that a pair starts in has it as its first segment, or as its last; the others as their first
+    const int64_t step = 2 * (int64_t)a.G * (D + 2);
+    const float* base = a.part + c0 * step + (int64_t)hd * (D + 2);
+    const int64_t skip = s == c0 * at.per ? 0 : step / 2;
+    auto part = [&](int c) { return base + c * step + (c == 0 ? skip : 0); };
     float mx = -INFINITY;
-    for (int c = 0; c < nc; ++c) mx = fmaxf(mx, src[(int64_t)c * (D + 2)]);
-    const float ref = mx == -INFINITY ? 0.f : mx;
-    float o = 0.f, l = 0.f;
-    for (int c = 0; c < nc; ++c) {
-        const float* p = src + (int64_t)c * (D + 2);
-        const float e = exp2f(p[0] - ref);
-        l += e * p[1];
-        o += e * p[2 + d];
+    for (int c = tid; c < n; c += kJoin * kMaxD) {
+        w_s[c] = part(c)[0];
+        mx = fmaxf(mx, w_s[c]);
     }
-    out[d] = __float2bfloat16_rn(o / l);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if (lane == 0) red[0][warp] = mx;
+    __syncthreads();
+    mx = red[0][0];
+#pragma unroll
+    for (int w = 1; w < kJoin * kMaxD / 32; ++w) mx = fmaxf(mx, red[0][w]);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float l = 0.f;
+    for (int c = tid; c < n; c += kJoin * kMaxD) {
+        const float w = ex2(w_s[c] - ref);
+        w_s[c] = w;
+        l += w * part(c)[1];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lane == 0) red[1][warp] = l;
+    __syncthreads();
+    float o = 0.f;
+    if (d < D)
+#pragma unroll 8
+        for (int c = j; c < n; c += kJoin) o += w_s[c] * part(c)[2 + d];
+    o_s[j][d] = o;
+    __syncthreads();
+    if (tid < D) {
+        float lv = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoin * kMaxD / 32; ++w) lv += red[1][w];
+        out[d] = __float2bfloat16_rn((o_s[0][d] + o_s[1][d] + o_s[2][d] + o_s[3][d]) / lv);
+    }
 }
 
 // ---- host side --------------------------------------------------------------------------------------
@@ -738,17 +892,28 @@ static int run_append(const hxq_kv8* c, const void* qkv, int64_t ld_qkv, int32_t
     const int64_t kv = (int64_t)S * c->nkv * 2 * a.n_blk, qc = ((int64_t)T + a.q_tokens - 1) / a.q_tokens;
     if (kv + qc > 0x7fffffffLL) return HXQ_E_SHAPE;
     a.kv_ctas = (int)kv;
-    const cudaError_t e = launch_pdl(append_kernel, dim3((unsigned)(kv + qc)), dim3(kAppendThreads), stream, a);
+    const cudaError_t e = launch_pdl(append_kernel, dim3((unsigned)(kv + qc)), dim3(kAppendThreads), stream, 0, a);
     return e == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
 }
 
-// CTAs that share one sequence and KV head.
-static int decode_splits(int B, int nkv, int max_len) {
-    const int64_t units = max_len / kBlock, pairs = (int64_t)B * nkv;
-    int64_t n = (148 * 8 + pairs - 1) / pairs;          // about eight CTAs of four warps per SM in all
-    const int64_t most = (units + kWarps - 1) / kWarps; // a block for each warp
-    if (n > most) n = most;
-    return (int)(n < 1 ? 1 : n);
+// CTAs: as many as fit, fewer where a full cache has not that many times four units.
+static int decode_ctas(int B, int nkv, int max_len) {
+    const int64_t units = (int64_t)(max_len / kBlock) * B * nkv, n = (units + kWarps - 1) / kWarps;
+    const int most = kDecodeCtas * 148;
+    return (int)(n < most ? (n < 1 ? 1 : n) : most);
+}
+
+template <int DP>
+static cudaError_t run_decode(const DecodeArgs& a, cudaStream_t stream) {
+    static bool attr_set[64] = {false};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!attr_set[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(decode_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeSmem<DP>::bytes);
+        if (e != cudaSuccess) return e;
+        attr_set[dev] = true;
+    }
+    return launch_pdl(decode_kernel<DP>, dim3(a.ctas), dim3(32 * kWarps), stream, DecodeSmem<DP>::bytes, a);
 }
 
 }  // namespace kv8
@@ -781,7 +946,7 @@ extern "C" int hxq_kv8_rows(const hxq_kv8* cache, const int64_t* len, int32_t le
     if (!hxq::aligned_to(k_out, 16) || !hxq::aligned_to(v_out, 16) || ld_seq % 8 != 0 || ld_head % 8 != 0 || ld_row % 8 != 0) return HXQ_E_ALIGN;
     const int n = rows < cache->max_len ? rows : cache->max_len;
     if (n == 0) return HXQ_OK;
-    const cudaError_t e = launch_pdl(rows_kernel, dim3((n + kBlock - 1) / kBlock, cache->nkv, S), dim3(256), reinterpret_cast<cudaStream_t>(stream),
+    const cudaError_t e = launch_pdl(rows_kernel, dim3((n + kBlock - 1) / kBlock, cache->nkv, S), dim3(256), reinterpret_cast<cudaStream_t>(stream), 0,
                                      cache_of(cache), len, (int)len_stride, n, reinterpret_cast<__nv_bfloat16*>(k_out),
                                      reinterpret_cast<__nv_bfloat16*>(v_out), ld_seq, ld_head, ld_row);
     return e == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
@@ -789,8 +954,7 @@ extern "C" int hxq_kv8_rows(const hxq_kv8* cache, const int64_t* len, int32_t le
 
 extern "C" size_t hxq_attn_decode_kv8_workspace_bytes(int32_t B, int32_t nq, int32_t nkv, int32_t D, int32_t max_len) {
     if (B <= 0 || nq <= 0 || nkv <= 0 || D <= 0 || max_len <= 0) return 0;
-    const int n = decode_splits(B, nkv, max_len);
-    return n == 1 ? 0 : (size_t)B * nq * n * (D + 2) * sizeof(float);
+    return (size_t)decode_ctas(B, nkv, max_len) * 2 * (nq / nkv) * (D + 2) * sizeof(float);
 }
 
 extern "C" int hxq_attn_decode_kv8(const hxq_kv8* cache, const void* q, int64_t ld_q, const int64_t* pos, int32_t pos_stride, void* out,
@@ -802,23 +966,20 @@ extern "C" int hxq_attn_decode_kv8(const hxq_kv8* cache, const void* q, int64_t 
     if (B > cache->slots || B > 65535 || nq % cache->nkv != 0 || nq / cache->nkv > kHeads || (pos_stride != 0 && pos_stride != 1)) return HXQ_E_SHAPE;
     if (ld_q < (int64_t)nq * cache->D || ld_out < (int64_t)nq * cache->D) return HXQ_E_SHAPE;
     if (!hxq::aligned_to(q, 16) || ld_q % 8 != 0) return HXQ_E_ALIGN;
-    DecodeArgs a;
-    a.splits = decode_splits(B, cache->nkv, cache->max_len);
-    if (a.splits > 1 && (!workspace || !hxq::aligned_to(workspace, 4) ||
-                         workspace_bytes < hxq_attn_decode_kv8_workspace_bytes(B, nq, cache->nkv, cache->D, cache->max_len)))
+    if (!workspace || !hxq::aligned_to(workspace, 4) || workspace_bytes < hxq_attn_decode_kv8_workspace_bytes(B, nq, cache->nkv, cache->D, cache->max_len))
         return HXQ_E_WORKSPACE;
+    DecodeArgs a;
     a.c = cache_of(cache);
     a.q = reinterpret_cast<const __nv_bfloat16*>(q);
     a.pos = pos;
     a.out = reinterpret_cast<__nv_bfloat16*>(out);
     a.part = reinterpret_cast<float*>(workspace);
     a.ld_q = ld_q; a.ld_out = ld_out;
-    a.pos_stride = pos_stride; a.nq = nq; a.G = nq / cache->nkv;
+    a.pos_stride = pos_stride; a.B = B; a.nq = nq; a.G = nq / cache->nkv;
+    a.ctas = decode_ctas(B, cache->nkv, cache->max_len);
     a.scale_log2 = scale * 1.4426950408889634f;
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-    const dim3 grid(a.splits, cache->nkv, B);
-    cudaError_t e = cache->D <= 64 ? launch_pdl(decode_kernel<64>, grid, dim3(32 * kWarps), stream, a)
-                                   : launch_pdl(decode_kernel<128>, grid, dim3(32 * kWarps), stream, a);
-    if (e == cudaSuccess && a.splits > 1) e = launch_pdl(combine_kernel, dim3(nq, B), dim3(kMaxD), stream, a);
+    cudaError_t e = cache->D <= 64 ? run_decode<64>(a, stream) : run_decode<128>(a, stream);
+    if (e == cudaSuccess) e = launch_pdl(combine_kernel, dim3(cache->nkv, a.G, B), dim3(kJoin * kMaxD), stream, 0, a);
     return e == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
 }
