@@ -343,15 +343,9 @@ __device__ __forceinline__ uint32_t bf2_of(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// Two biased bytes (code + 128), picked by sel out of x, as two exact fp16 integers: 0x64nn is 1024 + nn.
+// Two biased bytes (code + 128), picked by sel out of x, as two fp16 numbers 1024 + byte (0x64nn): the code + 1152, exactly.
 template <uint32_t SEL>
-__device__ __forceinline__ uint32_t codes2(uint32_t x) {
-    const uint32_t h = __byte_perm(x, 0x64646464u, SEL);
-    const uint32_t bias = 0x64806480u;      // 1152
-    uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(bias));
-    return r;
-}
+__device__ __forceinline__ uint32_t codes2(uint32_t x) { return __byte_perm(x, 0x64646464u, SEL); }
 __device__ __forceinline__ float quad_max(float v) {
     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
     return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
@@ -439,7 +433,7 @@ __device__ __forceinline__ Share find(const DecodeArgs& a, int cta, int at, int6
 
 // Every CTA takes the same number of units, whatever the sequences' lengths: a contiguous share of the row of all
 // units, i.e. a few segments, each of one sequence and KV head with all of its (up to eight) query heads.  In a segment a
-// warp takes units of 64 positions in turn, 32 positions at a step.  A segment that is a whole pair writes the output, the
+// warp takes units of 64 positions in turn.  A segment that is a whole pair writes the output, the
 // others partial results, which the next launch joins.
 //
 // Bound by HBM: each code is read once, 2 D bytes a position and KV head.  On the CUDA cores G query heads cost G
@@ -448,33 +442,34 @@ __device__ __forceinline__ Share find(const DecodeArgs& a, int cta, int at, int6
 //   * Q K^T runs in int8, the codes as they are.  A query row is rounded to 16 bits, a step of 2^-16 of its largest element
 //     (bf16 itself has steps of 2^-9 of each), as two int8 planes q = 256 hi + lo: heads' high parts are rows 0-7 of the
 //     MMA, low parts rows 8-15, and both sums of a score end in one lane.  They are exact; scales multiply in fp32.
-//   * P V runs in fp16 with fp32 sums: codes become fp16 exactly (two byte permutes and a subtraction for two), dimensions
-//     are the MMA's rows and heads its columns, which is how the scores' layout already holds P.  Probabilities are scaled by
+//   * P V runs in fp16 with fp32 sums: a code becomes the fp16 number code + 1152 (byte permutes alone), the sum starts at
+//     -1152 times the sum of the probabilities (32 positions at a time: it costs a hundredth of the output's rounding).
+//     Dimensions are the MMA's rows and heads its columns, which is how the scores' layout already holds P.  Probabilities are scaled by
 //     2^10 and rounded to fp16: 2^-12 relative (a sixteenth of the output's own rounding) down to 2^-24 of the largest, 2^-35
 //     of it absolute below that; the sum that divides takes them in fp32.
 //   * the order of a contraction's index is free, so it is chosen such that every lane's operands are 16 consecutive
-//     bytes of a cache row: no lane needs another's bytes.  They pass through a ring in shared memory that each lane
-//     fills (asynchronous copies) and reads back for itself: a step of 8 KB a warp is in flight while one is used, nothing
-//     but its own copies is waited for, and there are no bank conflicts (a slot of 16 bytes per lane).
+//     bytes of a cache row, read without bank conflicts.  Rows pass through a ring in shared memory, one per warp, filled by
+//     asynchronous copies of whole rows: pieces of 16 bytes trade places only within 128 (spread over a slot per lane, the copies
+//     took every sector twice and stopped at 4.3 TB/s).  The next unit's keys are fetched as soon as this one's are used, its values likewise:
+//     8 to 16 KB a warp are in flight.
 //   * the tail's products run in bf16, 16 positions to a warp, with each probability as the sum of two bf16 numbers (2^-17).
-constexpr int kStages = 2;
 template <int DP>
-struct DecodeSmem { static constexpr int bytes = kWarps * kStages * 64 * DP; };
+struct DecodeSmem { static constexpr int bytes = kWarps * 128 * DP; };
 
-template <int DP>
+template <int DP, bool FULL>
 __global__ void __launch_bounds__(32 * kWarps, kDecodeCtas) decode_kernel(const DecodeArgs a) {
     constexpr int KS = DP / 32;        // k steps of Q K^T
     constexpr int MT = DP / 16;        // m tiles of P V
     constexpr int KC = DP / 64;        // 16-byte pieces of a key row per lane
     constexpr int NT = DP / 8;         // bytes of a value row per lane
-    constexpr int STAGE = 64 * DP;     // a step's bytes: 32 positions of keys, then of values
-    extern __shared__ __align__(16) char ring_smem[];
+    constexpr int RING = 128 * DP;     // a unit of keys, then of values
+    extern __shared__ __align__(128) char ring_smem[];
     float (*o_s)[kHeads][DP] = reinterpret_cast<float (*)[kHeads][DP]>(ring_smem);      // at a segment's end, in the rings' place
     static_assert(sizeof(float) * kWarps * kHeads * DP <= DecodeSmem<DP>::bytes, "the sums fit");
     __shared__ float m_s[kWarps][kHeads], l_s[kWarps][kHeads];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int D = a.c.D;
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(ring_smem) + (uint32_t)(warp * kStages * STAGE);
+    const int D = FULL ? DP : a.c.D;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(ring_smem) + (uint32_t)(warp * RING);
     pdl_enter();
     int64_t total;
     const Share at = find(a, blockIdx.x, -1, total);
@@ -496,45 +491,54 @@ __global__ void __launch_bounds__(32 * kWarps, kDecodeCtas) decode_kernel(const 
         const int u_end = u1 < whole ? u1 : whole;
         const int64_t head = (int64_t)b * a.c.nkv + kvh;
         const __nv_bfloat16* q = a.q + (int64_t)b * a.ld_q + ((int64_t)kvh * a.G + (g < a.G ? g : 0)) * D;
-        const int8_t* kp = a.c.k + head * a.c.max_len * D + g * D + 16 * t;
-        const int8_t* vp = a.c.v + head * a.c.max_len * D + 2 * t * D + NT * g;
+        const int8_t* kp = a.c.k + head * a.c.max_len * D;
+        const int8_t* vp = a.c.v + head * a.c.max_len * D;
         const float* ksp = a.c.ks + head * (a.c.max_len / kBlock);
         const float* vsp = a.c.vs + head * (a.c.max_len / kBlock);
         const int first = u0 + warp;
-        const int steps = first < u_end ? 2 * ((u_end - first + kWarps - 1) / kWarps) : 0;       // of 32 positions
-        auto fetch = [&](int step, uint32_t st) {       // always one group
-            if (step < steps) {
-                const int64_t row = (int64_t)(first + (step >> 1) * kWarps) * kBlock + (step & 1) * 32;
-                const int8_t* k = kp + row * D;
-                const int8_t* v = vp + row * D;
+        // The copies of a unit's keys, or values, into their half of the ring: always one group.  Rows stay rows, eight lanes
+        // to 128 bytes; pieces of 16 bytes trade places within 128 (by the row, as the reads below want it).
+        const int c_cp = DP == 128 ? lane & 7 : lane & 3, r_cp = DP == 128 ? lane >> 3 : lane >> 2;        // this lane's piece and row
+        const int64_t off_cp = (int64_t)r_cp * D + 16 * c_cp;
+        const uint32_t k_cp = ring + (uint32_t)(DP == 128 ? r_cp * 128 + ((c_cp ^ ((r_cp & 1) << 2 | r_cp >> 1)) << 4) : lane * 16);
+        const uint32_t v_cp = ring + (uint32_t)(64 * DP + (DP == 128 ? r_cp * 128 + ((c_cp ^ r_cp) << 4)
+                                                                     : (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3 & 1) << 2 | (lane >> 4) << 1)) << 4)));
+        auto fetch_k = [&](int unit) {
+            if (unit < u_end && (FULL || 16 * c_cp < D)) {
+                const int8_t* k = kp + (int64_t)unit * kBlock * D + off_cp;
 #pragma unroll
-                for (int n = 0; n < 4; ++n)
-#pragma unroll
-                    for (int i = 0; i < KC; ++i) {
-                        const uint32_t bytes = 64 * i + 16 * t < D ? 16u : 0u;
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                                     :: "r"(st + (uint32_t)((n * KC + i) * 512 + lane * 16)), "l"(bytes ? k + n * 8 * D + 64 * i : kp), "r"(bytes) : "memory");
-                    }
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {       // rows 16 (j / 4) + 8 (j / 2 % 2) + 2 t + j % 2
-                    const int8_t* vr = v + (16 * (j >> 2) + 8 * ((j >> 1) & 1) + (j & 1)) * D;
-                    const uint32_t bytes = NT * g < D ? (uint32_t)NT : 0u;
-                    const uint32_t dst = st + (uint32_t)(32 * DP + j * 32 * NT + lane * NT);
-                    if constexpr (NT == 16)
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(bytes ? vr : vp - NT * g), "r"(bytes) : "memory");
-                    else
-                        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" :: "r"(dst), "l"(bytes ? vr : vp - NT * g), "r"(bytes) : "memory");
-                }
+                for (int i = 0; i < 8 * KC; ++i)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                                 :: "r"((k_cp ^ (uint32_t)(DP == 128 ? (i & 1) * 32 : 0)) + (uint32_t)(i * 512)), "l"(k + i * (DP == 128 ? 4 : 8) * D) : "memory");
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
+        auto fetch_v = [&](int unit) {
+            if (unit < u_end && (FULL || 16 * c_cp < D)) {
+                const int8_t* v = vp + (int64_t)unit * kBlock * D + off_cp;
+#pragma unroll
+                for (int i = 0; i < 8 * KC; ++i)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                                 :: "r"((v_cp ^ (uint32_t)(DP == 128 ? (i & 1) * 64 : 0)) + (uint32_t)(i * 512)), "l"(v + i * (DP == 128 ? 4 : 8) * D) : "memory");
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        // where this lane's operands are: keys of row 8 n + g, piece 4 i + t, and values of rows 8 k + 2 t + b, bytes NT g ..
+        const uint32_t k_rd = ring + (uint32_t)(DP == 128 ? g * 128 + ((t ^ ((g & 1) << 2 | g >> 1)) << 4) : lane * 16);
+        const uint32_t v_rd = ring + (uint32_t)(64 * DP + (DP == 128 ? t * 256 + ((g ^ 2 * t) << 4)
+                                                                     : t * 128 + (((g >> 1) ^ ((t & 1) << 2 | (t >> 1) << 1)) << 4) + 8 * (g & 1)));
         auto take = [&](uint32_t addr) {
             uint4 v;
             asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
             return v;
         };
-#pragma unroll
-        for (int k = 0; k < kStages - 1; ++k) fetch(k, ring + k * STAGE);
+        if (!FULL) {        // the slots of dimensions that there are not: zeros
+            for (int i = 0; i < RING / 512; ++i)
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" :: "r"(ring + (uint32_t)(i * 512 + lane * 16)), "r"(0u) : "memory");
+            __syncwarp();
+        }
+        fetch_k(first);
+        fetch_v(first);
 
         float o[MT][4];        // dimensions 16 g + 2 i and + 1 (rows g, g + 8) of heads 2 t and 2 t + 1
 #pragma unroll
@@ -563,7 +567,7 @@ __global__ void __launch_bounds__(32 * kWarps, kDecodeCtas) decode_kernel(const 
             m = mx;
         };
 
-        if (steps > 0) {
+        if (first < u_end) {
             float ks = ksp[first], vs = vsp[first], ks_next = 0.f, vs_next = 0.f;
             // query rows as int8 A operands: lane (g, t) holds the dimensions of the key pieces it loads
             uint32_t qa[KS][4];
@@ -613,76 +617,92 @@ __global__ void __launch_bounds__(32 * kWarps, kDecodeCtas) decode_kernel(const 
                             qa[2 * i + hh][2 * w + 1] = lo;
                         }
             }
-            uint32_t st = ring;
 #pragma unroll 1
-            for (int step = 0; step < steps; ++step) {
-                asm volatile("cp.async.wait_group %0;" :: "n"(kStages - 2) : "memory");      // this step has landed
-                fetch(step + kStages - 1, st == ring ? ring + (kStages - 1) * STAGE : st - STAGE);      // where the step before was
-                if ((step & 1) == 0) {
-                    const int next = first + ((step >> 1) + 1) * kWarps;
-                    if (next < u_end) { ks_next = ksp[next]; vs_next = vsp[next]; }
-                }
-                float s[8];
-                int c4[4][4];
+            for (int u = first; u < u_end; u += kWarps) {
+                const int next = u + kWarps;
+                if (next < u_end) { ks_next = ksp[next]; vs_next = vsp[next]; }
+                asm volatile("cp.async.wait_group 1;" ::: "memory");      // the keys have landed, their values are under way
+                __syncwarp();
+                float s[16];
+                int c4[8][4];
 #pragma unroll
-                for (int n = 0; n < 4; ++n) c4[n][0] = c4[n][1] = c4[n][2] = c4[n][3] = 0;
+                for (int n = 0; n < 8; ++n) c4[n][0] = c4[n][1] = c4[n][2] = c4[n][3] = 0;
 #pragma unroll
                 for (int i = 0; i < KC; ++i) {
-                    uint4 kr[4];
+                    uint4 kr[8];
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) kr[n] = take(st + (uint32_t)((n * KC + i) * 512 + lane * 16));
+                    for (int n = 0; n < 8; ++n) kr[n] = take((k_rd ^ (uint32_t)(i * 64)) + (uint32_t)(n * KC * 512));
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) mma_s8(c4[n], qa[2 * i], kr[n].x, kr[n].y);
+                    for (int n = 0; n < 8; ++n) mma_s8(c4[n], qa[2 * i], kr[n].x, kr[n].y);
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) mma_s8(c4[n], qa[2 * i + 1], kr[n].z, kr[n].w);
+                    for (int n = 0; n < 8; ++n) mma_s8(c4[n], qa[2 * i + 1], kr[n].z, kr[n].w);
                 }
                 const float back = ks * q_back;
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
+                for (int n = 0; n < 8; ++n) {
                     s[2 * n] = (float)(c4[n][0] * 256 + c4[n][2]) * back;
                     s[2 * n + 1] = (float)(c4[n][1] * 256 + c4[n][3]) * back;
                 }
-                softmax(s, 8);
-                uint32_t p[4];
+                __syncwarp();
+                fetch_k(next);                  // where these keys were
+                softmax(s, 16);
+                uint32_t p[8];
 #pragma unroll
-                for (int n = 0; n < 4; ++n) p[n] = half2_of(s[2 * n] * 1024.f, s[2 * n + 1] * 1024.f);
+                for (int n = 0; n < 8; ++n) p[n] = half2_of(s[2 * n] * 1024.f, s[2 * n + 1] * 1024.f);
                 const float vb = vs * (1.f / 1024.f);
-                uint4 vr[8];
+                asm volatile("cp.async.wait_group 1;" ::: "memory");      // and now the values
+                __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t src = st + (uint32_t)(32 * DP + j * 32 * NT + lane * NT);
-                    if constexpr (NT == 16) {
-                        vr[j] = take(src);
-                    } else {
-                        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(vr[j].x), "=r"(vr[j].y) : "r"(src) : "memory");
-                        vr[j].z = vr[j].w = 0u;
-                    }
-                }
+                for (int h = 0; h < 2; ++h) {                 // 32 positions
+                    uint4 vr[8];
 #pragma unroll
-                for (int w = 0; w < NT / 4; ++w) {            // four dimensions: two m tiles
-                    float c[2][4];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {             // sixteen positions
-                        uint32_t x[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint32_t v4[4] = {vr[4 * j + k].x, vr[4 * j + k].y, vr[4 * j + k].z, vr[4 * j + k].w};
-                            x[k] = v4[w] ^ 0x80808080u;
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t src = (v_rd ^ (uint32_t)((j & 1) * (DP == 128 ? 16 : 64))) + (uint32_t)((4 * h + (j >> 1)) * 8 * DP + (DP == 128 ? (j & 1) * 128 : 0));
+                        if constexpr (NT == 16) {
+                            vr[j] = take(src);
+                        } else {
+                            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(vr[j].x), "=r"(vr[j].y) : "r"(src) : "memory");
+                            vr[j].z = vr[j].w = 0u;
                         }
-                        const uint32_t a01 = __byte_perm(x[0], x[1], 0x5140), a23 = __byte_perm(x[0], x[1], 0x7362);
-                        const uint32_t b01 = __byte_perm(x[2], x[3], 0x5140), b23 = __byte_perm(x[2], x[3], 0x7362);
-                        mma_f16(c[0], codes2<0x4140>(a01), codes2<0x4342>(a01), codes2<0x4140>(b01), codes2<0x4342>(b01), p[2 * j], p[2 * j + 1]);
-                        mma_f16(c[1], codes2<0x4140>(a23), codes2<0x4342>(a23), codes2<0x4140>(b23), codes2<0x4342>(b23), p[2 * j], p[2 * j + 1]);
                     }
+                    float off[4] = {0.f, 0.f, 0.f, 0.f};       // sums of the rounded probabilities of heads 2 t and 2 t + 1: what the 1152 adds
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                    for (int j = 0; j < 2; ++j)
+                        mma_f16(off, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, p[4 * h + 2 * j], p[4 * h + 2 * j + 1]);
+                    off[0] *= -1152.f;
+                    off[1] *= -1152.f;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[2 * w + i][e] = fmaf(vb, c[i][e], o[2 * w + i][e]);
+                    for (int w = 0; w < NT / 4; ++w) {            // four dimensions: two m tiles
+                        float c[2][4];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            c[i][0] = c[i][2] = off[0];
+                            c[i][1] = c[i][3] = off[1];
+                        }
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {             // sixteen positions
+                            uint32_t x[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const uint32_t v4[4] = {vr[4 * j + k].x, vr[4 * j + k].y, vr[4 * j + k].z, vr[4 * j + k].w};
+                                x[k] = v4[w] ^ 0x80808080u;
+                            }
+                            const uint32_t p0 = p[4 * h + 2 * j], p1 = p[4 * h + 2 * j + 1];
+                            const uint32_t a01 = __byte_perm(x[0], x[1], 0x5140), a23 = __byte_perm(x[0], x[1], 0x7362);
+                            const uint32_t b01 = __byte_perm(x[2], x[3], 0x5140), b23 = __byte_perm(x[2], x[3], 0x7362);
+                            mma_f16(c[0], codes2<0x4140>(a01), codes2<0x4342>(a01), codes2<0x4140>(b01), codes2<0x4342>(b01), p0, p1);
+                            mma_f16(c[1], codes2<0x4140>(a23), codes2<0x4342>(a23), codes2<0x4140>(b23), codes2<0x4342>(b23), p0, p1);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[2 * w + i][e] = fmaf(vb, c[i][e], o[2 * w + i][e]);
+                    }
                 }
-                st = st + STAGE == ring + kStages * STAGE ? ring : st + STAGE;
-                if (step & 1) { ks = ks_next; vs = vs_next; }
+                __syncwarp();
+                fetch_v(next);                  // where these values were
+                ks = ks_next;
+                vs = vs_next;
             }
         }
 
@@ -903,17 +923,17 @@ static int decode_ctas(int B, int nkv, int max_len) {
     return (int)(n < most ? (n < 1 ? 1 : n) : most);
 }
 
-template <int DP>
+template <int DP, bool FULL>
 static cudaError_t run_decode(const DecodeArgs& a, cudaStream_t stream) {
     static bool attr_set[64] = {false};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if (!attr_set[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(decode_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeSmem<DP>::bytes);
+        const cudaError_t e = cudaFuncSetAttribute(decode_kernel<DP, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeSmem<DP>::bytes);
         if (e != cudaSuccess) return e;
         attr_set[dev] = true;
     }
-    return launch_pdl(decode_kernel<DP>, dim3(a.ctas), dim3(32 * kWarps), stream, DecodeSmem<DP>::bytes, a);
+    return launch_pdl(decode_kernel<DP, FULL>, dim3(a.ctas), dim3(32 * kWarps), stream, DecodeSmem<DP>::bytes, a);
 }
 
 }  // namespace kv8
@@ -979,7 +999,9 @@ extern "C" int hxq_attn_decode_kv8(const hxq_kv8* cache, const void* q, int64_t 
     a.ctas = decode_ctas(B, cache->nkv, cache->max_len);
     a.scale_log2 = scale * 1.4426950408889634f;
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-    cudaError_t e = cache->D <= 64 ? run_decode<64>(a, stream) : run_decode<128>(a, stream);
+    const int D = cache->D;
+    cudaError_t e = D == 128 ? run_decode<128, true>(a, stream) : D > 64 ? run_decode<128, false>(a, stream)
+                    : D == 64 ? run_decode<64, true>(a, stream) : run_decode<64, false>(a, stream);
     if (e == cudaSuccess) e = launch_pdl(combine_kernel, dim3(cache->nkv, a.G, B), dim3(kJoin * kMaxD), stream, 0, a);
     return e == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
 }
