@@ -320,6 +320,7 @@ __global__ void __launch_bounds__(256) rows_kernel(const Cache c, const int64_t*
 
 constexpr int kWarps = 4;
 constexpr int kDecodeCtas = 3;      // per SM
+constexpr int kCluster = 8;
 constexpr int kHeads = 8;           // query heads of a KV head: the used rows of an MMA's sixteen
 
 // d (+)= a * b, one warp: int8 with 32 dimensions, fp16 and bf16 with 16.
@@ -378,63 +379,57 @@ struct DecodeArgs {
     float scale_log2;       // scale * log2(e)
 };
 
-// The units of all (sequence, KV head) pairs in a row, sequence by sequence, head by head: where the share of a CTA starts.
-// Every warp works it out for itself from the positions.
+// The units of all (sequence, KV head) pairs in a row, sequence by sequence, head by head, each pair followed by kPad empty
+// ones, which stand for what a segment costs besides its units (queries, the sums' meeting: about four units' time; without
+// them a CTA with many short pairs would be the last to finish).  Where the share of a CTA starts, every warp works
+// out for itself from the positions.
+constexpr int kPad = 4;
 struct Share {
-    int64_t per;        // units per CTA
-    int64_t before;     // units of the sequences before b, of one head
-    int b, units;       // the sequence that holds the given unit (or sequence `at`), and its units
+    int64_t per;        // places per CTA
+    int64_t before;     // places of the sequences before b, of one head
+    int b, units;       // the sequence that holds the given place (or sequence `at`), and its units
 };
-// Where flat unit `flat` (>= 0) lies, or, with flat < 0, sequence `at`.
+// The share that place per * cta lies in, or, with at >= 0, sequence `at`.  b < 0: past the end.
 __device__ __forceinline__ Share find(const DecodeArgs& a, int cta, int at, int64_t& total) {
     const int lane = threadIdx.x & 31;
+    auto padded = [](int u) { return u > 0 ? u + kPad : 0; };
+    auto units = [&](int b) { return b < a.B ? units_of(a.pos[(int64_t)b * a.pos_stride], a.c.max_len) : 0; };
     Share r;
-    int64_t sum = 0;
-    if (a.pos_stride == 0) {            // all alike
-        r.units = units_of(a.pos[0], a.c.max_len);
-        sum = (int64_t)r.units * a.B;
-    } else {
-        for (int b0 = 0; b0 < a.B; b0 += 32) {
-            int u = b0 + lane < a.B ? units_of(a.pos[b0 + lane], a.c.max_len) : 0;
-            sum += __reduce_add_sync(0xffffffffu, u);
-        }
-    }
+    const int first = units(lane);
+    int64_t sum = __reduce_add_sync(0xffffffffu, padded(first));
+    for (int b0 = 32; b0 < a.B; b0 += 32) sum += __reduce_add_sync(0xffffffffu, padded(units(b0 + lane)));
     total = sum * a.c.nkv;
     r.per = (total + a.ctas - 1) / a.ctas;
     if (r.per < kWarps) r.per = kWarps;       // a unit for each warp at least
-    const int64_t flat = at < 0 ? r.per * cta : 0;
-    if (at < 0 && flat >= total) { r.b = -1; r.before = 0; r.units = 0; return r; }
-    if (a.pos_stride == 0) {
-        r.b = at < 0 ? (int)(flat / ((int64_t)r.units * a.c.nkv)) : at;
-        r.before = (int64_t)r.b * r.units;
-        return r;
-    }
-    int64_t before = 0;
-    for (int b0 = 0;; b0 += 32) {
-        const int u = b0 + lane < a.B ? units_of(a.pos[b0 + lane], a.c.max_len) : 0;
-        int incl = u;
+    const int64_t place = r.per * cta;
+    r.b = -1; r.before = 0; r.units = 0;
+    if (at < 0 && place >= total) return r;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+        const int u = b0 == 0 ? first : units(b0 + lane);
+        int incl = padded(u);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += v;
         }
-        const uint32_t hit = at < 0 ? __ballot_sync(0xffffffffu, (before + incl) * a.c.nkv > flat)
-                                    : (at - b0 < 32 ? 1u << (at - b0) : 0u);
-        if (hit != 0u || b0 + 32 >= a.B) {
-            const int l = hit != 0u ? __ffs(hit) - 1 : 31;
+        const uint32_t hit = at < 0 ? __ballot_sync(0xffffffffu, (r.before + incl) * a.c.nkv > place) : (at < b0 + 32 ? 1u << (at - b0) : 0u);
+        if (hit != 0u) {
+            const int l = __ffs(hit) - 1;
             r.b = b0 + l;
             r.units = __shfl_sync(0xffffffffu, u, l);
-            r.before = before + __shfl_sync(0xffffffffu, incl, l) - r.units;
+            r.before += __shfl_sync(0xffffffffu, incl - padded(u), l);
             return r;
         }
-        before += __shfl_sync(0xffffffffu, incl, 31);
+        r.before += __shfl_sync(0xffffffffu, incl, 31);
     }
+    return r;
 }
 
-// Every CTA takes the same number of units, whatever the sequences' lengths: a contiguous share of the row of all
-// units, i.e. a few segments, each of one sequence and KV head with all of its (up to eight) query heads.  In a segment a
-// warp takes units of 64 positions in turn.  A segment that is a whole pair writes the output, the
-// others partial results, which the next launch joins.
+// Every CTA takes the same share of all units, whatever the sequences' lengths: a few segments, each of one sequence and
+// KV head with all of its (up to eight) query heads.  In a segment a warp takes units of 64 positions in turn.  A segment
+// that is a whole pair writes the output, the others partial results, which the next launch joins.
+// CLUSTER, for few pairs and short caches: a pair has a cluster of eight CTAs, whose results meet over their shared
+// memories, and there is no next launch.
 //
 // Bound by HBM: each code is read once, 2 D bytes a position and KV head.  On the CUDA cores G query heads cost G
 // multiply-adds a code, more than the cores have at the memory's pace from G = 5 on, so both products go through
@@ -456,7 +451,7 @@ __device__ __forceinline__ Share find(const DecodeArgs& a, int cta, int at, int6
 template <int DP>
 struct DecodeSmem { static constexpr int bytes = kWarps * 128 * DP; };
 
-template <int DP, bool FULL>
+template <int DP, bool FULL, bool CLUSTER>
 __global__ void __launch_bounds__(32 * kWarps, kDecodeCtas) decode_kernel(const DecodeArgs a) {
     constexpr int KS = DP / 32;        // k steps of Q K^T
     constexpr int MT = DP / 16;        // m tiles of P V
@@ -465,27 +460,41 @@ __global__ void __launch_bounds__(32 * kWarps, kDecodeCtas) decode_kernel(const 
     constexpr int RING = 128 * DP;     // a unit of keys, then of values
     extern __shared__ __align__(128) char ring_smem[];
     float (*o_s)[kHeads][DP] = reinterpret_cast<float (*)[kHeads][DP]>(ring_smem);      // at a segment's end, in the rings' place
-    static_assert(sizeof(float) * kWarps * kHeads * DP <= DecodeSmem<DP>::bytes, "the sums fit");
-    __shared__ float m_s[kWarps][kHeads], l_s[kWarps][kHeads];
+    static_assert(sizeof(float) * (kWarps + 1) * kHeads * DP <= DecodeSmem<DP>::bytes, "the sums fit");
+    __shared__ float m_s[kWarps][kHeads], l_s[kWarps][kHeads], m_c[kHeads], l_c[kHeads];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int D = FULL ? DP : a.c.D;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(ring_smem) + (uint32_t)(warp * RING);
     pdl_enter();
-    int64_t total;
-    const Share at = find(a, blockIdx.x, -1, total);
-    if (at.b < 0) return;
-    int64_t flat = at.per * blockIdx.x;
-    const int64_t flat_end = flat + at.per < total ? flat + at.per : total;
-    int b = at.b, units = at.units;
-    int64_t pair0 = at.before * a.c.nkv;           // flat unit at which head kvh of sequence b starts
-    int kvh = (int)((flat - pair0) / units);
-    pair0 += (int64_t)kvh * units;
-    int slot = 0;
+    int b, kvh, units;
+    int64_t flat = 0, flat_end = 0, pair0 = 0;     // this CTA's places, and the place at which the pair starts
+    if (CLUSTER) {
+        const int pair = blockIdx.x / kCluster, rank = blockIdx.x % kCluster;
+        b = pair / a.c.nkv;
+        kvh = pair - b * a.c.nkv;
+        units = units_of(a.pos[(int64_t)b * a.pos_stride], a.c.max_len);
+        const int per = (units + kCluster - 1) / kCluster;
+        flat = rank * per < units ? rank * per : units;
+        flat_end = flat + per < units ? flat + per : units;
+    } else {
+        int64_t total;
+        const Share at = find(a, blockIdx.x, -1, total);
+        if (at.b < 0) return;
+        flat = at.per * blockIdx.x;
+        flat_end = flat + at.per < total ? flat + at.per : total;
+        b = at.b;
+        units = at.units;
+        pair0 = at.before * a.c.nkv;
+        kvh = (int)((flat - pair0) / (units + kPad));
+        pair0 += (int64_t)kvh * (units + kPad);
+    }
+    const int64_t start = flat;
 
     while (true) {          // segments
         const int64_t pos = a.pos[(int64_t)b * a.pos_stride];
-        const int u0 = (int)(flat - pair0);
+        const int u0 = flat - pair0 < units ? (int)(flat - pair0) : units;
         const int u1 = flat_end - pair0 < units ? (int)(flat_end - pair0) : units;
+        if (CLUSTER || u0 < u1) {
         const int tail_n = (int)((pos + 1) % kBlock);        // rows of the unfinished block
         const int whole = tail_n ? units - 1 : units;        // units below this one are finished blocks
         const int u_end = u1 < whole ? u1 : whole;
@@ -566,6 +575,62 @@ __global__ void __launch_bounds__(32 * kWarps, kDecodeCtas) decode_kernel(const 
             }
             m = mx;
         };
+
+        // the unfinished block first, while the copies are under way: bf16 rows, sixteen positions to a warp
+        if (u0 < u1 && u1 == units && 16 * warp < tail_n) {
+            const __nv_bfloat16* kt = a.c.kt + head * kBlock * D;
+            const __nv_bfloat16* vt = a.c.vt + head * kBlock * D;
+            const int p = 16 * warp;
+            float s[4];
+            uint32_t qb[KC * 2][4];
+#pragma unroll
+            for (int i = 0; i < 2 * KC; ++i) {
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (32 * i + 8 * t < D && g < a.G) w = ld16(q + 32 * i + 8 * t);
+                qb[i][0] = w.x; qb[i][1] = w.y; qb[i][2] = w.z; qb[i][3] = w.w;
+            }
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int row = p + 8 * n + g;
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < 2 * KC; ++i) {
+                    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                    if (32 * i + 8 * t < D && row < tail_n) w = ld16(kt + row * D + 32 * i + 8 * t);
+                    mma_bf16(c, qb[i][0], 0u, qb[i][1], 0u, w.x, w.y);
+                    mma_bf16(c, qb[i][2], 0u, qb[i][3], 0u, w.z, w.w);
+                }
+                const int col = p + 8 * n + 2 * t;
+                s[2 * n] = col < tail_n ? c[0] * a.scale_log2 : -INFINITY;
+                s[2 * n + 1] = col + 1 < tail_n ? c[1] * a.scale_log2 : -INFINITY;
+            }
+            softmax(s, 4);
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const float h0 = __bfloat162float(__float2bfloat16_rn(s[2 * n])), h1 = __bfloat162float(__float2bfloat16_rn(s[2 * n + 1]));
+                hi[n] = bf2_of(h0, h1);
+                lo[n] = bf2_of(s[2 * n] - h0, s[2 * n + 1] - h1);
+            }
+#pragma unroll
+            for (int n0 = 0; n0 < NT; n0 += 8) {          // eight dimensions of four rows at a time
+                uint4 w[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int row = p + 2 * t + (k & 1) + 8 * (k >> 1);
+                    w[k] = make_uint4(0u, 0u, 0u, 0u);
+                    if (NT * g + n0 < D && row < tail_n) w[k] = ld16(vt + row * D + NT * g + n0);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {             // a word is two dimensions: rows g and g + 8 of an m tile
+                    const uint32_t x0 = (&w[0].x)[e], x1 = (&w[1].x)[e], x2 = (&w[2].x)[e], x3 = (&w[3].x)[e];
+                    const uint32_t a0 = __byte_perm(x0, x1, 0x5410), a1 = __byte_perm(x0, x1, 0x7632);
+                    const uint32_t a2 = __byte_perm(x2, x3, 0x5410), a3 = __byte_perm(x2, x3, 0x7632);
+                    mma_bf16(o[n0 / 2 + e], a0, a1, a2, a3, hi[0], hi[1]);
+                    mma_bf16(o[n0 / 2 + e], a0, a1, a2, a3, lo[0], lo[1]);
+                }
+            }
+        }
 
         if (first < u_end) {
             float ks = ksp[first], vs = vsp[first], ks_next = 0.f, vs_next = 0.f;
@@ -706,62 +771,6 @@ __global__ void __launch_bounds__(32 * kWarps, kDecodeCtas) decode_kernel(const 
             }
         }
 
-        // the unfinished block: bf16 rows, sixteen positions to a warp
-        if (u1 == units && 16 * warp < tail_n) {
-            const __nv_bfloat16* kt = a.c.kt + head * kBlock * D;
-            const __nv_bfloat16* vt = a.c.vt + head * kBlock * D;
-            const int p = 16 * warp;
-            float s[4];
-            uint32_t qb[KC * 2][4];
-#pragma unroll
-            for (int i = 0; i < 2 * KC; ++i) {
-                uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if (32 * i + 8 * t < D && g < a.G) w = ld16(q + 32 * i + 8 * t);
-                qb[i][0] = w.x; qb[i][1] = w.y; qb[i][2] = w.z; qb[i][3] = w.w;
-            }
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const int row = p + 8 * n + g;
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < 2 * KC; ++i) {
-                    uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                    if (32 * i + 8 * t < D && row < tail_n) w = ld16(kt + row * D + 32 * i + 8 * t);
-                    mma_bf16(c, qb[i][0], 0u, qb[i][1], 0u, w.x, w.y);
-                    mma_bf16(c, qb[i][2], 0u, qb[i][3], 0u, w.z, w.w);
-                }
-                const int col = p + 8 * n + 2 * t;
-                s[2 * n] = col < tail_n ? c[0] * a.scale_log2 : -INFINITY;
-                s[2 * n + 1] = col + 1 < tail_n ? c[1] * a.scale_log2 : -INFINITY;
-            }
-            softmax(s, 4);
-            uint32_t hi[2], lo[2];
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const float h0 = __bfloat162float(__float2bfloat16_rn(s[2 * n])), h1 = __bfloat162float(__float2bfloat16_rn(s[2 * n + 1]));
-                hi[n] = bf2_of(h0, h1);
-                lo[n] = bf2_of(s[2 * n] - h0, s[2 * n + 1] - h1);
-            }
-#pragma unroll
-            for (int n0 = 0; n0 < NT; n0 += 8) {          // eight dimensions of four rows at a time
-                uint4 w[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int row = p + 2 * t + (k & 1) + 8 * (k >> 1);
-                    w[k] = make_uint4(0u, 0u, 0u, 0u);
-                    if (NT * g + n0 < D && row < tail_n) w[k] = ld16(vt + row * D + NT * g + n0);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {             // a word is two dimensions: rows g and g + 8 of an m tile
-                    const uint32_t x0 = (&w[0].x)[e], x1 = (&w[1].x)[e], x2 = (&w[2].x)[e], x3 = (&w[3].x)[e];
-                    const uint32_t a0 = __byte_perm(x0, x1, 0x5410), a1 = __byte_perm(x0, x1, 0x7632);
-                    const uint32_t a2 = __byte_perm(x2, x3, 0x5410), a3 = __byte_perm(x2, x3, 0x7632);
-                    mma_bf16(o[n0 / 2 + e], a0, a1, a2, a3, hi[0], hi[1]);
-                    mma_bf16(o[n0 / 2 + e], a0, a1, a2, a3, lo[0], lo[1]);
-                }
-            }
-        }
-
         // ---- the four warps' (m, l, o) meet
         asm volatile("cp.async.wait_all;" ::: "memory");
         l = quad_sum(l);
@@ -774,6 +783,7 @@ __global__ void __launch_bounds__(32 * kWarps, kDecodeCtas) decode_kernel(const 
         }
         __syncthreads();
         const bool all = u0 == 0 && u1 == units;
+        float* o_c = reinterpret_cast<float*>(ring_smem) + kWarps * kHeads * DP;      // CLUSTER: this CTA's [G][D]
         for (int i = threadIdx.x; i < a.G * D; i += 32 * kWarps) {
             const int hd = i / D, d = i - hd * D;
             float mx = m_s[0][hd];
@@ -787,23 +797,58 @@ __global__ void __launch_bounds__(32 * kWarps, kDecodeCtas) decode_kernel(const 
                 ov += e * o_s[w][hd][d];
                 lv += e * l_s[w][hd];
             }
-            if (all) {
+            if (CLUSTER) {
+                o_c[i] = ov;
+                if (d == 0) { m_c[hd] = mx; l_c[hd] = lv; }
+            } else if (all) {
                 a.out[(int64_t)b * a.ld_out + ((int64_t)kvh * a.G + hd) * D + d] = __float2bfloat16_rn(ov / lv);
             } else {
-                float* dst = a.part + (((int64_t)blockIdx.x * 2 + slot) * a.G + hd) * (D + 2);
+                // (of a pair that started before this CTA, or with it, and of the one that it leaves unfinished)
+                float* dst = a.part + (((int64_t)blockIdx.x * 2 + (pair0 <= start ? 0 : 1)) * a.G + hd) * (D + 2);
                 dst[2 + d] = ov;
                 if (d == 0) { dst[0] = mx; dst[1] = lv; }
             }
         }
-        slot = 1;
-        flat = pair0 + u1;
-        if (flat >= flat_end) return;
         __syncthreads();              // the sums have been read
-        pair0 = flat;                 // the next pair
+        }
+        if (CLUSTER) break;
+        flat = pair0 + units + kPad;  // the next pair
+        if (flat >= flat_end) return;
+        pair0 = flat;
         if (++kvh == a.c.nkv) {
             kvh = 0;
             do units = units_of(a.pos[(int64_t)(++b) * a.pos_stride], a.c.max_len); while (units == 0);
         }
+    }
+    if (CLUSTER) {
+        const uint32_t o_at = (uint32_t)__cvta_generic_to_shared(ring_smem) + sizeof(float) * kWarps * kHeads * DP;
+        const uint32_t m_at = (uint32_t)__cvta_generic_to_shared(m_c), l_at = (uint32_t)__cvta_generic_to_shared(l_c);
+        auto peer = [](uint32_t addr, int rank) {       // a float of another CTA of the cluster
+            uint32_t at;
+            float v;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+            return v;
+        };
+        asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+        const int rank = blockIdx.x % kCluster, n = a.G * D, share = (n + kCluster - 1) / kCluster;
+        const int end = (rank + 1) * share < n ? (rank + 1) * share : n;
+        for (int i = rank * share + threadIdx.x; i < end; i += 32 * kWarps) {
+            const int hd = i / D;
+            float mv[kCluster], mx = -INFINITY, ov = 0.f, lv = 0.f;
+#pragma unroll
+            for (int c = 0; c < kCluster; ++c) { mv[c] = peer(m_at + 4u * hd, c); mx = fmaxf(mx, mv[c]); }
+            const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+            for (int c = 0; c < kCluster; ++c) {
+                const float e = ex2(mv[c] - ref);
+                ov += e * peer(o_at + 4u * i, c);
+                lv += e * peer(l_at + 4u * hd, c);
+            }
+            // (a sequence with nothing to see: zeros; NaN passes)
+            a.out[(int64_t)b * a.ld_out + (int64_t)kvh * n + i] = __float2bfloat16_rn(units == 0 ? 0.f : ov / lv);
+        }
+        asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");     // nobody leaves while it is read
     }
 }
 
@@ -823,10 +868,10 @@ __global__ void __launch_bounds__(kJoin * kMaxD) combine_kernel(const DecodeArgs
         if (tid < D) out[tid] = __float2bfloat16_rn(0.f);
         return;
     }
-    const int64_t s = at.before * a.c.nkv + (int64_t)kvh * at.units, e = s + at.units;
+    const int64_t s = at.before * a.c.nkv + (int64_t)kvh * (at.units + kPad), e = s + at.units;
     const int c0 = (int)(s / at.per), n = (int)((e - 1) / at.per) - c0 + 1;
     if (n == 1) return;           // one CTA had it all and wrote it
-    // the CTA that a pair starts in has it as its first segment, or as its last; the others as their first
+    // the CTA that a pair starts in has it in its first slot if it starts there, too, the others always
     const int64_t step = 2 * (int64_t)a.G * (D + 2);
     const float* base = a.part + c0 * step + (int64_t)hd * (D + 2);
     const int64_t skip = s == c0 * at.per ? 0 : step / 2;
@@ -916,24 +961,49 @@ static int run_append(const hxq_kv8* c, const void* qkv, int64_t ld_qkv, int32_t
     return e == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
 }
 
-// CTAs: as many as fit, fewer where a full cache has not that many times four units.
+// A cluster of eight CTAs for each (sequence, KV head) pair, where that many are resident at once and no warp has more than
+// four units of a full cache to walk.
+static bool decode_clustered(int B, int nkv, int max_len) {
+    return (int64_t)B * nkv * kCluster <= kDecodeCtas * 148 && max_len <= kBlock * kCluster * kWarps * 4;
+}
+// Otherwise CTAs as many as fit, fewer where a full cache has not that many times four units.
 static int decode_ctas(int B, int nkv, int max_len) {
-    const int64_t units = (int64_t)(max_len / kBlock) * B * nkv, n = (units + kWarps - 1) / kWarps;
+    const int64_t units = (int64_t)(max_len / kBlock + kPad) * B * nkv, n = (units + kWarps - 1) / kWarps;
     const int most = kDecodeCtas * 148;
-    return (int)(n < most ? (n < 1 ? 1 : n) : most);
+    return (int)(n < most ? n : most);
 }
 
-template <int DP, bool FULL>
+template <int DP, bool FULL, bool CLUSTER>
 static cudaError_t run_decode(const DecodeArgs& a, cudaStream_t stream) {
     static bool attr_set[64] = {false};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    const auto kernel = decode_kernel<DP, FULL, CLUSTER>;
     if (!attr_set[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(decode_kernel<DP, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeSmem<DP>::bytes);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeSmem<DP>::bytes);
         if (e != cudaSuccess) return e;
         attr_set[dev] = true;
     }
-    return launch_pdl(decode_kernel<DP, FULL>, dim3(a.ctas), dim3(32 * kWarps), stream, DecodeSmem<DP>::bytes, a);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(CLUSTER ? a.B * a.c.nkv * kCluster : a.ctas);
+    cfg.blockDim = dim3(32 * kWarps);
+    cfg.stream = stream;
+    cfg.dynamicSmemBytes = DecodeSmem<DP>::bytes;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = kCluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = CLUSTER ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+template <bool CLUSTER>
+static cudaError_t run_decode(const DecodeArgs& a, cudaStream_t stream) {
+    const int D = a.c.D;
+    return D == 128 ? run_decode<128, true, CLUSTER>(a, stream) : D > 64 ? run_decode<128, false, CLUSTER>(a, stream)
+           : D == 64 ? run_decode<64, true, CLUSTER>(a, stream) : run_decode<64, false, CLUSTER>(a, stream);
 }
 
 }  // namespace kv8
@@ -974,6 +1044,7 @@ extern "C" int hxq_kv8_rows(const hxq_kv8* cache, const int64_t* len, int32_t le
 
 extern "C" size_t hxq_attn_decode_kv8_workspace_bytes(int32_t B, int32_t nq, int32_t nkv, int32_t D, int32_t max_len) {
     if (B <= 0 || nq <= 0 || nkv <= 0 || D <= 0 || max_len <= 0) return 0;
+    if (decode_clustered(B, nkv, max_len)) return 0;
     return (size_t)decode_ctas(B, nkv, max_len) * 2 * (nq / nkv) * (D + 2) * sizeof(float);
 }
 
@@ -986,7 +1057,8 @@ extern "C" int hxq_attn_decode_kv8(const hxq_kv8* cache, const void* q, int64_t 
     if (B > cache->slots || B > 65535 || nq % cache->nkv != 0 || nq / cache->nkv > kHeads || (pos_stride != 0 && pos_stride != 1)) return HXQ_E_SHAPE;
     if (ld_q < (int64_t)nq * cache->D || ld_out < (int64_t)nq * cache->D) return HXQ_E_SHAPE;
     if (!hxq::aligned_to(q, 16) || ld_q % 8 != 0) return HXQ_E_ALIGN;
-    if (!workspace || !hxq::aligned_to(workspace, 4) || workspace_bytes < hxq_attn_decode_kv8_workspace_bytes(B, nq, cache->nkv, cache->D, cache->max_len))
+    const bool clustered = decode_clustered(B, cache->nkv, cache->max_len);
+    if (!clustered && (!workspace || !hxq::aligned_to(workspace, 4) || workspace_bytes < hxq_attn_decode_kv8_workspace_bytes(B, nq, cache->nkv, cache->D, cache->max_len)))
         return HXQ_E_WORKSPACE;
     DecodeArgs a;
     a.c = cache_of(cache);
@@ -999,9 +1071,8 @@ extern "C" int hxq_attn_decode_kv8(const hxq_kv8* cache, const void* q, int64_t 
     a.ctas = decode_ctas(B, cache->nkv, cache->max_len);
     a.scale_log2 = scale * 1.4426950408889634f;
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
-    const int D = cache->D;
-    cudaError_t e = D == 128 ? run_decode<128, true>(a, stream) : D > 64 ? run_decode<128, false>(a, stream)
-                    : D == 64 ? run_decode<64, true>(a, stream) : run_decode<64, false>(a, stream);
+    if (clustered) return run_decode<true>(a, stream) == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
+    cudaError_t e = run_decode<false>(a, stream);
     if (e == cudaSuccess) e = launch_pdl(combine_kernel, dim3(cache->nkv, a.G, B), dim3(kJoin * kMaxD), stream, 0, a);
     return e == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
 }

@@ -179,9 +179,9 @@ def attn_decode_kv8(q: torch.Tensor, cache: Kv8Cache, pos: torch.Tensor, out: to
     nb = _ws_bytes.get(key)
     if nb is None:
         nb = _ws_bytes[key] = _lib.lib().hxq_attn_decode_kv8_workspace_bytes(*key)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
     _call(dev, "hxq_attn_decode_kv8", cache._ref, q.data_ptr(), q.stride(0), pos.data_ptr(), stride, out.data_ptr(), out.stride(0),
-          ws.data_ptr(), nb, B, nq, scale)
+          None if ws is None else ws.data_ptr(), nb, B, nq, scale)
     return out
 
 

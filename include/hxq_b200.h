@@ -303,7 +303,7 @@ int hxq_rope_append_prompt_kv8(const hxq_kv8* cache, const void* qkv, int64_t ld
 
 /* hxq_attn_decode over an 8-bit cache: positions 0 .. pos[b] of slot b, the finished blocks from their codes, the
  * last one from the tail.  A position < 0 or >= max_len gives zeros.  nq / nkv <= 8.  workspace:
- * hxq_attn_decode_kv8_workspace_bytes() of plain scratch. */
+ * hxq_attn_decode_kv8_workspace_bytes() of plain scratch (0: none needed). */
 size_t hxq_attn_decode_kv8_workspace_bytes(int32_t B, int32_t nq, int32_t nkv, int32_t D, int32_t max_len);
 int hxq_attn_decode_kv8(const hxq_kv8* cache, const void* q, int64_t ld_q, const int64_t* pos, int32_t pos_stride,
                         void* out, int64_t ld_out, void* workspace, size_t workspace_bytes, int32_t B, int32_t nq,

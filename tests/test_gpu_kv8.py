@@ -257,6 +257,29 @@ def test_attn_decode_kv8_values(case):
         assert rel_l2(got[s][~nan], want[~nan]) < TOL, case
 
 
+@pytest.mark.parametrize("nq,nkv,D", [(4, 2, 64), (7, 1, 128), (2, 1, 112)])
+@pytest.mark.parametrize("B", [14, 33, 70, 130])
+def test_attn_decode_kv8_many_sequences(nq, nkv, D, B):
+    """More sequences than a warp has lanes, lengths from nothing to many blocks, idle slots in between and at both ends: every
+    CTA finds its share; all at one position too."""
+    from helix_substrate_b200.kv8 import attn_decode_kv8
+    dev, max_len = _dev(), 1280
+    g = torch.Generator().manual_seed(B)
+    lens = [0, 0] + [int(x) for x in torch.randint(0, 1281, (B - 4,), generator=g) // torch.randint(1, 20, (B - 4,), generator=g)] + [1280, 0]
+    cache, ref = _filled(B, nkv, max_len, D, lens, seed=B)
+    q = torch.randn(B, nq * D, generator=g).bfloat16()
+    out = torch.full((B, nq * D), 5.0, device=dev, dtype=torch.bfloat16)
+    attn_decode_kv8(q.to(dev), cache, torch.tensor([n - 1 for n in lens], device=dev), out, nq, 0.2)
+    for s, n in enumerate(lens):
+        want = attention(q[s].view(nq, 1, D), ref.values("k", s), ref.values("v", s), 0.2)[:, 0].reshape(-1) if n else torch.zeros(nq * D).double()
+        assert (not bool(out[s].any()) if n == 0 else rel_l2(out[s].cpu().double(), want) < TOL), (s, n)
+    held = [s for s, n in enumerate(lens) if n > 66]
+    attn_decode_kv8(q.to(dev), cache, torch.tensor([63], device=dev), out, nq, 0.2)      # the first block of everybody
+    for s in held[:5] + held[-5:]:
+        want = attention(q[s].view(nq, 1, D), ref.values("k", s)[:, :64], ref.values("v", s)[:, :64], 0.2)[:, 0].reshape(-1)
+        assert rel_l2(out[s].cpu().double(), want) < TOL, s
+
+
 def test_a_long_cache_past_32_bit_offsets():
     """Slots whose codes lie beyond 2^31 bytes: appended to, read, attended to."""
     from helix_substrate_b200.kv8 import Kv8Cache, attn_decode_kv8, kv8_rows, rope_append_kv8
