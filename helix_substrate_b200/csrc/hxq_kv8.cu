@@ -72,26 +72,63 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 }
 __device__ __forceinline__ uint4 ld16(const void* p) { return *reinterpret_cast<const uint4*>(p); }
 
-// x cos - y sin in 64 bits (the products are exact there), rounded to bf16: a value next to a border of bf16 lands on
-// the side it is on, whatever the order of the operations elsewhere.
-__device__ __forceinline__ float turn(float x, float c, float y, float s) {
-    return __bfloat162float(__float2bfloat16_rn(__double2float_rn((double)x * (double)c + (double)y * (double)s)));
+// Rotary embedding of the pieces at d and d + D / 2 of one head, packed bf16 in and out: x cos + y sin as 64-bit arithmetic
+// has it (its products are exact there), rounded to fp32 and to bf16, so that a value next to a border lands on the side it is
+// on.  Nearly always fp32 tells the same: r = fma(x, cos, fl(y sin)) is off by 2^-24 (|y sin| + |r|) at most and the
+// true sum's fp32 value by one more rounding, so where r - d and r + d, d = 2^-23 (|y sin| + |r|), round to the same bf16, that is
+// it.  One value in some 2^13 takes the 64-bit path.  (All in 64 bits, conversions alone filled half of the time: 86 us for 8191
+// tokens of 28 + 4 heads, 31 as it is.)
+__device__ __forceinline__ uint32_t turn(float x, float c, float y, float s, bool& sure) {
+    const float p = y * s, r = fmaf(x, c, p);
+    const float d = fmaf(fabsf(p) + fabsf(r), 1.0001f * 1.1920929e-7f, 2.8e-45f);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(r - d, r + d);
+    const uint32_t v = *reinterpret_cast<const uint32_t*>(&h);
+    sure = sure && v == __byte_perm(v, v, 0x1010);
+    return v;
 }
-// The rotated pair of eight-element pieces at d and d + D / 2 of one head, `row` being the table's row.
-__device__ __forceinline__ void rotate16(float (&lo)[8], float (&hi)[8], const float* cos_row, const float* sin_row, int d, int half) {
+__device__ __forceinline__ uint32_t turn_exactly(float x, float c, float y, float s) {
+    return __bfloat16_as_ushort(__float2bfloat16_rn(__double2float_rn((double)x * (double)c + (double)y * (double)s)));
+}
+struct Angles {          // cos and sin of eight dimensions of the lower and of the upper half
+    float c0[8], s0[8], c1[8], s1[8];
+    __device__ __forceinline__ Angles(const float* cos_row, const float* sin_row, int d, int half) {
+        const float* from[4] = {cos_row + d, sin_row + d, cos_row + d + half, sin_row + d + half};
+        float* to[4] = {c0, s0, c1, s1};
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const float4 c0 = *reinterpret_cast<const float4*>(cos_row + d + 4 * q), s0 = *reinterpret_cast<const float4*>(sin_row + d + 4 * q);
-        const float4 c1 = *reinterpret_cast<const float4*>(cos_row + d + half + 4 * q), s1 = *reinterpret_cast<const float4*>(sin_row + d + half + 4 * q);
-        const float ca[4] = {c0.x, c0.y, c0.z, c0.w}, sa[4] = {s0.x, s0.y, s0.z, s0.w};
-        const float cb[4] = {c1.x, c1.y, c1.z, c1.w}, sb[4] = {s1.x, s1.y, s1.z, s1.w};
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const float4 v = *reinterpret_cast<const float4*>(from[k] + 4 * q);
+                to[k][4 * q] = v.x; to[k][4 * q + 1] = v.y; to[k][4 * q + 2] = v.z; to[k][4 * q + 3] = v.w;
+            }
+    }
+};
+__device__ __forceinline__ void rotate16(uint4& lo, uint4& hi, const Angles& a) {
+    float x0[8], x1[8];
+    unpack8(lo, x0);
+    unpack8(hi, x1);
+    uint32_t l[4], h[4];
+    bool sure = true;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        l[e] = __byte_perm(turn(x0[2 * e], a.c0[2 * e], -x1[2 * e], a.s0[2 * e], sure), turn(x0[2 * e + 1], a.c0[2 * e + 1], -x1[2 * e + 1], a.s0[2 * e + 1], sure), 0x5410);
+        h[e] = __byte_perm(turn(x1[2 * e], a.c1[2 * e], x0[2 * e], a.s1[2 * e], sure), turn(x1[2 * e + 1], a.c1[2 * e + 1], x0[2 * e + 1], a.s1[2 * e + 1], sure), 0x5410);
+    }
+    if (!sure) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float x0 = lo[4 * q + e], x1 = hi[4 * q + e];
-            lo[4 * q + e] = turn(x0, ca[e], -x1, sa[e]);
-            hi[4 * q + e] = turn(x1, cb[e], x0, sb[e]);
+            l[e] = turn_exactly(x0[2 * e], a.c0[2 * e], -x1[2 * e], a.s0[2 * e]) | turn_exactly(x0[2 * e + 1], a.c0[2 * e + 1], -x1[2 * e + 1], a.s0[2 * e + 1]) << 16;
+            h[e] = turn_exactly(x1[2 * e], a.c1[2 * e], x0[2 * e], a.s1[2 * e]) | turn_exactly(x1[2 * e + 1], a.c1[2 * e + 1], x0[2 * e + 1], a.s1[2 * e + 1]) << 16;
         }
     }
+    lo = make_uint4(l[0], l[1], l[2], l[3]);
+    hi = make_uint4(h[0], h[1], h[2], h[3]);
+}
+// Largest magnitudes of two bf16 pairs; NaN wins.
+__device__ __forceinline__ uint32_t abs_max2(uint32_t m, uint32_t x) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(m), "r"(x & 0x7fff7fffu));
+    return r;
 }
 
 // ---- append -----------------------------------------------------------------------------------------
@@ -109,6 +146,7 @@ struct AppendArgs {
 
 constexpr int kAppendThreads = 256;
 constexpr int kMaxD = 128;
+constexpr int kHeadsEach = 4;       // query heads of a thread
 constexpr int kUnits = 4 * kMaxD / kAppendThreads;      // pairs of eight-element pieces a thread holds of a block
 
 // Sequence s: its first row of qkv, the number of its new rows that have a place in the cache, its first position.
@@ -129,7 +167,7 @@ __device__ __forceinline__ int sequence(const AppendArgs& a, int s, int& row0, i
 
 // One block of one KV head's keys or values: rows from r_old on are new, rows before it stand in the tail.
 // A whole block is quantised, of an unfinished one the new rows go to the tail.
-__device__ void append_block(const AppendArgs& a, bool is_k, int s, int h, int blk, int row0, int64_t p0, int n, float* red) {
+__device__ void append_block(const AppendArgs& a, bool is_k, int s, int h, int blk, int row0, int64_t p0, int n, uint32_t* red) {
     const int D = a.c.D, half = D >> 1, pieces = D >> 4;
     const int64_t b0 = (int64_t)blk * kBlock;
     const int r_old = p0 > b0 ? (int)(p0 - b0) : 0;
@@ -139,80 +177,89 @@ __device__ void append_block(const AppendArgs& a, bool is_k, int s, int h, int b
     __nv_bfloat16* tail = (is_k ? a.c.kt : a.c.vt) + head * kBlock * D;
     const int col = (a.nq + (is_k ? 0 : a.c.nkv) + h) * D;
 
-    float lo[kUnits][8], hi[kUnits][8];
-    float amax = 0.f;
-    bool bad = false;
+    uint4 lo[kUnits], hi[kUnits];
+    uint32_t most = 0u;
 #pragma unroll
     for (int j = 0; j < kUnits; ++j) {
         const int u = threadIdx.x + j * kAppendThreads;
         const int r = u / pieces, d = (u - r * pieces) * 8;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) lo[j][e] = hi[j][e] = 0.f;
+        lo[j] = hi[j] = make_uint4(0u, 0u, 0u, 0u);
         if (r >= r_end || (!whole && r < r_old)) continue;
         if (r < r_old) {
-            unpack8(ld16(tail + r * D + d), lo[j]);
-            unpack8(ld16(tail + r * D + d + half), hi[j]);
+            lo[j] = ld16(tail + r * D + d);
+            hi[j] = ld16(tail + r * D + d + half);
         } else {
-            const int64_t p = b0 + r;
-            const int64_t t = row0 + (p - p0);
-            const __nv_bfloat16* src = a.qkv + t * a.ld_qkv + col;
-            unpack8(ld16(src + d), lo[j]);
-            unpack8(ld16(src + d + half), hi[j]);
-            if (is_k) {
-                rotate16(lo[j], hi[j], a.cos_t + p * D, a.sin_t + p * D, d, half);
-                if (a.k_out != nullptr) {
-                    __nv_bfloat16* dst = a.k_out + t * a.ld_k + h * D + d;
-                    *reinterpret_cast<uint4*>(dst) = pack8(lo[j]);
-                    *reinterpret_cast<uint4*>(dst + half) = pack8(hi[j]);
-                }
-            }
-            if (!whole) {
-                *reinterpret_cast<uint4*>(tail + r * D + d) = pack8(lo[j]);
-                *reinterpret_cast<uint4*>(tail + r * D + d + half) = pack8(hi[j]);
+            const __nv_bfloat16* src = a.qkv + (row0 + (b0 + r - p0)) * a.ld_qkv + col;
+            lo[j] = ld16(src + d);
+            hi[j] = ld16(src + d + half);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kUnits; ++j) {
+        const int u = threadIdx.x + j * kAppendThreads;
+        const int r = u / pieces, d = (u - r * pieces) * 8;
+        if (r >= r_end || r < r_old) continue;            // a new row
+        const int64_t p = b0 + r, t = row0 + (p - p0);
+        if (is_k) {
+            rotate16(lo[j], hi[j], Angles(a.cos_t + p * D, a.sin_t + p * D, d, half));
+            if (a.k_out != nullptr) {
+                __nv_bfloat16* dst = a.k_out + t * a.ld_k + h * D + d;
+                *reinterpret_cast<uint4*>(dst) = lo[j];
+                *reinterpret_cast<uint4*>(dst + half) = hi[j];
             }
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            amax = fmaxf(amax, fmaxf(fabsf(lo[j][e]), fabsf(hi[j][e])));
-            bad |= !(fabsf(lo[j][e]) <= 3.4e38f) || !(fabsf(hi[j][e]) <= 3.4e38f);
+        if (!whole) {
+            *reinterpret_cast<uint4*>(tail + r * D + d) = lo[j];
+            *reinterpret_cast<uint4*>(tail + r * D + d + half) = hi[j];
         }
     }
     if (!whole) return;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    bad = __any_sync(0xffffffffu, bad);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = bad ? INFINITY : amax;
+    for (int j = 0; j < kUnits; ++j) {
+        const uint32_t w[8] = {lo[j].x, lo[j].y, lo[j].z, lo[j].w, hi[j].x, hi[j].y, hi[j].z, hi[j].w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = abs_max2(most, w[e]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = abs_max2(most, __shfl_xor_sync(0xffffffffu, most, o));
+    most = abs_max2(most, most >> 16);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = most;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kAppendThreads / 32; ++w) amax = fmaxf(amax, red[w]);
+    for (int w = 0; w < kAppendThreads / 32; ++w) most = abs_max2(most, red[w]);
     __syncthreads();                 // (red is used again, and the tail's rows have been read)
-    bad = amax == INFINITY;
+    const float amax = __uint_as_float(most << 16);
+    const bool bad = !(amax <= 3.4e38f);
     float scale = __uint_as_float((__float_as_uint(__fdiv_rn(amax, 127.f)) + 0xffffu) & 0xffff0000u);
     scale = fmaxf(scale, 1.17549435e-38f);
     int8_t* codes = (is_k ? a.c.k : a.c.v) + (head * a.c.max_len + b0) * D;
     if (threadIdx.x == 0) (is_k ? a.c.ks : a.c.vs)[head * (a.c.max_len / kBlock) + blk] = bad ? __uint_as_float(0x7fc00000u) : scale;
+    // x / s is a tie exactly or at least 1/512 off one (both have 8 significant bits): x * fl(1 / s), off by 2^-16 at most, is
+    // snapped to multiples of 1/1024, where ties are ties again, and then rounded; the code is the low byte of 1.5 * 2^23 + it.
+    const float inv = bad ? 0.f : __fdiv_rn(1.f, scale);
+    auto code = [&](float x) {
+        const float q = bad ? 0.f : __fadd_rn(__fmaf_rn(x, inv, 12288.f), -12288.f);
+        return __float_as_uint(__fadd_rn(q, 12582912.f));
+    };
+    auto codes4 = [&](uint32_t w0, uint32_t w1) {
+        const uint32_t c0 = code(__uint_as_float(w0 << 16)), c1 = code(__uint_as_float(w0 & 0xffff0000u));
+        const uint32_t c2 = code(__uint_as_float(w1 << 16)), c3 = code(__uint_as_float(w1 & 0xffff0000u));
+        return __byte_perm(__byte_perm(c0, c1, 0x0040), __byte_perm(c2, c3, 0x0040), 0x5410);
+    };
 #pragma unroll
     for (int j = 0; j < kUnits; ++j) {
         const int u = threadIdx.x + j * kAppendThreads;
         const int r = u / pieces, d = (u - r * pieces) * 8;
         if (r >= kBlock) continue;
-        uint32_t w[4] = {0u, 0u, 0u, 0u};
-        if (!bad) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                w[e >> 2] |= ((uint32_t)__float2int_rn(__fdiv_rn(lo[j][e], scale)) & 0xffu) << (8 * (e & 3));
-                w[2 + (e >> 2)] |= ((uint32_t)__float2int_rn(__fdiv_rn(hi[j][e], scale)) & 0xffu) << (8 * (e & 3));
-            }
-        }
-        *reinterpret_cast<uint2*>(codes + r * D + d) = make_uint2(w[0], w[1]);
-        *reinterpret_cast<uint2*>(codes + r * D + d + half) = make_uint2(w[2], w[3]);
+        *reinterpret_cast<uint2*>(codes + r * D + d) = make_uint2(codes4(lo[j].x, lo[j].y), codes4(lo[j].z, lo[j].w));
+        *reinterpret_cast<uint2*>(codes + r * D + d + half) = make_uint2(codes4(hi[j].x, hi[j].y), codes4(hi[j].z, hi[j].w));
     }
 }
 
 // The first kv_ctas CTAs take one (sequence, KV head, keys or values, block) each, the others q_tokens rows of query
 // heads.  Bound by HBM for prompts, by one memory round trip and the launch for single tokens.
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
-    __shared__ float red[kAppendThreads / 32];
+    __shared__ uint32_t red[kAppendThreads / 32];
     pdl_enter();
     const int D = a.c.D;
     if ((int)blockIdx.x < a.kv_ctas) {
@@ -237,15 +284,15 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
         if (waits && blk == first) append_block(a, is_k, s, h, last, row0, p0, n, red);
         return;
     }
-    // query heads: a thread takes the pair of pieces (d, d + D / 2) of one head and row
+    // query heads: a thread takes the pieces at d and d + D / 2 of up to kHeadsEach heads of one row, under one set of angles
     const int pieces = D >> 4, half = D >> 1;
     const int t0 = ((int)blockIdx.x - a.kv_ctas) * a.q_tokens;
-    const int per_token = a.nq * pieces;
+    const int groups = (a.nq + kHeadsEach - 1) / kHeadsEach, per_token = groups * pieces;
     for (int u = threadIdx.x; u < a.q_tokens * per_token; u += kAppendThreads) {
         const int t = t0 + u / per_token;
         if (t >= a.T) break;
         const int rem = u % per_token;
-        const int d = (rem % pieces) * 8;
+        const int d = (rem % pieces) * 8, h0 = rem / pieces;         // heads h0, h0 + groups, ...
         int64_t p = -1;
         if (a.cu == nullptr) {
             p = a.pos[(int64_t)t * a.pos_stride];
@@ -260,14 +307,23 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
             if (first >= 0 && i >= 0 && i < a.max_q && t < a.cu[lo + 1]) p = first + i;
         }
         if (p < 0 || p >= a.c.max_len) continue;
-        const __nv_bfloat16* src = a.qkv + (int64_t)t * a.ld_qkv + (rem / pieces) * D + d;
-        float lo8[8], hi8[8];
-        unpack8(ld16(src), lo8);
-        unpack8(ld16(src + half), hi8);
-        rotate16(lo8, hi8, a.cos_t + p * D, a.sin_t + p * D, d, half);
-        __nv_bfloat16* dst = a.q_out + (int64_t)t * a.ld_q + (rem / pieces) * D + d;
-        *reinterpret_cast<uint4*>(dst) = pack8(lo8);
-        *reinterpret_cast<uint4*>(dst + half) = pack8(hi8);
+        const __nv_bfloat16* src = a.qkv + (int64_t)t * a.ld_qkv + h0 * D + d;
+        uint4 lo[kHeadsEach], hi[kHeadsEach];
+#pragma unroll
+        for (int k = 0; k < kHeadsEach; ++k)
+            if (h0 + k * groups < a.nq) {
+                lo[k] = ld16(src + k * groups * D);
+                hi[k] = ld16(src + k * groups * D + half);
+            }
+        const Angles angles(a.cos_t + p * D, a.sin_t + p * D, d, half);
+        __nv_bfloat16* dst = a.q_out + (int64_t)t * a.ld_q + h0 * D + d;
+#pragma unroll
+        for (int k = 0; k < kHeadsEach; ++k)
+            if (h0 + k * groups < a.nq) {
+                rotate16(lo[k], hi[k], angles);
+                *reinterpret_cast<uint4*>(dst + k * groups * D) = lo[k];
+                *reinterpret_cast<uint4*>(dst + k * groups * D + half) = hi[k];
+            }
     }
 }
 
@@ -951,9 +1007,9 @@ static int run_append(const hxq_kv8* c, const void* qkv, int64_t ld_qkv, int32_t
     a.pos_stride = pos_stride; a.T = T; a.S = S; a.nq = nq;
     a.max_q = max_q < c->max_len ? max_q : c->max_len;
     a.n_blk = cu ? (a.max_q + 2 * kBlock - 2) / kBlock : 1;          // blocks that max_q rows can touch, wherever they start
-    // rows of query heads per CTA: about two steps of its threads
-    const int per_token = nq * (c->D / 16);
-    a.q_tokens = 2 * kAppendThreads / per_token > 0 ? 2 * kAppendThreads / per_token : 1;
+    // rows of query heads per CTA: about as many as its threads take in one step
+    const int per_token = (nq + kHeadsEach - 1) / kHeadsEach * (c->D / 16);
+    a.q_tokens = kAppendThreads / per_token > 0 ? kAppendThreads / per_token : 1;
     const int64_t kv = (int64_t)S * c->nkv * 2 * a.n_blk, qc = ((int64_t)T + a.q_tokens - 1) / a.q_tokens;
     if (kv + qc > 0x7fffffffLL) return HXQ_E_SHAPE;
     a.kv_ctas = (int)kv;
