@@ -77,7 +77,7 @@ __device__ __forceinline__ uint4 ld16(const void* p) { return *reinterpret_cast<
 // on.  Nearly always fp32 tells the same: r = fma(x, cos, fl(y sin)) is off by 2^-24 (|y sin| + |r|) at most and the
 // true sum's fp32 value by one more rounding, so where r - d and r + d, d = 2^-23 (|y sin| + |r|), round to the same bf16, that is
 // it.  One value in some 2^13 takes the 64-bit path.  (All in 64 bits, conversions alone filled half of the time: 86 us for 8191
-// tokens of 28 + 4 heads, 31 as it is.)
+// tokens of 28 + 4 heads, 41 as it is; exact sums of products and their rests in packed fp32 took 42 to 48.)
 __device__ __forceinline__ uint32_t turn(float x, float c, float y, float s, bool& sure) {
     const float p = y * s, r = fmaf(x, c, p);
     const float d = fmaf(fabsf(p) + fabsf(r), 1.0001f * 1.1920929e-7f, 2.8e-45f);
@@ -141,7 +141,7 @@ struct AppendArgs {
     const float *cos_t, *sin_t;
     __nv_bfloat16 *q_out, *k_out;
     int64_t ld_qkv, ld_q, ld_k;
-    int pos_stride, T, S, max_q, nq, n_blk, kv_ctas, q_tokens;
+    int pos_stride, T, S, max_q, nq, groups;        // groups: of kHeadsEach query heads
 };
 
 constexpr int kAppendThreads = 256;
@@ -256,75 +256,92 @@ __device__ void append_block(const AppendArgs& a, bool is_k, int s, int h, int b
     }
 }
 
-// The first kv_ctas CTAs take one (sequence, KV head, keys or values, block) each, the others q_tokens rows of query
-// heads.  Bound by HBM for prompts, by one memory round trip and the launch for single tokens.
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs a) {
+// The query heads h0, h0 + groups, ... (up to kHeadsEach) of one row, the pieces at d and d + D / 2, under one set of angles.
+__device__ __forceinline__ void turn_queries(const AppendArgs& a, int64_t t, int64_t p, int h0, int d) {
+    const int D = a.c.D, half = D >> 1;
+    const __nv_bfloat16* src = a.qkv + t * a.ld_qkv + h0 * D + d;
+    uint4 lo[kHeadsEach], hi[kHeadsEach];
+#pragma unroll
+    for (int k = 0; k < kHeadsEach; ++k)
+        if (h0 + k * a.groups < a.nq) {
+            lo[k] = ld16(src + k * a.groups * D);
+            hi[k] = ld16(src + k * a.groups * D + half);
+        }
+    const Angles angles(a.cos_t + p * D, a.sin_t + p * D, d, half);
+    __nv_bfloat16* dst = a.q_out + t * a.ld_q + h0 * D + d;
+#pragma unroll
+    for (int k = 0; k < kHeadsEach; ++k)
+        if (h0 + k * a.groups < a.nq) {
+            rotate16(lo[k], hi[k], angles);
+            *reinterpret_cast<uint4*>(dst + k * a.groups * D) = lo[k];
+            *reinterpret_cast<uint4*>(dst + k * a.groups * D + half) = hi[k];
+        }
+}
+
+// A CTA takes one block of one sequence and either one KV head's keys or values or a group of query heads.
+// STEP: one token a sequence, the CTA's block being the token's; a CTA for all query heads.
+// Else the blocks that the sequences' new rows touch stand in a row, and every warp works out for itself where its CTA's lies.
+// Bound by HBM for prompts (and by instructions nearly as much), by one memory round trip and the launch for single tokens.
+template <bool STEP>
+__global__ void __launch_bounds__(kAppendThreads, STEP ? 1 : 2) append_kernel(const AppendArgs a) {
     __shared__ uint32_t red[kAppendThreads / 32];
     pdl_enter();
-    const int D = a.c.D;
-    if ((int)blockIdx.x < a.kv_ctas) {
-        int i = blockIdx.x;
-        const int j = i % a.n_blk;
-        i /= a.n_blk;
-        const bool is_k = (i & 1) == 0;
-        i >>= 1;
-        const int h = i % a.c.nkv, s = i / a.c.nkv;
-        int row0;
-        int64_t p0;
-        const int n = sequence(a, s, row0, p0);
+    const int D = a.c.D, pieces = D >> 4, lane = threadIdx.x & 31;
+    const int parts = (kBlock * pieces + kAppendThreads - 1) / kAppendThreads;       // of a block, for query heads: one step of the threads each
+    const int roles = (STEP ? 1 : a.groups * parts) + 2 * a.c.nkv;
+    const int role = blockIdx.x % roles;
+    int s = blockIdx.x / roles, row0, blk, n, first, last;
+    int64_t p0;
+    if (STEP) {
+        n = sequence(a, s, row0, p0);
         if (n == 0) return;
-        const int first = (int)(p0 / kBlock), last = (int)((p0 + n - 1) / kBlock);
-        const int blk = first + j;
-        if (blk > last) return;
-        // An unfinished last block's rows take the place of the tail's rows that the first block takes in: where both
-        // happen, the first block's CTA does one after the other.
-        const bool waits = p0 % kBlock != 0 && last != first && (p0 + n) % kBlock != 0;
-        if (waits && blk == last) return;
-        append_block(a, is_k, s, h, blk, row0, p0, n, red);
-        if (waits && blk == first) append_block(a, is_k, s, h, last, row0, p0, n, red);
+        blk = first = last = (int)(p0 / kBlock);
+    } else {
+        int at = s, before = 0;
+        s = -1;
+        for (int s0 = 0; s0 < a.S && s < 0; s0 += 32) {
+            int rows = 0, r0 = 0, f = 0, l = -1;
+            int64_t p = 0;
+            if (s0 + lane < a.S) rows = sequence(a, s0 + lane, r0, p);
+            if (rows > 0) { f = (int)(p / kBlock); l = (int)((p + rows - 1) / kBlock); }
+            int incl = l - f + 1;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            const uint32_t hit = __ballot_sync(0xffffffffu, before + incl > at);
+            if (hit != 0u) {
+                const int k = __ffs(hit) - 1;
+                s = s0 + k;
+                n = __shfl_sync(0xffffffffu, rows, k);
+                row0 = __shfl_sync(0xffffffffu, r0, k);
+                p0 = __shfl_sync(0xffffffffu, p, k);
+                first = __shfl_sync(0xffffffffu, f, k);
+                last = __shfl_sync(0xffffffffu, l, k);
+                blk = first + at - (before + __shfl_sync(0xffffffffu, incl - (l - f + 1), k));
+            }
+            before += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (s < 0) return;
+    }
+    if (role < roles - 2 * a.c.nkv) {
+        if (STEP) {
+            for (int u = threadIdx.x; u < a.groups * pieces; u += kAppendThreads) turn_queries(a, row0, p0, u / pieces, (u % pieces) * 8);
+        } else {
+            const int64_t p = (int64_t)blk * kBlock + (role % parts) * (kBlock / parts) + threadIdx.x / pieces;
+            if ((int)threadIdx.x < kBlock / parts * pieces && p >= p0 && p < p0 + n) turn_queries(a, row0 + (p - p0), p, role / parts, (threadIdx.x % pieces) * 8);
+        }
         return;
     }
-    // query heads: a thread takes the pieces at d and d + D / 2 of up to kHeadsEach heads of one row, under one set of angles
-    const int pieces = D >> 4, half = D >> 1;
-    const int t0 = ((int)blockIdx.x - a.kv_ctas) * a.q_tokens;
-    const int groups = (a.nq + kHeadsEach - 1) / kHeadsEach, per_token = groups * pieces;
-    for (int u = threadIdx.x; u < a.q_tokens * per_token; u += kAppendThreads) {
-        const int t = t0 + u / per_token;
-        if (t >= a.T) break;
-        const int rem = u % per_token;
-        const int d = (rem % pieces) * 8, h0 = rem / pieces;         // heads h0, h0 + groups, ...
-        int64_t p = -1;
-        if (a.cu == nullptr) {
-            p = a.pos[(int64_t)t * a.pos_stride];
-        } else {
-            int lo = 0, hi = a.S;          // the sequence with cu[s] <= t < cu[s + 1]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (a.cu[mid] <= t) lo = mid; else hi = mid;
-            }
-            const int64_t first = a.pos[(int64_t)lo * a.pos_stride];
-            const int i = t - a.cu[lo];
-            if (first >= 0 && i >= 0 && i < a.max_q && t < a.cu[lo + 1]) p = first + i;
-        }
-        if (p < 0 || p >= a.c.max_len) continue;
-        const __nv_bfloat16* src = a.qkv + (int64_t)t * a.ld_qkv + h0 * D + d;
-        uint4 lo[kHeadsEach], hi[kHeadsEach];
-#pragma unroll
-        for (int k = 0; k < kHeadsEach; ++k)
-            if (h0 + k * groups < a.nq) {
-                lo[k] = ld16(src + k * groups * D);
-                hi[k] = ld16(src + k * groups * D + half);
-            }
-        const Angles angles(a.cos_t + p * D, a.sin_t + p * D, d, half);
-        __nv_bfloat16* dst = a.q_out + (int64_t)t * a.ld_q + h0 * D + d;
-#pragma unroll
-        for (int k = 0; k < kHeadsEach; ++k)
-            if (h0 + k * groups < a.nq) {
-                rotate16(lo[k], hi[k], angles);
-                *reinterpret_cast<uint4*>(dst + k * groups * D) = lo[k];
-                *reinterpret_cast<uint4*>(dst + k * groups * D + half) = hi[k];
-            }
-    }
+    const int kv = role - (roles - 2 * a.c.nkv), h = kv >> 1;
+    const bool is_k = (kv & 1) == 0;
+    // An unfinished last block's rows take the place of the tail's rows that the first block takes in: where both
+    // happen, the first block's CTA does one after the other.
+    const bool waits = !STEP && p0 % kBlock != 0 && last != first && (p0 + n) % kBlock != 0;
+    if (waits && blk == last) return;
+    append_block(a, is_k, s, h, blk, row0, p0, n, red);
+    if (waits && blk == first) append_block(a, is_k, s, h, last, row0, p0, n, red);
 }
 
 // ---- rows back as bf16 ------------------------------------------------------------------------------
@@ -1006,14 +1023,12 @@ static int run_append(const hxq_kv8* c, const void* qkv, int64_t ld_qkv, int32_t
     a.ld_qkv = ld_qkv; a.ld_q = ld_q; a.ld_k = ld_k;
     a.pos_stride = pos_stride; a.T = T; a.S = S; a.nq = nq;
     a.max_q = max_q < c->max_len ? max_q : c->max_len;
-    a.n_blk = cu ? (a.max_q + 2 * kBlock - 2) / kBlock : 1;          // blocks that max_q rows can touch, wherever they start
-    // rows of query heads per CTA: about as many as its threads take in one step
-    const int per_token = (nq + kHeadsEach - 1) / kHeadsEach * (c->D / 16);
-    a.q_tokens = kAppendThreads / per_token > 0 ? kAppendThreads / per_token : 1;
-    const int64_t kv = (int64_t)S * c->nkv * 2 * a.n_blk, qc = ((int64_t)T + a.q_tokens - 1) / a.q_tokens;
-    if (kv + qc > 0x7fffffffLL) return HXQ_E_SHAPE;
-    a.kv_ctas = (int)kv;
-    const cudaError_t e = launch_pdl(append_kernel, dim3((unsigned)(kv + qc)), dim3(kAppendThreads), stream, 0, a);
+    a.groups = (nq + kHeadsEach - 1) / kHeadsEach;
+    // blocks that n rows touch: n / 64 and up to two more, wherever they start
+    const int64_t blocks = cu ? (int64_t)T / kBlock + 2 * (int64_t)S : S, grid = blocks * ((cu ? a.groups * ((kBlock * (c->D / 16) + kAppendThreads - 1) / kAppendThreads) : 1) + 2 * c->nkv);
+    if (grid > 0x7fffffffLL) return HXQ_E_SHAPE;
+    const cudaError_t e = cu ? launch_pdl(append_kernel<false>, dim3((unsigned)grid), dim3(kAppendThreads), stream, 0, a)
+                             : launch_pdl(append_kernel<true>, dim3((unsigned)grid), dim3(kAppendThreads), stream, 0, a);
     return e == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
 }
 

@@ -83,6 +83,58 @@ def test_append_prompts_in_pieces(nq, nkv, D):
         _check_cache(cache, ref)
 
 
+def test_append_of_many_packed_prompts():
+    """More sequences than a warp has lanes, most of them short or empty, one long: every block finds its CTA."""
+    from helix_substrate_b200.kv8 import Kv8Cache, rope_append_prompt_kv8
+    dev, S, nq, nkv, D, max_len = _dev(), 75, 5, 1, 112, 1024
+    g = torch.Generator().manual_seed(8)
+    cache, ref = Kv8Cache.empty(S, nkv, max_len, D, dev), RefCache(S, nkv, D)
+    cos, sin = tables(max_len, D, "cpu")
+    for turn in range(2):
+        lens = [int(x) for x in torch.randint(0, 30, (S,), generator=g)]
+        lens[3], lens[40], lens[74] = 500, 0, 64
+        pos = [ref.length(s) for s in range(S)]
+        cu = [sum(lens[:s]) for s in range(S + 1)]
+        qkv = torch.randn(cu[-1], (nq + 2 * nkv) * D, generator=g).bfloat16()
+        q_out = torch.empty(cu[-1], nq * D, device=dev, dtype=torch.bfloat16)
+        rope_append_prompt_kv8(qkv.to(dev), torch.tensor(cu, dtype=torch.int32, device=dev), 500, torch.tensor(pos, device=dev), cos.to(dev), sin.to(dev),
+                               q_out, None, cache, nq)
+        x = qkv.view(-1, nq + 2 * nkv, D)
+        at = torch.tensor([p + i for p, n in zip(pos, lens) for i in range(n)])
+        turned = rotate(x[:, : nq + nkv], cos[at][:, None], sin[at][:, None])
+        assert torch.equal(q_out.cpu(), turned[:, :nq].flatten(1))
+        for s in range(S):
+            ref.append(s, turned[cu[s]: cu[s + 1], nq:], x[cu[s]: cu[s + 1], nq + nkv:])
+        _check_cache(cache, ref)
+
+
+def test_rotation_next_to_borders():
+    """Angles and values for which fp32 sums lie on or next to a border of bf16, cancel to nothing, or overflow: as 64-bit arithmetic
+    rounds them; infinities and NaNs stay what they are."""
+    from helix_substrate_b200.kv8 import Kv8Cache, rope_append_prompt_kv8
+    dev, D, n = _dev(), 128, 640
+    g = torch.Generator().manual_seed(12)
+    x = torch.randn(n, 3, D, generator=g).bfloat16()
+    x[:64] = torch.randint(-300, 300, (64, 3, D), generator=g).bfloat16()
+    x[64:128] *= 1e30
+    x[128:192] *= 1e-38
+    x[200, 0, 5], x[201, 0, 70], x[202, 0, 9] = float("inf"), float("-inf"), float("nan")
+    x[203, 0, 3], x[203, 0, 67] = 3.3e38, -3.3e38
+    x[192:256, 1:] = 1.0
+    cos, sin = torch.randn(n, D, generator=g), torch.randn(n, D, generator=g)
+    cos[:32], sin[:32] = 1.0, 2.0 ** -9          # sums half-way between two bf16 numbers
+    cos[32:64], sin[32:64] = 0.5, 0.5            # and sums that cancel
+    cos[300:400] = sin[300:400] + 1e-7 * torch.randn(100, D, generator=g)
+    x[300:400, :, 64:] = x[300:400, :, :64]
+    cache = Kv8Cache.empty(1, 1, n, D, dev)
+    q_out = torch.empty(n, D, device=dev, dtype=torch.bfloat16)
+    rope_append_prompt_kv8(x.flatten(1).to(dev), torch.tensor([0, n], dtype=torch.int32, device=dev), n, torch.zeros(1, dtype=torch.int64, device=dev),
+                           cos.to(dev), sin.to(dev), q_out, None, cache, 1)
+    want, got = rotate(x[:, 0], cos, sin), q_out.cpu()
+    assert torch.equal(want.isnan(), got.isnan())
+    assert torch.equal(want.nan_to_num(0.0, 1.0, -1.0), got.nan_to_num(0.0, 1.0, -1.0))
+
+
 @pytest.mark.parametrize("one_pos", [False, True])
 def test_append_steps(one_pos):
     """130 tokens one at a time (two finished blocks), all slots alike or each at its own position."""
