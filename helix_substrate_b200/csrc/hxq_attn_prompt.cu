@@ -48,6 +48,8 @@ constexpr int BN = 128;                     // keys of a step
 constexpr int NUM_THREADS = 384;
 constexpr int kMaxStages = 8;
 constexpr int kBarBytes = 512;
+constexpr int kPolyOf4 = 1;                 // of four pairs of weights, how many are made on the multiply-add units
+constexpr int kRegsSoftmax = 208, kRegsOther = 88;      // of a thread, after the roles have parted
 
 template <int DP>
 struct Sizes {
@@ -97,6 +99,39 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// ---- pairs of fp32 numbers
+typedef uint64_t f2;
+__device__ __forceinline__ f2 pair(float lo, float hi) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void split(f2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) { f2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) { f2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ float max3(float a, float b, float c) {       // NaN wins
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x of a pair on the multiply-add units: x = n + f with n whole, |f| <= 1/2 (adding and taking off 1.5 * 2^23 leaves n, in
+// the low bits too); 2^f by a polynomial of least largest relative error, 1.0e-4 (a twentieth of P's rounding), with the
+// constant term 1; n added to the exponent.  From x = -127 down, and at -inf, it is 0 (there f = 0, and 1's exponent is
+// 127).  x <= 127.
+__device__ __forceinline__ f2 ex2_pair(f2 x) {
+    float lo, hi;
+    split(x, lo, hi);
+    x = pair(fmaxf(lo, -127.f), fmaxf(hi, -127.f));
+    const f2 t = add2(x, pair(12582912.f, 12582912.f));
+    const f2 f = fma2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f), x);
+    f2 p = fma2(f, pair(0.0550089329f, 0.0550089329f), pair(0.242210969f, 0.242210969f));
+    p = fma2(f, p, pair(0.693282902f, 0.693282902f));
+    p = fma2(f, p, pair(1.f, 1.f));
+    float tl, th;
+    split(t, tl, th);
+    split(p, lo, hi);
+    return pair(__uint_as_float((__float_as_uint(tl) << 23) + __float_as_uint(lo)), __uint_as_float((__float_as_uint(th) << 23) + __float_as_uint(hi)));
 }
 __device__ __forceinline__ uint32_t bf2(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -211,6 +246,10 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const uint32_t tmem = *tmem_slot;       // S0 | S1 | O0 | O1, 128 columns each
     bool ok = true;
 
+    // 168 registers a thread at launch: 256 * 208 + 128 * 88 is what 384 * 168 gives
+    static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= NUM_THREADS * 168, "no more than the launch brings");
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == 8) {
         // ------------------------------------------------------------ loads
         if (lane == 0 && n > 0) {
@@ -298,7 +337,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 }
             }
         }
-    } else if (warp >= 10) {
+    } else {
         // ------------------------------------------------------------ V tiles that some row sees only in part
         uint32_t raw_ph = 0;
         for (int j = jc; j < n; ++j) {
@@ -332,8 +371,10 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             __syncwarp();
             if (lane == 0) sm100::mbar_arrive(&clean[slot]);
         }
+    }
     } else {
         // ------------------------------------------------------------ softmax and epilogue: TMEM lane == row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         const int x = warp >> 2, row = 32 * (warp & 3) + lane;
         const int nx = x ? n1 : n0;
         const int tok = i0 + x * a.tpg + row / a.G;
@@ -349,19 +390,23 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             sm100::tc_fence_after_sync();
             const bool edge = (j + 1) * BN > seen;
             const int lim = cnt - j * BN;
-            float mx = -INFINITY;
-#pragma unroll 1
-            for (int c = 0; c < BN; c += 32) {
-                uint32_t r[32];
-                sm100::tmem_ld_32x32(ts + c, r);
-                sm100::tmem_ld_wait();
-                if (edge) {
+            uint32_t r[BN];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) if (c + e >= lim) r[e] = 0xff800000u;
-                }
+            for (int c = 0; c < BN; c += 32) sm100::tmem_ld_32x32(ts + c, reinterpret_cast<uint32_t(&)[32]>(r[c]));
+            sm100::tmem_ld_wait();
+            if (edge) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(r[e]));
+                for (int e = 0; e < BN; ++e) if (e >= lim) r[e] = 0xff800000u;
             }
+            float mx = -INFINITY, m4[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                m4[k] = max3(__uint_as_float(r[k]), __uint_as_float(r[4 + k]), __uint_as_float(r[8 + k]));
+#pragma unroll
+                for (int e = 12 + k; e < BN - 4; e += 8) m4[k] = max3(m4[k], __uint_as_float(r[e]), __uint_as_float(r[e + 4]));
+            }
+            mx = max3(max3(m4[0], m4[1], m4[2]), m4[3], max3(__uint_as_float(r[BN - 4]), __uint_as_float(r[BN - 3]), max3(__uint_as_float(r[BN - 2]), __uint_as_float(r[BN - 1]), -INFINITY)));
+            if (!(mx < INFINITY)) l = __uint_as_float(0x7fc00000u);        // a score that is infinite or none: so is the row
             // a new reference point where the maximum has grown by more than 2^8
             const bool move = (mx - ref) * sc > 8.f;        // (-inf - -inf is NaN: no)
             const float old = ref;
@@ -388,28 +433,37 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             // scores are so large that it is itself large; then the difference is taken first
             const bool far = __any_sync(0xffffffffu, ref != -INFINITY && fabsf(ref * sc) > 65536.f);
             const float bias = ref == -INFINITY || far ? 0.f : -ref * sc;
-            const float first = ref == -INFINITY ? 0.f : ref;
-#pragma unroll 1
+            if (far) {
+                const float first = ref == -INFINITY ? 0.f : ref;
+#pragma unroll
+                for (int e = 0; e < BN; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) - first);
+            }
+            const f2 sc2 = pair(sc, sc), bias2 = pair(bias, bias);
+            f2 l2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+#pragma unroll
             for (int c = 0; c < BN; c += 32) {
-                uint32_t r[32], p[16];
-                sm100::tmem_ld_32x32(ts + c, r);
-                sm100::tmem_ld_wait();
-                if (edge) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) if (c + e >= lim) r[e] = 0xff800000u;
-                }
-                if (far) {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) - first);
-                }
+                uint32_t p[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const float p0 = ex2(fmaf(__uint_as_float(r[2 * e]), sc, bias)), p1 = ex2(fmaf(__uint_as_float(r[2 * e + 1]), sc, bias));
-                    l += p0 + p1;
-                    p[e] = bf2(p0, p1);
+                    f2 y = fma2(pair(__uint_as_float(r[c + 2 * e]), __uint_as_float(r[c + 2 * e + 1])), sc2, bias2);
+                    float y0, y1;
+                    if (e % 4 < kPolyOf4) {
+                        y = ex2_pair(y);
+                        split(y, y0, y1);
+                    } else {
+                        split(y, y0, y1);
+                        y0 = ex2(y0);
+                        y1 = ex2(y1);
+                        y = pair(y0, y1);
+                    }
+                    l2[e & 1] = add2(l2[e & 1], y);
+                    p[e] = bf2(y0, y1);
                 }
                 tmem_st_32x16(ts + c / 2, p);
             }
+            float l0, l1;
+            split(add2(l2[0], l2[1]), l0, l1);
+            l += l0 + l1;
             tmem_st_wait();
             sm100::tc_fence_before_sync();
             __syncwarp();
@@ -506,6 +560,8 @@ static int run(const hxq_attn* p, int32_t* status, cudaStream_t stream) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return HXQ_E_DEVICE;
     if (!attr_set[dev]) {
+        cudaFuncAttributes fa;        // the warps' exchange of registers counts on what the launch brings
+        if (cudaFuncGetAttributes(&fa, attn_prompt_kernel<DP>) != cudaSuccess || fa.numRegs < 168) return HXQ_E_DEVICE;
         if (cudaFuncSetAttribute(attn_prompt_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::kSmem) != cudaSuccess) return HXQ_E_DEVICE;
         attr_set[dev] = true;
     }
