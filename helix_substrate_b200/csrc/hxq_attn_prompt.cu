@@ -45,17 +45,18 @@ namespace attnp {
 
 constexpr int BM = 128;                     // rows of a tile
 constexpr int BN = 128;                     // keys of a step
-constexpr int NUM_THREADS = 384;
+constexpr int SM_WARPS = 16;                // softmax: eight per tile
+constexpr int NUM_THREADS = 32 * (SM_WARPS + 4);
 constexpr int kMaxStages = 8;
-constexpr int kBarBytes = 512;
+constexpr int kBarBytes = 512 + 2 * 2 * 128 * 4;        // barriers, and what the two halves of a row tell each other
 constexpr int kPolyOf4 = 1;                 // of four pairs of weights, how many are made on the multiply-add units
-constexpr int kRegsSoftmax = 208, kRegsOther = 88;      // of a thread, after the roles have parted
+constexpr int kRegsLaunch = 96, kRegsSoftmax = 104, kRegsOther = 64;      // of a thread, after the roles have parted
 
 template <int DP>
 struct Sizes {
     static constexpr int kTile = BM * DP * 2;                 // a Q, K or V tile
     static constexpr int kStages = DP == 128 ? 5 : 8;
-    static constexpr int kSmem = (2 + kStages) * kTile + kBarBytes + 1024;
+    static constexpr int kSmem = (2 + kStages) * kTile + kBarBytes;
 };
 
 struct Args {
@@ -93,6 +94,12 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r
         "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
         ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
           "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
@@ -155,8 +162,11 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                    const __grid_constant__ CUtensorMap map_v, const Args a) {
     using Z = Sizes<DP>;
     constexpr int NS = Z::kStages, TILE = Z::kTile, HALF = BM * 128;      // HALF: 64 of the dimensions of a tile
-    extern __shared__ char smem_raw[];
-    char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(1024) char smem[];        // (no room for slack: the swizzled tiles need that alignment, checked here)
+    if (sm100::smem_u32(smem) % 1024 != 0) {
+        if (threadIdx.x == 0 && a.status != nullptr) atomicExch(a.status, HXQ_E_ALIGN);
+        return;
+    }
     char* ring = smem + 2 * TILE;
     uint64_t* full = reinterpret_cast<uint64_t*>(ring + NS * TILE);     // [NS] a tile has landed, ready for its product
     uint64_t* empty = full + kMaxStages;        // [NS] its products have retired
@@ -168,8 +178,10 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     uint64_t* o_done = p_ready + 2;             // [2] the last product of a tile has retired
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* gave_up = abort_flag + 2;     // [2] the step at which a softmax warp's wait ran out
     volatile int* odd_v = abort_flag + 1;       // a V tile held an infinity or a NaN that some row does not see
-    static_assert((4 * kMaxStages + 7) * 8 + 12 <= kBarBytes, "barrier area");
+    float* talk = reinterpret_cast<float*>(ring + NS * TILE + 512);        // [2 tiles][2 halves][128 rows]
+    static_assert((4 * kMaxStages + 7) * 8 + 20 <= 512, "barrier area");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -218,17 +230,18 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         sm100::mbar_init(q_full, 1);
         for (int x = 0; x < 2; ++x) {
             sm100::mbar_init(&s_full[x], 1);
-            sm100::mbar_init(&p_ready[x], 4);
+            sm100::mbar_init(&p_ready[x], SM_WARPS / 2);
             sm100::mbar_init(&o_done[x], 1);
         }
         *abort_flag = 0;
         *odd_v = 0;
+        gave_up[0] = gave_up[1] = 0x7fffffff;
         sm100::fence_barrier_init();
         sm100::prefetch_tensormap(&map_q);
         sm100::prefetch_tensormap(&map_k);
         sm100::prefetch_tensormap(&map_v);
     }
-    if (warp == 9) {
+    if (warp == SM_WARPS + 1) {
         sm100::tmem_alloc(tmem_slot, 512);
         sm100::tmem_relinquish();
     }
@@ -246,11 +259,10 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const uint32_t tmem = *tmem_slot;       // S0 | S1 | O0 | O1, 128 columns each
     bool ok = true;
 
-    // 168 registers a thread at launch: 256 * 208 + 128 * 88 is what 384 * 168 gives
-    static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= NUM_THREADS * 168, "no more than the launch brings");
-    if (warp >= 8) {
+    static_assert(32 * SM_WARPS * kRegsSoftmax + 128 * kRegsOther <= NUM_THREADS * kRegsLaunch, "no more registers than the launch brings");
+    if (warp >= SM_WARPS) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-    if (warp == 8) {
+    if (warp == SM_WARPS) {
         // ------------------------------------------------------------ loads
         if (lane == 0 && n > 0) {
             sm100::mbar_arrive_expect_tx(q_full, 2u * (DP / 64) * (uint32_t)rows * 128u);
@@ -270,7 +282,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 if (++slot == NS) { slot = 0; ph ^= 1u; }
             }
         }
-    } else if (warp == 9) {
+    } else if (warp == SM_WARPS + 1) {
         // ------------------------------------------------------------ MMAs
         if (lane == 0 && n > 0) {
             const uint32_t idesc_s = sm100::make_idesc_bf16(BM, BN);
@@ -348,7 +360,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             char* tile = ring + slot * TILE;
             const int from = seen_by_all - j * BN > 0 ? seen_by_all - j * BN : 0;         // rows before it are everybody's
             bool odd = false;
-            for (int i = (warp - 10) * 32 + lane; i < (DP / 64) * (BN - from) * 8; i += 64) {
+            for (int i = (warp - SM_WARPS - 2) * 32 + lane; i < (DP / 64) * (BN - from) * 8; i += 64) {
                 const int part = i / ((BN - from) * 8), rem = i - part * (BN - from) * 8;
                 const int row = from + (rem >> 3);
                 uint4* p = reinterpret_cast<uint4*>(tile + part * HALF + row * 128 + (rem & 7) * 16);
@@ -374,38 +386,48 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     }
     } else {
         // ------------------------------------------------------------ softmax and epilogue: TMEM lane == row
+        // Two threads to a row, in two warps: one per half of a step's keys, and of the output's dimensions.
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-        const int x = warp >> 2, row = 32 * (warp & 3) + lane;
+        constexpr int HK = BN / 2, HD = DP / 2;
+        const int x = warp >> 3, hf = (warp >> 2) & 1, row = 32 * (warp & 3) + lane;
         const int nx = x ? n1 : n0;
         const int tok = i0 + x * a.tpg + row / a.G;
         const int cnt = count(tok);
         const int seen = nx > 0 ? count(i0 + x * a.tpg) : 0;        // keys that every row of the tile sees
         const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-        const uint32_t ts = t_lane + 128u * x, to = t_lane + 256u + 128u * x;
+        const uint32_t ts = t_lane + 128u * x, to = t_lane + 256u + 128u * x + (uint32_t)(hf * HD);
         const float sc = a.scale_log2;
-        float ref = -INFINITY, l = 0.f;         // in units of S
+        float* mine = talk + (2 * x + hf) * 128 + row;
+        const float* other = talk + (2 * x + (hf ^ 1)) * 128 + row;
+        auto meet = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + x), "n"(32 * SM_WARPS / 2) : "memory"); };        // the tile's eight warps
+        float ref = -INFINITY, l = 0.f;         // in units of S; l: of this half's keys
         for (int j = 0; j < nx; ++j) {
             ok = __all_sync(0xffffffffu, sm100::mbar_wait(&s_full[x], (uint32_t)j & 1u, abort_flag));
-            if (!ok) break;
+            if (!ok && lane == 0) gave_up[x] = j;
             sm100::tc_fence_after_sync();
-            const bool edge = (j + 1) * BN > seen;
-            const int lim = cnt - j * BN;
-            uint32_t r[BN];
+            uint32_t r[HK];
 #pragma unroll
-            for (int c = 0; c < BN; c += 32) sm100::tmem_ld_32x32(ts + c, reinterpret_cast<uint32_t(&)[32]>(r[c]));
+            for (int c = 0; c < HK; c += 32) sm100::tmem_ld_32x32(ts + hf * HK + c, reinterpret_cast<uint32_t(&)[32]>(r[c]));
             sm100::tmem_ld_wait();
-            if (edge) {
+            if ((j + 1) * BN > seen) {
+                const int lim = cnt - j * BN - hf * HK;
 #pragma unroll
-                for (int e = 0; e < BN; ++e) if (e >= lim) r[e] = 0xff800000u;
+                for (int e = 0; e < HK; ++e) if (e >= lim) r[e] = 0xff800000u;
             }
-            float mx = -INFINITY, m4[4];
+            float m4[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 m4[k] = max3(__uint_as_float(r[k]), __uint_as_float(r[4 + k]), __uint_as_float(r[8 + k]));
 #pragma unroll
-                for (int e = 12 + k; e < BN - 4; e += 8) m4[k] = max3(m4[k], __uint_as_float(r[e]), __uint_as_float(r[e + 4]));
+                for (int e = 12 + k; e < HK - 4; e += 8) m4[k] = max3(m4[k], __uint_as_float(r[e]), __uint_as_float(r[e + 4]));
             }
-            mx = max3(max3(m4[0], m4[1], m4[2]), m4[3], max3(__uint_as_float(r[BN - 4]), __uint_as_float(r[BN - 3]), max3(__uint_as_float(r[BN - 2]), __uint_as_float(r[BN - 1]), -INFINITY)));
+            static_assert((HK - 16) % 8 == 0, "the pairs above end four before the end");
+            float mx = max3(max3(m4[0], m4[1], __uint_as_float(r[HK - 4])), max3(m4[2], m4[3], __uint_as_float(r[HK - 3])),
+                            max3(__uint_as_float(r[HK - 2]), __uint_as_float(r[HK - 1]), -INFINITY));
+            *mine = mx;
+            meet();
+            if (gave_up[x] <= j) { ok = false; break; }        // all eight warps leave at the same step: nobody is missed at a barrier
+            mx = max3(mx, *other, -INFINITY);
             if (!(mx < INFINITY)) l = __uint_as_float(0x7fc00000u);        // a score that is infinite or none: so is the row
             // a new reference point where the maximum has grown by more than 2^8
             const bool move = (mx - ref) * sc > 8.f;        // (-inf - -inf is NaN: no)
@@ -416,16 +438,13 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 l *= corr;
                 if (j > 0) {
 #pragma unroll 1
-                    for (int c = 0; c < DP; c += 16) {
-                        uint32_t r[16];
-                        asm volatile(
-                            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-                              "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(to + c) : "memory");
+                    for (int c = 0; c < HD; c += 16) {
+                        uint32_t o[16];
+                        tmem_ld_32x16(to + c, o);
                         sm100::tmem_ld_wait();
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * corr);
-                        tmem_st_32x16(to + c, r);
+                        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                        tmem_st_32x16(to + c, o);
                     }
                 }
             }
@@ -436,12 +455,12 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             if (far) {
                 const float first = ref == -INFINITY ? 0.f : ref;
 #pragma unroll
-                for (int e = 0; e < BN; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) - first);
+                for (int e = 0; e < HK; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) - first);
             }
             const f2 sc2 = pair(sc, sc), bias2 = pair(bias, bias);
             f2 l2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
-            for (int c = 0; c < BN; c += 32) {
+            for (int c = 0; c < HK; c += 32) {
                 uint32_t p[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -459,7 +478,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                     l2[e & 1] = add2(l2[e & 1], y);
                     p[e] = bf2(y0, y1);
                 }
-                tmem_st_32x16(ts + c / 2, p);
+                tmem_st_32x16(ts + (hf * HK + c) / 2, p);        // over scores that both halves have taken
             }
             float l0, l1;
             split(add2(l2[0], l2[1]), l0, l1);
@@ -470,6 +489,10 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             if (lane == 0) sm100::mbar_arrive(&p_ready[x]);
         }
         if (ok && nx > 0) ok = __all_sync(0xffffffffu, sm100::mbar_wait(&o_done[x], 0, abort_flag));
+        meet();              // (the last maxima have been read)
+        *mine = l;
+        meet();
+        l += *other;
         if (ok) {
             sm100::tc_fence_after_sync();
             const bool live = row < rows && tok < lq;
@@ -477,7 +500,8 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             __nv_bfloat16* dst = a.out + (int64_t)(q0 + tok) * a.o_tok + (int64_t)(kvh * a.G + row % a.G) * a.o_head;
             const bool odd = nx > 0 && *odd_v != 0;
 #pragma unroll 1
-            for (int c = 0; c < DP; c += 32) {
+            for (int c = 0; c < HD; c += 32) {
+                const int d = hf * HD + c;
                 uint32_t r[32];
                 if (nx > 0) {
                     sm100::tmem_ld_32x32(to + c, r);
@@ -487,35 +511,35 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                     for (int e = 0; e < 32; ++e) r[e] = 0u;
                 }
                 if (live) {
-                    float f[32];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) f[e] = inv == 0.f ? 0.f : __uint_as_float(r[e]) * inv;
+                    for (int e = 0; e < 32; ++e) r[e] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(r[e]) * inv);
                     if (odd) {      // infinities and NaNs that were taken out of V, back to the rows that see them
                         const __nv_bfloat16* vp = a.v + (a.cu_k != nullptr ? 0 : (int64_t)s * a.v_seq) + (int64_t)kvh * a.v_head + (int64_t)k0 * a.v_row;
                         for (int kk = seen_by_all; kk < cnt; ++kk)
 #pragma unroll
                             for (int e = 0; e < 32; ++e) {
-                                const float y = c + e < a.D ? __bfloat162float(vp[(int64_t)kk * a.v_row + c + e]) : 0.f;
-                                if (!(fabsf(y) <= 3.4e38f)) f[e] += y;
+                                const float y = d + e < a.D ? __bfloat162float(vp[(int64_t)kk * a.v_row + d + e]) : 0.f;
+                                if (!(fabsf(y) <= 3.4e38f)) r[e] = __float_as_uint(__uint_as_float(r[e]) + y);
                             }
                     }
+                    uint32_t h[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) h[e] = bf2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (c + 8 * e < a.D)
-                            *reinterpret_cast<uint4*>(dst + c + 8 * e) = make_uint4(bf2(f[8 * e], f[8 * e + 1]), bf2(f[8 * e + 2], f[8 * e + 3]),
-                                                                                   bf2(f[8 * e + 4], f[8 * e + 5]), bf2(f[8 * e + 6], f[8 * e + 7]));
+                        if (d + 8 * e < a.D) *reinterpret_cast<uint4*>(dst + d + 8 * e) = make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
                 }
             }
         }
     }
 
-    if (!ok && (warp == 8 || warp == 9)) {     // gave up: let copies and products already in flight land
+    if (!ok && (warp == SM_WARPS || warp == SM_WARPS + 1)) {     // gave up: let copies and products already in flight land
         const long long t0 = clock64();
         while (clock64() - t0 < 20000000LL) { }
     }
     sm100::tc_fence_before_sync();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == SM_WARPS + 1) {
         sm100::tc_fence_after_sync();
         sm100::tmem_dealloc(tmem, 512);
     }
@@ -561,7 +585,7 @@ static int run(const hxq_attn* p, int32_t* status, cudaStream_t stream) {
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return HXQ_E_DEVICE;
     if (!attr_set[dev]) {
         cudaFuncAttributes fa;        // the warps' exchange of registers counts on what the launch brings
-        if (cudaFuncGetAttributes(&fa, attn_prompt_kernel<DP>) != cudaSuccess || fa.numRegs < 168) return HXQ_E_DEVICE;
+        if (cudaFuncGetAttributes(&fa, attn_prompt_kernel<DP>) != cudaSuccess || fa.numRegs < kRegsLaunch) return HXQ_E_DEVICE;
         if (cudaFuncSetAttribute(attn_prompt_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::kSmem) != cudaSuccess) return HXQ_E_DEVICE;
         attr_set[dev] = true;
     }
