@@ -8,7 +8,7 @@
 //
 // One CTA takes two tiles of 128 rows.  A row is (token, head of the group): the G query heads of a KV head share
 // its keys, so a tile spans 128 / G tokens, the causal edge wastes that much less, and a short prompt fills its
-// tiles G times better than with a head per CTA.  Per 128 keys and tile, all on the tensor cores (tcgen05):
+// tiles G times better than with a head per CTA.  Per 64 keys and tile, all on the tensor cores (tcgen05):
 //
 //     S = Q K^T       both operands in shared memory (TMA, 128-byte swizzle), S in tensor memory
 //     P = 2^(scale' S - m)      one thread per row, in registers: running maximum m and sum; P goes back to tensor
@@ -16,10 +16,16 @@
 //     O += P V        A operand from tensor memory, V as it lies in memory (its rows are the contraction), O in
 //                     tensor memory for the whole row
 //
-// Roles: warps 0-3 and 4-7 are the two tiles' softmax (and epilogue), warp 8 feeds K and V through a ring of
-// 128-row tiles, warp 9 issues the MMAs (while one tile's softmax runs, the other tile's products do), warps 10 and 11
-// clean V tiles.  P is rounded to bf16, V's type (the MMA takes no other beside it): 2^-9 at most per weight, as much as
-// the output's own rounding; the sum that divides takes the weights before rounding.
+// Roles: warps 0-3 and 4-7 are the two tiles' softmax and epilogue, warp 8 feeds K and V through a ring of
+// 64-row tiles, warp 9 issues the MMAs, warps 10 and 11 clean V tiles.  P is rounded to bf16, V's type (the MMA takes no
+// other beside it): 2^-9 at most per weight, as much as the output's own rounding; the sum that divides takes the weights
+// before rounding.
+//
+// A step's products, its softmax and the signals between them (about 1000 cycles of the last two thirds each) depend on
+// one another, and two tiles alone do not hide that: with 128 keys a step, S of the next waiting for P V of this one,
+// a step took 3900 cycles, its MMAs 2048.  So S has two buffers a tile, of 64 keys, tensor memory being full with them
+// and O: the next step's scores are there when a warp comes for them.  (Products of 64 keys cost a third more, 670 cycles a
+// step and tile instead of 512: a Q tile is read from shared memory for half the work.)
 //
 // The reference point m moves only when the maximum has grown by more than 2^8: weights stay below 256, nothing
 // overflows, the result is the same, and O is rarely rescaled.
@@ -44,19 +50,19 @@ bool make_map_nd(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void*
 namespace attnp {
 
 constexpr int BM = 128;                     // rows of a tile
-constexpr int BN = 128;                     // keys of a step
-constexpr int SM_WARPS = 16;                // softmax: eight per tile
+constexpr int BN = 64;                      // keys of a step
+constexpr int SM_WARPS = 8;                 // softmax: four per tile
 constexpr int NUM_THREADS = 32 * (SM_WARPS + 4);
-constexpr int kMaxStages = 8;
-constexpr int kBarBytes = 512 + 2 * 2 * 128 * 4;        // barriers, and what the two halves of a row tell each other
+constexpr int kMaxStages = 16;
+constexpr int kBarBytes = 768;
 constexpr int kPolyOf4 = 1;                 // of four pairs of weights, how many are made on the multiply-add units
-constexpr int kRegsLaunch = 96, kRegsSoftmax = 104, kRegsOther = 64;      // of a thread, after the roles have parted
+constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 88;      // of a thread: at launch, and after the roles have parted
 
 template <int DP>
 struct Sizes {
-    static constexpr int kTile = BM * DP * 2;                 // a Q, K or V tile
-    static constexpr int kStages = DP == 128 ? 5 : 8;
-    static constexpr int kSmem = (2 + kStages) * kTile + kBarBytes;
+    static constexpr int kQ = BM * DP * 2, kTile = BN * DP * 2;      // a Q tile, a K or V tile
+    static constexpr int kStages = DP == 128 ? 10 : 16;
+    static constexpr int kSmem = 2 * kQ + kStages * kTile + kBarBytes;
 };
 
 struct Args {
@@ -80,13 +86,26 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(sm100::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
-// D[tmem] (+)= A[tmem] * B[smem]
-__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+// D[tmem] (+)= A * B[smem], A in shared memory or in tensor memory, and the arrival when all products so far have retired; by the
+// lane whose `leader` is set.
+__device__ __forceinline__ void umma_ss(uint32_t leader, uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t leader, uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t leader, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(sm100::smem_u32(bar)), "r"(leader) : "memory");
 }
 __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
@@ -102,6 +121,31 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// As sm100::mbar_wait, bounded by the number of tries (each of which the hardware may stretch to microseconds) and in few instructions: every role's
+// loop shares a small instruction cache.
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+#pragma unroll 1
+    for (int i = 0; i < (1 << 19); ++i) {
+        if (sm100::mbar_try_wait(bar, parity)) return true;
+        if (*abort != 0) return false;
+    }
+    *abort = 1;
+    return false;
+}
+__device__ __forceinline__ uint32_t elect_one() {       // one lane of the whole warp
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+    return p;
+}
+__device__ __forceinline__ uint32_t peek(uint64_t* bar, uint32_t parity) {       // has the phase completed?
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(sm100::smem_u32(bar)), "r"(parity) : "memory");
+    return done;
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -161,27 +205,26 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
 attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v, const Args a) {
     using Z = Sizes<DP>;
-    constexpr int NS = Z::kStages, TILE = Z::kTile, HALF = BM * 128;      // HALF: 64 of the dimensions of a tile
+    constexpr int NS = Z::kStages, QT = Z::kQ, TILE = Z::kTile;
+    constexpr int QHALF = BM * 128, HALF = BN * 128;      // 64 of the dimensions of a Q tile, of a K or V tile
     extern __shared__ __align__(1024) char smem[];        // (no room for slack: the swizzled tiles need that alignment, checked here)
     if (sm100::smem_u32(smem) % 1024 != 0) {
         if (threadIdx.x == 0 && a.status != nullptr) atomicExch(a.status, HXQ_E_ALIGN);
         return;
     }
-    char* ring = smem + 2 * TILE;
+    char* ring = smem + 2 * QT;
     uint64_t* full = reinterpret_cast<uint64_t*>(ring + NS * TILE);     // [NS] a tile has landed, ready for its product
     uint64_t* empty = full + kMaxStages;        // [NS] its products have retired
     uint64_t* raw = empty + kMaxStages;         // [NS] a V tile that is to be cleaned has landed (full is not signalled) ...
     uint64_t* clean = raw + kMaxStages;         // [NS] ... and has been cleaned
     uint64_t* q_full = clean + kMaxStages;
-    uint64_t* s_full = q_full + 1;              // [2] S of a tile is complete (and the product before it)
-    uint64_t* p_ready = s_full + 2;             // [2] P is written, O is rescaled
-    uint64_t* o_done = p_ready + 2;             // [2] the last product of a tile has retired
+    uint64_t* s_full = q_full + 1;              // [2 tiles][2 buffers] S is complete
+    uint64_t* p_ready = s_full + 4;             // [2][2] P is written, O is rescaled
+    uint64_t* o_done = p_ready + 4;             // [2] P V has retired, once a step
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile int* gave_up = abort_flag + 2;     // [2] the step at which a softmax warp's wait ran out
     volatile int* odd_v = abort_flag + 1;       // a V tile held an infinity or a NaN that some row does not see
-    float* talk = reinterpret_cast<float*>(ring + NS * TILE + 512);        // [2 tiles][2 halves][128 rows]
-    static_assert((4 * kMaxStages + 7) * 8 + 20 <= 512, "barrier area");
+    static_assert((4 * kMaxStages + 11) * 8 + 12 <= kBarBytes, "barrier area");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -228,14 +271,14 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             sm100::mbar_init(&clean[i], 2);
         }
         sm100::mbar_init(q_full, 1);
-        for (int x = 0; x < 2; ++x) {
-            sm100::mbar_init(&s_full[x], 1);
-            sm100::mbar_init(&p_ready[x], SM_WARPS / 2);
-            sm100::mbar_init(&o_done[x], 1);
+        for (int i = 0; i < 4; ++i) {
+            sm100::mbar_init(&s_full[i], 1);
+            sm100::mbar_init(&p_ready[i], SM_WARPS / 2);
         }
+        sm100::mbar_init(&o_done[0], 1);
+        sm100::mbar_init(&o_done[1], 1);
         *abort_flag = 0;
         *odd_v = 0;
-        gave_up[0] = gave_up[1] = 0x7fffffff;
         sm100::fence_barrier_init();
         sm100::prefetch_tensormap(&map_q);
         sm100::prefetch_tensormap(&map_k);
@@ -248,7 +291,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     // rows of the Q tiles that no token fills
     for (int i = threadIdx.x; i < 2 * (DP / 64) * (BM - rows) * 8; i += NUM_THREADS) {
         const int part = i / ((BM - rows) * 8), rem = i - part * (BM - rows) * 8;
-        *reinterpret_cast<uint4*>(smem + part * HALF + (rows + (rem >> 3)) * 128 + (rem & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(smem + part * QHALF + (rows + (rem >> 3)) * 128 + (rem & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
     }
     sm100::fence_proxy_async_smem();
     sm100::tc_fence_before_sync();
@@ -256,105 +299,122 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     sm100::tc_fence_after_sync();
     // The next kernel may come in only now: one that took tensor memory before this CTA did would keep it waiting.
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const uint32_t tmem = *tmem_slot;       // S0 | S1 | O0 | O1, 128 columns each
+    const uint32_t tmem = *tmem_slot;       // S of tile 0: two buffers of 64 columns; of tile 1; O of either, 128 columns each
     bool ok = true;
 
     static_assert(32 * SM_WARPS * kRegsSoftmax + 128 * kRegsOther <= NUM_THREADS * kRegsLaunch, "no more registers than the launch brings");
     if (warp >= SM_WARPS) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == SM_WARPS) {
-        // ------------------------------------------------------------ loads
+        // ------------------------------------------------------------ loads, in the order of their use: K0 K1 | V0 K2 | V1 K3 | ...
         if (lane == 0 && n > 0) {
             sm100::mbar_arrive_expect_tx(q_full, 2u * (DP / 64) * (uint32_t)rows * 128u);
             for (int x = 0; x < 2; ++x)
                 for (int h = 0; h < DP / 64; ++h)
-                    tma_load_3d(sm100::smem_u32(smem + x * TILE + h * HALF), &map_q, q_full, 64 * h, kvh * a.G, q0 + i0 + x * a.tpg);
+                    tma_load_3d(sm100::smem_u32(smem + x * QT + h * QHALF), &map_q, q_full, 64 * h, kvh * a.G, q0 + i0 + x * a.tpg);
             int slot = 0;
             uint32_t ph = 1;
-            for (int it = 0; it < 2 * n && ok; ++it) {
-                ok = sm100::mbar_wait(&empty[slot], ph, abort_flag);
-                if (!ok) break;
-                uint64_t* bar = (it & 1) && (it >> 1) >= jc ? &raw[slot] : &full[slot];
+            auto load = [&](bool is_v, int j) {
+                ok = bar_wait(&empty[slot], ph, abort_flag);
+                if (!ok) return;
+                uint64_t* bar = is_v && j >= jc ? &raw[slot] : &full[slot];
                 sm100::mbar_arrive_expect_tx(bar, TILE);
                 const uint32_t dst = sm100::smem_u32(ring + slot * TILE);
                 for (int h = 0; h < DP / 64; ++h)
-                    tma_load_4d(dst + h * HALF, (it & 1) ? &map_v : &map_k, bar, 64 * h, k0 + (it >> 1) * BN, kvh, a.cu_k != nullptr ? 0 : s);
+                    tma_load_4d(dst + h * HALF, is_v ? &map_v : &map_k, bar, 64 * h, k0 + j * BN, kvh, a.cu_k != nullptr ? 0 : s);
                 if (++slot == NS) { slot = 0; ph ^= 1u; }
+            };
+            load(false, 0);
+            if (ok && n > 1) load(false, 1);
+            for (int j = 0; j < n && ok; ++j) {
+                load(true, j);
+                if (ok && j + 2 < n) load(false, j + 2);
             }
         }
     } else if (warp == SM_WARPS + 1) {
         // ------------------------------------------------------------ MMAs
-        if (lane == 0 && n > 0) {
+        // The whole warp walks the steps without a branch that its lanes could part at, and a predicate picks the lane that issues:
+        // what the loop computes is then known to be the same in every lane and stays in uniform registers, where the products
+        // want it.  A barrier is looked at before the products in front of its use are issued, and waited for
+        // only if it was not done then: issuing is in order, so a wait holds up what comes after it, 150 cycles and more even
+        // when there is nothing to wait for.  (670 cycles a step and tile, which is its products' time; with the loop inside an
+        // "if (lane == 0)" 1000 and more, each descriptor being moved between register files, with four waits a step 1000.)
+        const int un = __shfl_sync(0xffffffffu, n, 0), un0 = __shfl_sync(0xffffffffu, n0, 0), un1 = __shfl_sync(0xffffffffu, n1, 0);
+        const int ujc = __shfl_sync(0xffffffffu, jc, 0);
+        const uint32_t ut = __shfl_sync(0xffffffffu, tmem, 0);
+        if (un > 0) {
+            const uint32_t leader = elect_one();
             const uint32_t idesc_s = sm100::make_idesc_bf16(BM, BN);
             const uint32_t idesc_o = sm100::make_idesc_bf16(BM, DP) | (1u << 16);      // B is N-major
-            int slot = 0;
+            const uint32_t q_at = sm100::smem_u32(smem), ring_at = sm100::smem_u32(ring);
             uint32_t full_ph = 0, clean_ph = 0;       // parity of each slot's next phase: not every round signals both
-            auto next = [&]() { if (++slot == NS) slot = 0; };
-            auto wait = [&](uint64_t* bars, uint32_t& phases, int sl) {
-                const bool done = sm100::mbar_wait(&bars[sl], (phases >> sl) & 1u, abort_flag);
-                phases ^= 1u << sl;
-                return done;
-            };
-            auto scores = [&](int x, int sl) {
-                const uint32_t qa = sm100::smem_u32(smem + x * TILE), ka = sm100::smem_u32(ring + sl * TILE);
+            auto after = [&](int sl) { return sl + 1 == NS ? 0 : sl + 1; };
+            auto scores = [&](int x, int buf, int sl) {
+                const uint32_t qa = q_at + (uint32_t)(x * QT), ka = ring_at + (uint32_t)(sl * TILE);
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k)
-                    sm100::umma_bf16(tmem + 128u * x, sm100::make_desc_k_sw128(qa + (k >> 2) * HALF) + 2 * (k & 3),
-                                     sm100::make_desc_k_sw128(ka + (k >> 2) * HALF) + 2 * (k & 3), idesc_s, k > 0);
-                sm100::umma_commit(&s_full[x]);
+                    umma_ss(leader, ut + (uint32_t)(128 * x + 64 * buf), sm100::make_desc_k_sw128(qa + (k >> 2) * QHALF) + 2 * (k & 3),
+                            sm100::make_desc_k_sw128(ka + (k >> 2) * HALF) + 2 * (k & 3), idesc_s, k > 0);
+                commit(leader, &s_full[2 * x + buf]);
             };
-            ok = sm100::mbar_wait(q_full, 0, abort_flag) && wait(full, full_ph, 0);
-            if (ok) {
-                sm100::tc_fence_after_sync();
-                if (n0 > 0) scores(0, 0);
-                if (n1 > 0) scores(1, 0);
-                sm100::umma_commit(&empty[0]);
-                next();
-            }
-            for (int j = 0; j < n && ok; ++j) {
-                const int v_slot = slot;
-                ok = j >= jc ? wait(clean, clean_ph, v_slot) : wait(full, full_ph, v_slot);
+            int slot = 0;
+            ok = bar_wait(q_full, 0, abort_flag);
+            for (int j = 0; j < 2 && j < un && ok; ++j) {
+                ok = __all_sync(0xffffffffu, bar_wait(&full[slot], 0, abort_flag));
+                full_ph ^= 1u << slot;
                 if (!ok) break;
                 sm100::tc_fence_after_sync();
-                next();
-                const int k_slot = slot;
-                bool have_k = false;
-                for (int x = 0; x < 2 && ok; ++x) {
-                    const int nx = x ? n1 : n0;
+                if (j < un0) scores(0, j, slot);
+                if (j < un1) scores(1, j, slot);
+                commit(leader, &empty[slot]);
+                slot = after(slot);
+            }
+            uint32_t kv_done = 0, p_done = 0;
+            for (int j = 0; j < un && ok; ++j) {
+                const int buf = j & 1, v_slot = slot, k_slot = after(slot);
+                const bool more = j + 2 < un, cleaned = j >= ujc;
+                if (!kv_done) {
+                    ok = bar_wait(cleaned ? &clean[v_slot] : &full[v_slot], ((cleaned ? clean_ph : full_ph) >> v_slot) & 1u, abort_flag);
+                    if (more) ok = bar_wait(&full[k_slot], (full_ph >> k_slot) & 1u, abort_flag) && ok;
+                }
+                if (cleaned) clean_ph ^= 1u << v_slot; else full_ph ^= 1u << v_slot;
+                if (more) full_ph ^= 1u << k_slot;
+                slot = more ? after(k_slot) : k_slot;
+                const uint64_t dv = make_desc_mn_sw128(ring_at + (uint32_t)(v_slot * TILE), HALF);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int nx = x ? un1 : un0;
+                    if (j < nx && !p_done) ok = bar_wait(&p_ready[2 * x + buf], (uint32_t)(j >> 1) & 1u, abort_flag) && ok;
+                    sm100::tc_fence_after_sync();
+                    // the next looks: at the other tile's weights of this step, or this tile's of the next and the next V and K
+                    if (x == 0) {
+                        p_done = peek(&p_ready[2 + buf], (uint32_t)(j >> 1) & 1u);
+                    } else {
+                        const bool next_cleaned = j + 1 >= ujc;
+                        const int ks = after(slot);
+                        p_done = peek(&p_ready[buf ^ 1], (uint32_t)((j + 1) >> 1) & 1u);
+                        kv_done = peek(next_cleaned ? &clean[slot] : &full[slot], ((next_cleaned ? clean_ph : full_ph) >> slot) & 1u);
+                        kv_done &= peek(&full[ks], (full_ph >> ks) & 1u) | (uint32_t)(j + 3 >= un);
+                    }
                     if (j < nx) {
-                        ok = sm100::mbar_wait(&p_ready[x], (uint32_t)j & 1u, abort_flag);
-                        if (!ok) break;
-                        sm100::tc_fence_after_sync();
-                        const uint64_t dv = make_desc_mn_sw128(sm100::smem_u32(ring + v_slot * TILE), HALF);
 #pragma unroll
                         for (int k = 0; k < BN / 16; ++k)
-                            umma_ts(tmem + 256u + 128u * x, tmem + 128u * x + 8 * k, dv + k * (2048 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
-                        if (j == nx - 1) sm100::umma_commit(&o_done[x]);
+                            umma_ts(leader, ut + (uint32_t)(256 + 128 * x), ut + (uint32_t)(128 * x + 64 * buf + 8 * k), dv + k * (2048 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+                        commit(leader, &o_done[x]);
                     }
-                    if (j + 1 < nx) {
-                        if (!have_k) {
-                            ok = wait(full, full_ph, k_slot);
-                            if (!ok) break;
-                            sm100::tc_fence_after_sync();
-                            have_k = true;
-                        }
-                        scores(x, k_slot);       // over P, which the product before it reads: issued in order
-                    }
+                    if (j + 2 < nx) scores(x, buf, k_slot);       // over P, which the product before it reads: issued in order
                 }
-                if (!ok) break;
-                sm100::umma_commit(&empty[v_slot]);
-                if (j + 1 < n) {
-                    sm100::umma_commit(&empty[k_slot]);
-                    next();
-                }
+                commit(leader, &empty[v_slot]);
+                if (more) commit(leader, &empty[k_slot]);
+                ok = __all_sync(0xffffffffu, ok);
             }
         }
     } else {
         // ------------------------------------------------------------ V tiles that some row sees only in part
         uint32_t raw_ph = 0;
         for (int j = jc; j < n; ++j) {
-            const int slot = (2 * j + 1) % NS;
-            ok = __all_sync(0xffffffffu, sm100::mbar_wait(&raw[slot], (raw_ph >> slot) & 1u, abort_flag));
+            const int slot = (j + (j + 2 < n ? j + 2 : n)) % NS;        // V tiles before it, and K tiles
+            ok = __all_sync(0xffffffffu, bar_wait(&raw[slot], (raw_ph >> slot) & 1u, abort_flag));
             raw_ph ^= 1u << slot;
             if (!ok) break;
             char* tile = ring + slot * TILE;
@@ -386,59 +446,61 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     }
     } else {
         // ------------------------------------------------------------ softmax and epilogue: TMEM lane == row
-        // Two threads to a row, in two warps: one per half of a step's keys, and of the output's dimensions.
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-        constexpr int HK = BN / 2, HD = DP / 2;
-        const int x = warp >> 3, hf = (warp >> 2) & 1, row = 32 * (warp & 3) + lane;
+        const int x = warp >> 2, row = 32 * (warp & 3) + lane;
         const int nx = x ? n1 : n0;
         const int tok = i0 + x * a.tpg + row / a.G;
         const int cnt = count(tok);
         const int seen = nx > 0 ? count(i0 + x * a.tpg) : 0;        // keys that every row of the tile sees
         const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-        const uint32_t ts = t_lane + 128u * x, to = t_lane + 256u + 128u * x + (uint32_t)(hf * HD);
+        const uint32_t to = t_lane + 256u + 128u * x;
         const float sc = a.scale_log2;
-        float* mine = talk + (2 * x + hf) * 128 + row;
-        const float* other = talk + (2 * x + (hf ^ 1)) * 128 + row;
-        auto meet = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + x), "n"(32 * SM_WARPS / 2) : "memory"); };        // the tile's eight warps
-        float ref = -INFINITY, l = 0.f;         // in units of S; l: of this half's keys
+        float ref = -INFINITY, l = 0.f;         // in units of S
+        float first = 0.f, bias = 0.f;
+        bool far = false;
         for (int j = 0; j < nx; ++j) {
-            ok = __all_sync(0xffffffffu, sm100::mbar_wait(&s_full[x], (uint32_t)j & 1u, abort_flag));
-            if (!ok && lane == 0) gave_up[x] = j;
+            const int buf = j & 1;
+            const uint32_t ts = t_lane + 128u * x + 64u * buf;
+            ok = __all_sync(0xffffffffu, bar_wait(&s_full[2 * x + buf], (uint32_t)(j >> 1) & 1u, abort_flag));
+            if (!ok) break;
             sm100::tc_fence_after_sync();
-            uint32_t r[HK];
+            uint32_t r[BN];
 #pragma unroll
-            for (int c = 0; c < HK; c += 32) sm100::tmem_ld_32x32(ts + hf * HK + c, reinterpret_cast<uint32_t(&)[32]>(r[c]));
+            for (int c = 0; c < BN; c += 32) sm100::tmem_ld_32x32(ts + c, reinterpret_cast<uint32_t(&)[32]>(r[c]));
             sm100::tmem_ld_wait();
             if ((j + 1) * BN > seen) {
-                const int lim = cnt - j * BN - hf * HK;
+                const int lim = cnt - j * BN;
 #pragma unroll
-                for (int e = 0; e < HK; ++e) if (e >= lim) r[e] = 0xff800000u;
+                for (int e = 0; e < BN; ++e) if (e >= lim) r[e] = 0xff800000u;
             }
             float m4[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 m4[k] = max3(__uint_as_float(r[k]), __uint_as_float(r[4 + k]), __uint_as_float(r[8 + k]));
 #pragma unroll
-                for (int e = 12 + k; e < HK - 4; e += 8) m4[k] = max3(m4[k], __uint_as_float(r[e]), __uint_as_float(r[e + 4]));
+                for (int e = 12 + k; e < BN - 4; e += 8) m4[k] = max3(m4[k], __uint_as_float(r[e]), __uint_as_float(r[e + 4]));
             }
-            static_assert((HK - 16) % 8 == 0, "the pairs above end four before the end");
-            float mx = max3(max3(m4[0], m4[1], __uint_as_float(r[HK - 4])), max3(m4[2], m4[3], __uint_as_float(r[HK - 3])),
-                            max3(__uint_as_float(r[HK - 2]), __uint_as_float(r[HK - 1]), -INFINITY));
-            *mine = mx;
-            meet();
-            if (gave_up[x] <= j) { ok = false; break; }        // all eight warps leave at the same step: nobody is missed at a barrier
-            mx = max3(mx, *other, -INFINITY);
-            if (!(mx < INFINITY)) l = __uint_as_float(0x7fc00000u);        // a score that is infinite or none: so is the row
+            static_assert((BN - 16) % 8 == 0, "the pairs above end four before the end");
+            const float mx = max3(max3(m4[0], m4[1], __uint_as_float(r[BN - 4])), max3(m4[2], m4[3], __uint_as_float(r[BN - 3])),
+                                  max3(__uint_as_float(r[BN - 2]), __uint_as_float(r[BN - 1]), -INFINITY));
             // a new reference point where the maximum has grown by more than 2^8
             const bool move = (mx - ref) * sc > 8.f;        // (-inf - -inf is NaN: no)
-            const float old = ref;
-            if (move) ref = mx;
-            if (__any_sync(0xffffffffu, move)) {
-                const float corr = move ? ex2((old - ref) * sc) : 1.f;
+            if (__any_sync(0xffffffffu, move || !(mx < INFINITY))) {
+                if (!(mx < INFINITY)) l = __uint_as_float(0x7fc00000u);        // a score that is infinite or none: so is the row
+                const float corr = move ? ex2((ref - mx) * sc) : 1.f;
+                if (move) ref = mx;
                 l *= corr;
+                // 2^(S sc - ref sc) in one multiply-add: the rounding of ref sc shifts a whole row and divides out, unless
+                // scores are so large that it is itself large; then the difference is taken first
+                far = __any_sync(0xffffffffu, ref != -INFINITY && fabsf(ref * sc) > 65536.f);
+                first = ref == -INFINITY ? 0.f : ref;
+                bias = far ? 0.f : -first * sc;
                 if (j > 0) {
+                    ok = __all_sync(0xffffffffu, bar_wait(&o_done[x], (uint32_t)(j - 1) & 1u, abort_flag));
+                    if (!ok) break;
+                    sm100::tc_fence_after_sync();
 #pragma unroll 1
-                    for (int c = 0; c < HD; c += 16) {
+                    for (int c = 0; c < DP; c += 16) {
                         uint32_t o[16];
                         tmem_ld_32x16(to + c, o);
                         sm100::tmem_ld_wait();
@@ -448,19 +510,14 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                     }
                 }
             }
-            // 2^(S sc - ref sc) in one multiply-add: the rounding of ref sc shifts a whole row and divides out, unless
-            // scores are so large that it is itself large; then the difference is taken first
-            const bool far = __any_sync(0xffffffffu, ref != -INFINITY && fabsf(ref * sc) > 65536.f);
-            const float bias = ref == -INFINITY || far ? 0.f : -ref * sc;
             if (far) {
-                const float first = ref == -INFINITY ? 0.f : ref;
 #pragma unroll
-                for (int e = 0; e < HK; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) - first);
+                for (int e = 0; e < BN; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) - first);
             }
             const f2 sc2 = pair(sc, sc), bias2 = pair(bias, bias);
             f2 l2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
-            for (int c = 0; c < HK; c += 32) {
+            for (int c = 0; c < BN; c += 32) {
                 uint32_t p[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -478,7 +535,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                     l2[e & 1] = add2(l2[e & 1], y);
                     p[e] = bf2(y0, y1);
                 }
-                tmem_st_32x16(ts + (hf * HK + c) / 2, p);        // over scores that both halves have taken
+                tmem_st_32x16(ts + c / 2, p);        // over scores that this warp has taken
             }
             float l0, l1;
             split(add2(l2[0], l2[1]), l0, l1);
@@ -486,13 +543,11 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             tmem_st_wait();
             sm100::tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) sm100::mbar_arrive(&p_ready[x]);
+            if (lane == 0) sm100::mbar_arrive(&p_ready[2 * x + buf]);
         }
-        if (ok && nx > 0) ok = __all_sync(0xffffffffu, sm100::mbar_wait(&o_done[x], 0, abort_flag));
-        meet();              // (the last maxima have been read)
-        *mine = l;
-        meet();
-        l += *other;
+        // (the last scores' barrier told that all but the last two products have retired)
+        if (ok && nx > 1) ok = __all_sync(0xffffffffu, bar_wait(&o_done[x], (uint32_t)(nx - 2) & 1u, abort_flag));
+        if (ok && nx > 0) ok = __all_sync(0xffffffffu, bar_wait(&o_done[x], (uint32_t)(nx - 1) & 1u, abort_flag));
         if (ok) {
             sm100::tc_fence_after_sync();
             const bool live = row < rows && tok < lq;
@@ -500,11 +555,10 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             __nv_bfloat16* dst = a.out + (int64_t)(q0 + tok) * a.o_tok + (int64_t)(kvh * a.G + row % a.G) * a.o_head;
             const bool odd = nx > 0 && *odd_v != 0;
 #pragma unroll 1
-            for (int c = 0; c < HD; c += 32) {
-                const int d = hf * HD + c;
+            for (int d = 0; d < DP; d += 32) {
                 uint32_t r[32];
                 if (nx > 0) {
-                    sm100::tmem_ld_32x32(to + c, r);
+                    sm100::tmem_ld_32x32(to + d, r);
                     sm100::tmem_ld_wait();
                 } else {
 #pragma unroll
