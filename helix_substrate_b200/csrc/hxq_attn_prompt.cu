@@ -38,6 +38,8 @@
 
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "hxq_common.cuh"
 #include "hxq_sm100.cuh"
 
@@ -53,7 +55,7 @@ constexpr int BM = 128;                     // rows of a tile
 constexpr int BN = 64;                      // keys of a step
 constexpr int SM_WARPS = 8;                 // softmax: four per tile
 constexpr int NUM_THREADS = 32 * (SM_WARPS + 4);
-constexpr int kMaxStages = 16;
+constexpr int kMaxStages = 8;
 constexpr int kBarBytes = 768;
 constexpr int kPolyOf4 = 1;                 // of four pairs of weights, how many are made on the multiply-add units
 constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 88;      // of a thread: at launch, and after the roles have parted
@@ -61,8 +63,8 @@ constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 88;      // of
 template <int DP>
 struct Sizes {
     static constexpr int kQ = BM * DP * 2, kTile = BN * DP * 2;      // a Q tile, a K or V tile
-    static constexpr int kStages = DP == 128 ? 10 : 16;
-    static constexpr int kSmem = 2 * kQ + kStages * kTile + kBarBytes;
+    static constexpr int kStages = DP == 128 ? 5 : 8;                // of two tiles: the first two of K, then one of V and one of K
+    static constexpr int kSmem = 2 * kQ + 2 * kStages * kTile + kBarBytes;
 };
 
 struct Args {
@@ -102,10 +104,10 @@ __device__ __forceinline__ void umma_ts(uint32_t leader, uint32_t tmem_d, uint32
         "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
 }
-__device__ __forceinline__ void commit(uint32_t leader, uint64_t* bar) {
+__device__ __forceinline__ void commit(uint32_t leader, uint32_t bar) {
     asm volatile(
         "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(sm100::smem_u32(bar)), "r"(leader) : "memory");
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(leader) : "memory");
 }
 __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
@@ -121,31 +123,38 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// As sm100::mbar_wait, bounded by the number of tries (each of which the hardware may stretch to microseconds) and in few instructions: every role's
-// loop shares a small instruction cache.
-__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
-#pragma unroll 1
-    for (int i = 0; i < (1 << 19); ++i) {
-        if (sm100::mbar_try_wait(bar, parity)) return true;
-        if (*abort != 0) return false;
-    }
-    *abort = 1;
-    return false;
-}
 __device__ __forceinline__ uint32_t elect_one() {       // one lane of the whole warp
     uint32_t p;
     asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
     return p;
 }
-__device__ __forceinline__ uint32_t peek(uint64_t* bar, uint32_t parity) {       // has the phase completed?
+__device__ __forceinline__ uint32_t peek(uint32_t bar, uint32_t parity) {       // has the phase completed?
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done) : "r"(sm100::smem_u32(bar)), "r"(parity) : "memory");
+        : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done;
 }
+// As sm100::mbar_wait, bounded by the number of tries (each of which the hardware may stretch to microseconds) and in few
+// instructions: every role's loop shares a small instruction cache.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+#pragma unroll 1
+    for (int i = 0; i < (1 << 19); ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        if (done) return true;
+        if (*abort != 0) return false;
+    }
+    *abort = 1;
+    return false;
+}
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* abort) { return bar_wait(sm100::smem_u32(bar), parity, abort); }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -213,14 +222,14 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         return;
     }
     char* ring = smem + 2 * QT;
-    uint64_t* full = reinterpret_cast<uint64_t*>(ring + NS * TILE);     // [NS] a tile has landed, ready for its product
+    uint64_t* full = reinterpret_cast<uint64_t*>(ring + NS * 2 * TILE);      // [NS] a stage has landed, ready for its products
     uint64_t* empty = full + kMaxStages;        // [NS] its products have retired
-    uint64_t* raw = empty + kMaxStages;         // [NS] a V tile that is to be cleaned has landed (full is not signalled) ...
+    uint64_t* raw = empty + kMaxStages;         // [NS] a stage whose V tile is to be cleaned has landed (full is not signalled) ...
     uint64_t* clean = raw + kMaxStages;         // [NS] ... and has been cleaned
     uint64_t* q_full = clean + kMaxStages;
     uint64_t* s_full = q_full + 1;              // [2 tiles][2 buffers] S is complete
     uint64_t* p_ready = s_full + 4;             // [2][2] P is written, O is rescaled
-    uint64_t* o_done = p_ready + 4;             // [2] P V has retired, once a step
+    uint64_t* o_done = p_ready + 4;             // [2] the last P V but one has retired, and the last
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* odd_v = abort_flag + 1;       // a V tile held an infinity or a NaN that some row does not see
@@ -312,23 +321,21 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             for (int x = 0; x < 2; ++x)
                 for (int h = 0; h < DP / 64; ++h)
                     tma_load_3d(sm100::smem_u32(smem + x * QT + h * QHALF), &map_q, q_full, 64 * h, kvh * a.G, q0 + i0 + x * a.tpg);
+            const int slab = a.cu_k != nullptr ? 0 : s;
             int slot = 0;
             uint32_t ph = 1;
-            auto load = [&](bool is_v, int j) {
+            for (int i = -1; i < n; ++i) {          // stage i + 1: V of step i (K of step 0 at the start) and K of step i + 2
                 ok = bar_wait(&empty[slot], ph, abort_flag);
-                if (!ok) return;
-                uint64_t* bar = is_v && j >= jc ? &raw[slot] : &full[slot];
-                sm100::mbar_arrive_expect_tx(bar, TILE);
-                const uint32_t dst = sm100::smem_u32(ring + slot * TILE);
+                if (!ok) break;
+                const bool two = i < 0 ? n > 1 : i + 2 < n;
+                uint64_t* bar = i >= 0 && i >= jc ? &raw[slot] : &full[slot];
+                sm100::mbar_arrive_expect_tx(bar, two ? 2 * TILE : TILE);
+                const uint32_t dst = sm100::smem_u32(ring + slot * 2 * TILE);
                 for (int h = 0; h < DP / 64; ++h)
-                    tma_load_4d(dst + h * HALF, is_v ? &map_v : &map_k, bar, 64 * h, k0 + j * BN, kvh, a.cu_k != nullptr ? 0 : s);
+                    tma_load_4d(dst + h * HALF, i < 0 ? &map_k : &map_v, bar, 64 * h, k0 + (i < 0 ? 0 : i) * BN, kvh, slab);
+                if (two)
+                    for (int h = 0; h < DP / 64; ++h) tma_load_4d(dst + TILE + h * HALF, &map_k, bar, 64 * h, k0 + (i + 2) * BN, kvh, slab);
                 if (++slot == NS) { slot = 0; ph ^= 1u; }
-            };
-            load(false, 0);
-            if (ok && n > 1) load(false, 1);
-            for (int j = 0; j < n && ok; ++j) {
-                load(true, j);
-                if (ok && j + 2 < n) load(false, j + 2);
             }
         }
     } else if (warp == SM_WARPS + 1) {
@@ -346,78 +353,87 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             const uint32_t leader = elect_one();
             const uint32_t idesc_s = sm100::make_idesc_bf16(BM, BN);
             const uint32_t idesc_o = sm100::make_idesc_bf16(BM, DP) | (1u << 16);      // B is N-major
-            const uint32_t q_at = sm100::smem_u32(smem), ring_at = sm100::smem_u32(ring);
-            uint32_t full_ph = 0, clean_ph = 0;       // parity of each slot's next phase: not every round signals both
-            auto after = [&](int sl) { return sl + 1 == NS ? 0 : sl + 1; };
-            auto scores = [&](int x, int buf, int sl) {
-                const uint32_t qa = q_at + (uint32_t)(x * QT), ka = ring_at + (uint32_t)(sl * TILE);
+            const uint32_t full_at = sm100::smem_u32(full), empty_at = sm100::smem_u32(empty), clean_at = sm100::smem_u32(clean);
+            const uint32_t s_at = sm100::smem_u32(s_full), p_at = sm100::smem_u32(p_ready), o_at = sm100::smem_u32(o_done);
+            const uint64_t dq = sm100::make_desc_k_sw128(sm100::smem_u32(smem)), dk = sm100::make_desc_k_sw128(sm100::smem_u32(ring));
+            const uint64_t dv = make_desc_mn_sw128(sm100::smem_u32(ring), HALF);
+            uint32_t stage = 0, full_ph = 0, clean_ph = 0;       // full_ph, clean_ph: of each stage its next phase, not every round signals both
+            auto scores = [&](int x, int buf, uint32_t at) {     // at: of the K tile in the ring
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k)
-                    umma_ss(leader, ut + (uint32_t)(128 * x + 64 * buf), sm100::make_desc_k_sw128(qa + (k >> 2) * QHALF) + 2 * (k & 3),
-                            sm100::make_desc_k_sw128(ka + (k >> 2) * HALF) + 2 * (k & 3), idesc_s, k > 0);
-                commit(leader, &s_full[2 * x + buf]);
+                    umma_ss(leader, ut + (uint32_t)(128 * x + 64 * buf), dq + (uint32_t)((x * QT + (k >> 2) * QHALF) / 16 + 2 * (k & 3)),
+                            dk + (uint32_t)(at / 16) + (uint32_t)((k >> 2) * HALF / 16 + 2 * (k & 3)), idesc_s, k > 0);
+                commit(leader, s_at + (uint32_t)(8 * (2 * x + buf)));        // (and the products before it)
             };
-            int slot = 0;
-            ok = bar_wait(q_full, 0, abort_flag);
-            for (int j = 0; j < 2 && j < un && ok; ++j) {
-                ok = __all_sync(0xffffffffu, bar_wait(&full[slot], 0, abort_flag));
-                full_ph ^= 1u << slot;
-                if (!ok) break;
+            ok = bar_wait(q_full, 0, abort_flag) && bar_wait(full_at, 0, abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            full_ph = 1u;
+            if (ok) {
                 sm100::tc_fence_after_sync();
-                if (j < un0) scores(0, j, slot);
-                if (j < un1) scores(1, j, slot);
-                commit(leader, &empty[slot]);
-                slot = after(slot);
+                if (un0 > 0) scores(0, 0, 0);
+                if (un1 > 0) scores(1, 0, 0);
+                if (un0 > 1) scores(0, 1, TILE);
+                if (un1 > 1) scores(1, 1, TILE);
+                commit(leader, empty_at);
             }
+            stage = 1;
             uint32_t kv_done = 0, p_done = 0;
-            for (int j = 0; j < un && ok; ++j) {
-                const int buf = j & 1, v_slot = slot, k_slot = after(slot);
-                const bool more = j + 2 < un, cleaned = j >= ujc;
-                if (!kv_done) {
-                    ok = bar_wait(cleaned ? &clean[v_slot] : &full[v_slot], ((cleaned ? clean_ph : full_ph) >> v_slot) & 1u, abort_flag);
-                    if (more) ok = bar_wait(&full[k_slot], (full_ph >> k_slot) & 1u, abort_flag) && ok;
-                }
-                if (cleaned) clean_ph ^= 1u << v_slot; else full_ph ^= 1u << v_slot;
-                if (more) full_ph ^= 1u << k_slot;
-                slot = more ? after(k_slot) : k_slot;
-                const uint64_t dv = make_desc_mn_sw128(ring_at + (uint32_t)(v_slot * TILE), HALF);
+            // One step.  PLAIN: both tiles take part in it and in the one after the next, no V tile is cleaned.
+            auto step = [&](int j, auto plain_, auto buf_) {
+                constexpr bool PLAIN = decltype(plain_)::value;
+                constexpr int buf = decltype(buf_)::value;
+                const uint32_t here = stage, at = here * (uint32_t)(2 * TILE), p_phase = (uint32_t)(j >> 1) & 1u;
+                const bool cleaned = !PLAIN && j >= ujc;
+                if (!kv_done) ok = bar_wait((cleaned ? clean_at : full_at) + 8 * here, ((cleaned ? clean_ph : full_ph) >> here) & 1u, abort_flag) && ok;
+                if (cleaned) clean_ph ^= 1u << here; else full_ph ^= 1u << here;
+                stage = here + 1 == NS ? 0 : here + 1;
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     const int nx = x ? un1 : un0;
-                    if (j < nx && !p_done) ok = bar_wait(&p_ready[2 * x + buf], (uint32_t)(j >> 1) & 1u, abort_flag) && ok;
+                    const bool live = PLAIN || j < nx;
+                    if (live && !p_done) ok = bar_wait(p_at + (uint32_t)(8 * (2 * x + buf)), p_phase, abort_flag) && ok;
                     sm100::tc_fence_after_sync();
-                    // the next looks: at the other tile's weights of this step, or this tile's of the next and the next V and K
+                    // the next looks: at the other tile's weights of this step, or this tile's of the next and the next stage
                     if (x == 0) {
-                        p_done = peek(&p_ready[2 + buf], (uint32_t)(j >> 1) & 1u);
+                        p_done = peek(p_at + (uint32_t)(8 * (2 + buf)), p_phase);
                     } else {
-                        const bool next_cleaned = j + 1 >= ujc;
-                        const int ks = after(slot);
-                        p_done = peek(&p_ready[buf ^ 1], (uint32_t)((j + 1) >> 1) & 1u);
-                        kv_done = peek(next_cleaned ? &clean[slot] : &full[slot], ((next_cleaned ? clean_ph : full_ph) >> slot) & 1u);
-                        kv_done &= peek(&full[ks], (full_ph >> ks) & 1u) | (uint32_t)(j + 3 >= un);
+                        const bool next_cleaned = !PLAIN && j + 1 >= ujc;
+                        p_done = peek(p_at + (uint32_t)(8 * (buf ^ 1)), (uint32_t)((j + 1) >> 1) & 1u);
+                        kv_done = peek((next_cleaned ? clean_at : full_at) + 8 * stage, ((next_cleaned ? clean_ph : full_ph) >> stage) & 1u);
                     }
-                    if (j < nx) {
+                    if (live) {
 #pragma unroll
                         for (int k = 0; k < BN / 16; ++k)
-                            umma_ts(leader, ut + (uint32_t)(256 + 128 * x), ut + (uint32_t)(128 * x + 64 * buf + 8 * k), dv + k * (2048 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
-                        commit(leader, &o_done[x]);
+                            umma_ts(leader, ut + (uint32_t)(256 + 128 * x), ut + (uint32_t)(128 * x + 64 * buf + 8 * k), dv + at / 16 + (uint32_t)(k * (2048 / 16)), idesc_o,
+                                    (j > 0 || k > 0) ? 1u : 0u);
+                        if (!PLAIN && j + 2 >= nx) commit(leader, o_at + (uint32_t)(8 * x));
                     }
-                    if (j + 2 < nx) scores(x, buf, k_slot);       // over P, which the product before it reads: issued in order
+                    if (PLAIN || j + 2 < nx) scores(x, buf, at + TILE);       // over P, which the product before it reads: issued in order
                 }
-                commit(leader, &empty[v_slot]);
-                if (more) commit(leader, &empty[k_slot]);
+                commit(leader, empty_at + 8 * here);
                 ok = __all_sync(0xffffffffu, ok);
+            };
+            int j = 0;
+            const int plain = min(min(un0, un1) - 2, ujc);
+            for (; j + 2 <= plain && ok; j += 2) {
+                step(j, std::true_type{}, std::integral_constant<int, 0>{});
+                if (ok) step(j + 1, std::true_type{}, std::integral_constant<int, 1>{});
+            }
+            kv_done = 0;        // (the last plain step's look did not reckon with cleaning)
+            for (; j < un && ok; ++j) {
+                if (j & 1) step(j, std::false_type{}, std::integral_constant<int, 1>{});
+                else step(j, std::false_type{}, std::integral_constant<int, 0>{});
             }
         }
     } else {
         // ------------------------------------------------------------ V tiles that some row sees only in part
         uint32_t raw_ph = 0;
         for (int j = jc; j < n; ++j) {
-            const int slot = (j + (j + 2 < n ? j + 2 : n)) % NS;        // V tiles before it, and K tiles
+            const int slot = (j + 1) % NS;
             ok = __all_sync(0xffffffffu, bar_wait(&raw[slot], (raw_ph >> slot) & 1u, abort_flag));
             raw_ph ^= 1u << slot;
             if (!ok) break;
-            char* tile = ring + slot * TILE;
+            char* tile = ring + slot * 2 * TILE;
             const int from = seen_by_all - j * BN > 0 ? seen_by_all - j * BN : 0;         // rows before it are everybody's
             bool odd = false;
             for (int i = (warp - SM_WARPS - 2) * 32 + lane; i < (DP / 64) * (BN - from) * 8; i += 64) {
@@ -496,7 +512,9 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 first = ref == -INFINITY ? 0.f : ref;
                 bias = far ? 0.f : -first * sc;
                 if (j > 0) {
-                    ok = __all_sync(0xffffffffu, bar_wait(&o_done[x], (uint32_t)(j - 1) & 1u, abort_flag));
+                    // the product before has retired: the next step's scores come after it, or, at the end, its own signal does
+                    const bool next = j + 1 < nx;
+                    ok = __all_sync(0xffffffffu, bar_wait(next ? &s_full[2 * x + (buf ^ 1)] : &o_done[x], next ? (uint32_t)((j + 1) >> 1) & 1u : 0u, abort_flag));
                     if (!ok) break;
                     sm100::tc_fence_after_sync();
 #pragma unroll 1
@@ -545,9 +563,8 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             __syncwarp();
             if (lane == 0) sm100::mbar_arrive(&p_ready[2 * x + buf]);
         }
-        // (the last scores' barrier told that all but the last two products have retired)
-        if (ok && nx > 1) ok = __all_sync(0xffffffffu, bar_wait(&o_done[x], (uint32_t)(nx - 2) & 1u, abort_flag));
-        if (ok && nx > 0) ok = __all_sync(0xffffffffu, bar_wait(&o_done[x], (uint32_t)(nx - 1) & 1u, abort_flag));
+        if (ok && nx > 0) ok = __all_sync(0xffffffffu, bar_wait(&o_done[x], 0, abort_flag));
+        if (ok && nx > 1) ok = __all_sync(0xffffffffu, bar_wait(&o_done[x], 1, abort_flag));
         if (ok) {
             sm100::tc_fence_after_sync();
             const bool live = row < rows && tok < lq;
