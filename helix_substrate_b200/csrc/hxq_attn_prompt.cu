@@ -122,6 +122,19 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
           "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
 }
+// The wait for loads from tensor memory, through which their registers pass: nothing that uses them can be moved in front of it.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :: "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t elect_one() {       // one lane of the whole warp
     uint32_t p;
@@ -229,11 +242,12 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     uint64_t* q_full = clean + kMaxStages;
     uint64_t* s_full = q_full + 1;              // [2 tiles][2 buffers] S is complete
     uint64_t* p_ready = s_full + 4;             // [2][2] P is written, O is rescaled
-    uint64_t* o_done = p_ready + 4;             // [2] the last P V but one has retired, and the last
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 2);
+    uint64_t* o_done = p_ready + 4;             // [2][2] the last P V but one has retired; the last (a phase each: a wait for the first of two
+                                                // could come after the second)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 4);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* odd_v = abort_flag + 1;       // a V tile held an infinity or a NaN that some row does not see
-    static_assert((4 * kMaxStages + 11) * 8 + 12 <= kBarBytes, "barrier area");
+    static_assert((4 * kMaxStages + 13) * 8 + 12 <= kBarBytes, "barrier area");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -284,8 +298,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             sm100::mbar_init(&s_full[i], 1);
             sm100::mbar_init(&p_ready[i], SM_WARPS / 2);
         }
-        sm100::mbar_init(&o_done[0], 1);
-        sm100::mbar_init(&o_done[1], 1);
+        for (int i = 0; i < 4; ++i) sm100::mbar_init(&o_done[i], 1);
         *abort_flag = 0;
         *odd_v = 0;
         sm100::fence_barrier_init();
@@ -406,7 +419,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                         for (int k = 0; k < BN / 16; ++k)
                             umma_ts(leader, ut + (uint32_t)(256 + 128 * x), ut + (uint32_t)(128 * x + 64 * buf + 8 * k), dv + at / 16 + (uint32_t)(k * (2048 / 16)), idesc_o,
                                     (j > 0 || k > 0) ? 1u : 0u);
-                        if (!PLAIN && j + 2 >= nx) commit(leader, o_at + (uint32_t)(8 * x));
+                        if (!PLAIN && j + 2 >= nx) commit(leader, o_at + (uint32_t)(16 * x) + (j + 1 == nx ? 8u : 0u));
                     }
                     if (PLAIN || j + 2 < nx) scores(x, buf, at + TILE);       // over P, which the product before it reads: issued in order
                 }
@@ -483,7 +496,8 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             uint32_t r[BN];
 #pragma unroll
             for (int c = 0; c < BN; c += 32) sm100::tmem_ld_32x32(ts + c, reinterpret_cast<uint32_t(&)[32]>(r[c]));
-            sm100::tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < BN; c += 32) tmem_ld_wait(reinterpret_cast<uint32_t(&)[32]>(r[c]));
             if ((j + 1) * BN > seen) {
                 const int lim = cnt - j * BN;
 #pragma unroll
@@ -514,14 +528,14 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 if (j > 0) {
                     // the product before has retired: the next step's scores come after it, or, at the end, its own signal does
                     const bool next = j + 1 < nx;
-                    ok = __all_sync(0xffffffffu, bar_wait(next ? &s_full[2 * x + (buf ^ 1)] : &o_done[x], next ? (uint32_t)((j + 1) >> 1) & 1u : 0u, abort_flag));
+                    ok = __all_sync(0xffffffffu, bar_wait(next ? &s_full[2 * x + (buf ^ 1)] : &o_done[2 * x], next ? (uint32_t)((j + 1) >> 1) & 1u : 0u, abort_flag));
                     if (!ok) break;
                     sm100::tc_fence_after_sync();
 #pragma unroll 1
                     for (int c = 0; c < DP; c += 16) {
                         uint32_t o[16];
                         tmem_ld_32x16(to + c, o);
-                        sm100::tmem_ld_wait();
+                        tmem_ld_wait(o);
 #pragma unroll
                         for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
                         tmem_st_32x16(to + c, o);
@@ -563,8 +577,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             __syncwarp();
             if (lane == 0) sm100::mbar_arrive(&p_ready[2 * x + buf]);
         }
-        if (ok && nx > 0) ok = __all_sync(0xffffffffu, bar_wait(&o_done[x], 0, abort_flag));
-        if (ok && nx > 1) ok = __all_sync(0xffffffffu, bar_wait(&o_done[x], 1, abort_flag));
+        if (ok && nx > 0) ok = __all_sync(0xffffffffu, bar_wait(&o_done[2 * x + 1], 0, abort_flag));
         if (ok) {
             sm100::tc_fence_after_sync();
             const bool live = row < rows && tok < lq;
@@ -576,7 +589,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 uint32_t r[32];
                 if (nx > 0) {
                     sm100::tmem_ld_32x32(to + d, r);
-                    sm100::tmem_ld_wait();
+                    tmem_ld_wait(r);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) r[e] = 0u;

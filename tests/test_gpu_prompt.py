@@ -18,6 +18,14 @@ def _dev():
     return torch.device("cuda:0")
 
 
+@pytest.fixture(autouse=True)
+def _no_wait_gave_up():
+    """Every wait in the kernels is bounded; none may have run out."""
+    yield
+    from helix_substrate_b200.packed import _status_word
+    assert int(_status_word(_dev())) == 0
+
+
 def _want(q, k, v, scale, causal):
     lq, lk = q.shape[0], k.shape[0]
     seen = torch.ones(lq, lk, dtype=torch.bool, device=q.device)
