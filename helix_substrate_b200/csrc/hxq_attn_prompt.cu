@@ -57,6 +57,7 @@ constexpr int SM_WARPS = 8;                 // softmax: four per tile
 constexpr int NUM_THREADS = 32 * (SM_WARPS + 4);
 constexpr int kMaxStages = 8;
 constexpr int kBarBytes = 768;
+constexpr int kShare = 8, kAlone = 16;       // key tiles: that a CTA of a shared item has at least; up to which an item is not shared
 constexpr int kPolyOf4 = 1;                 // of four pairs of weights, how many are made on the multiply-add units
 constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 88;      // of a thread: at launch, and after the roles have parted
 
@@ -74,9 +75,105 @@ struct Args {
     __nv_bfloat16* out;
     int32_t* status;
     int64_t v_seq, v_head, v_row, o_tok, o_head;
-    int32_t Tq, Tk, S, nkv, G, D, tpg, n_ct, causal;
+    float* part;            // splits > 1: [items][splits][DP + 2][2 * BM]: reference point, sum, output before the division
+    int32_t Tq, Tk, S, nkv, G, D, tpg, n_ct, causal, splits, groups;       // groups of 32 rows of an item that any token can fill
     float scale_log2;
 };
+
+// ---- what a CTA is for
+
+struct Seq {
+    int q0, lq, k0, lk;     // first row and number of its queries, of its keys
+};
+__device__ __forceinline__ Seq sequence(const Args& a, int s) {
+    Seq r = {0, 0, 0, 0};
+    if (s >= a.S) return r;
+    const int q0 = a.cu_q[s], q1 = a.cu_q[s + 1];
+    if (a.cu_k == nullptr) {
+        const int64_t n = a.k_len[s];
+        r.lk = n < 0 ? 0 : (n > a.Tk ? a.Tk : (int)n);
+    } else {
+        const int k0 = a.cu_k[s], k1 = a.cu_k[s + 1];
+        r.k0 = k0 < 0 ? 0 : k0;
+        r.lk = (k1 > a.Tk ? a.Tk : k1) - r.k0;
+    }
+    r.q0 = q0 < 0 ? 0 : q0;
+    r.lq = (q1 > a.Tq ? a.Tq : q1) - r.q0;
+    if (r.lq < 0) r.lq = 0;
+    if (r.lk < 0) r.lk = 0;
+    return r;
+}
+__device__ __forceinline__ int reach(const Args& a, int lq, int keys, int i) {      // keys that token i sees
+    if (!a.causal || i >= lq) return keys;
+    const int n = keys - lq + i + 1;
+    return n > 0 ? n : 0;
+}
+// An item's key tiles are shared out among `used` CTAs, `per` tiles each.  Both follow from the item and a.splits, of which a larger
+// one than `used` changes nothing: the same bits from a slab of any length.
+struct Share {
+    int used, per;
+};
+__device__ __forceinline__ Share find_share(const Args& a, int lq, int keys, int i0) {
+    if (a.splits == 1) return {1, 0};
+    const int last = i0 + 2 * a.tpg < lq ? i0 + 2 * a.tpg - 1 : lq - 1;
+    const int total = (reach(a, lq, keys, last) + BN - 1) / BN, each = (total + a.splits - 1) / a.splits;
+    if (total <= kAlone) return {1, 0};
+    const int per = each > kShare ? each : kShare;
+    return {(total + per - 1) / per, per};
+}
+// Item i: two tiles' tokens (from ct * 2 * tpg on) of one sequence and KV head.  The items of all sequences stand in a row by
+// falling ct, the longest work (of causal attention) first, with no gaps for sequences that are shorter than others.
+// Every warp finds its item for itself: F(c), the number of items with ct >= c of one head, falls in c.
+__device__ __forceinline__ bool find_item(const Args& a, int i, Seq& q, int& s, int& ct, int& kvh) {
+    const int lane = threadIdx.x & 31;
+    kvh = i % a.nkv;
+    i /= a.nkv;
+    auto items = [&](int lq) {
+        const int n = (lq + 2 * a.tpg - 1) / (2 * a.tpg);
+        return n < a.n_ct ? n : a.n_ct;
+    };
+    if (a.S == 1) {             // (0.7 us less, of 5)
+        s = 0;
+        q = sequence(a, 0);
+        ct = items(q.lq) - 1 - i;
+        return ct >= 0;
+    }
+    const Seq mine = sequence(a, lane);
+    const int my_items = items(mine.lq);
+    auto from = [&](int c) {
+        int sum = __reduce_add_sync(0xffffffffu, my_items > c ? my_items - c : 0);
+        for (int b = 32; b < a.S; b += 32) {
+            const int n = items(sequence(a, b + lane).lq);
+            sum += __reduce_add_sync(0xffffffffu, n > c ? n - c : 0);
+        }
+        return sum;
+    };
+    if (from(0) <= i) return false;
+    int lo = 0, hi = a.n_ct, before = 0;        // F(lo) > i >= F(hi) = before
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1, n = from(mid);
+        if (n > i) lo = mid; else { hi = mid; before = n; }
+    }
+    ct = lo;
+    i -= before;                                // the i-th of the sequences that are long enough
+    for (int b = 0; b < a.S; b += 32) {
+        const Seq here = b == 0 ? mine : sequence(a, b + lane);
+        uint32_t has = __ballot_sync(0xffffffffu, items(here.lq) > lo);
+        const int n = __popc(has);
+        if (i < n) {
+            for (; i > 0; --i) has &= has - 1;
+            const int at = __ffs(has) - 1;
+            s = b + at;
+            q.q0 = __shfl_sync(0xffffffffu, here.q0, at);
+            q.lq = __shfl_sync(0xffffffffu, here.lq, at);
+            q.k0 = __shfl_sync(0xffffffffu, here.k0, at);
+            q.lk = __shfl_sync(0xffffffffu, here.lk, at);
+            return true;
+        }
+        i -= n;
+    }
+    return false;
+}
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
     asm volatile(
@@ -125,6 +222,14 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
 // The wait for loads from tensor memory, through which their registers pass: nothing that uses them can be moved in front of it.
 __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
+}
+// ... and a second load's registers, behind the same wait
+__device__ __forceinline__ void tmem_ld_tie(uint32_t (&r)[32]) {
+    asm volatile(""
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
                    "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
                    "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
@@ -247,34 +352,24 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 4);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* odd_v = abort_flag + 1;       // a V tile held an infinity or a NaN that some row does not see
-    static_assert((4 * kMaxStages + 13) * 8 + 12 <= kBarBytes, "barrier area");
+    volatile int* later = odd_v + 1;            // what only the end needs: out of the softmax's registers
+    static_assert((4 * kMaxStages + 13) * 8 + 12 + 7 * 4 <= kBarBytes, "barrier area");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    // ---- what this CTA is for (every thread works it out): longest work first
-    const int hs = blockIdx.x % (a.nkv * a.S), ct = a.n_ct - 1 - blockIdx.x / (a.nkv * a.S);
-    const int kvh = hs % a.nkv, s = hs / a.nkv;
-    int q0 = a.cu_q[s], q1 = a.cu_q[s + 1];
-    q0 = q0 < 0 ? 0 : q0;
-    q1 = q1 > a.Tq ? a.Tq : q1;
-    const int lq = q1 - q0, i0 = ct * 2 * a.tpg;
-    if (i0 >= lq) return;
-    int k0 = 0, lk;
-    if (a.cu_k != nullptr) {
-        int k1 = a.cu_k[s + 1];
-        k0 = a.cu_k[s];
-        k0 = k0 < 0 ? 0 : k0;
-        k1 = k1 > a.Tk ? a.Tk : k1;
-        lk = k1 > k0 ? k1 - k0 : 0;
-    } else {
-        const int64_t n = a.k_len[s];
-        lk = n < 0 ? 0 : (n > a.Tk ? a.Tk : (int)n);
-    }
-    auto count = [&](int i) {           // keys that token i sees
-        if (!a.causal || i >= lq) return lk;
-        const int n = lk - lq + i + 1;
-        return n > 0 ? n : 0;
+    const int item = a.splits == 1 ? blockIdx.x : blockIdx.x / a.splits, share = blockIdx.x - item * a.splits;
+    Seq seq;
+    int s, ct, kvh;
+    if (!find_item(a, item, seq, s, ct, kvh)) return;
+    const int q0 = seq.q0, lq = seq.lq, all_keys = seq.lk, i0 = ct * 2 * a.tpg;
+    const Share sh = find_share(a, lq, all_keys, i0);
+    if (share >= sh.used) return;
+    const int skip = share * sh.per * BN, lk = all_keys - skip;        // keys before this CTA's first, and from it on
+    const int k0 = seq.k0 + skip;
+    auto count = [&](int i) {           // of this CTA's keys, those that token i sees
+        const int n = reach(a, lq, all_keys, i) - skip;
+        return n < 0 ? 0 : (sh.used > 1 && n > sh.per * BN ? sh.per * BN : n);
     };
     auto steps = [&](int x) {           // key tiles of Q tile x
         const int first = i0 + x * a.tpg;
@@ -301,6 +396,13 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         for (int i = 0; i < 4; ++i) sm100::mbar_init(&o_done[i], 1);
         *abort_flag = 0;
         *odd_v = 0;
+        later[0] = q0 + i0;
+        later[1] = lq - i0;
+        later[2] = kvh;
+        later[3] = k0;
+        later[4] = seen_by_all;
+        later[5] = sh.used;
+        later[6] = s;
         sm100::fence_barrier_init();
         sm100::prefetch_tensormap(&map_q);
         sm100::prefetch_tensormap(&map_k);
@@ -478,8 +580,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         const int x = warp >> 2, row = 32 * (warp & 3) + lane;
         const int nx = x ? n1 : n0;
-        const int tok = i0 + x * a.tpg + row / a.G;
-        const int cnt = count(tok);
+        const int cnt = count(i0 + x * a.tpg + row / a.G);
         const int seen = nx > 0 ? count(i0 + x * a.tpg) : 0;        // keys that every row of the tile sees
         const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t to = t_lane + 256u + 128u * x;
@@ -496,8 +597,8 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             uint32_t r[BN];
 #pragma unroll
             for (int c = 0; c < BN; c += 32) sm100::tmem_ld_32x32(ts + c, reinterpret_cast<uint32_t(&)[32]>(r[c]));
-#pragma unroll
-            for (int c = 0; c < BN; c += 32) tmem_ld_wait(reinterpret_cast<uint32_t(&)[32]>(r[c]));
+            tmem_ld_wait(reinterpret_cast<uint32_t(&)[32]>(r[0]));
+            tmem_ld_tie(reinterpret_cast<uint32_t(&)[32]>(r[32]));
             if ((j + 1) * BN > seen) {
                 const int lim = cnt - j * BN;
 #pragma unroll
@@ -580,10 +681,16 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (ok && nx > 0) ok = __all_sync(0xffffffffu, bar_wait(&o_done[2 * x + 1], 0, abort_flag));
         if (ok) {
             sm100::tc_fence_after_sync();
-            const bool live = row < rows && tok < lq;
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            __nv_bfloat16* dst = a.out + (int64_t)(q0 + tok) * a.o_tok + (int64_t)(kvh * a.G + row % a.G) * a.o_head;
+            const int at = x * a.tpg + row / a.G, head = later[2], shared = later[5] > 1;      // at: token of this CTA
+            const bool live = row < a.G * a.tpg && at < later[1];
+            const float inv = shared ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+            __nv_bfloat16* dst = a.out + (int64_t)(later[0] + at) * a.o_tok + (int64_t)(head * a.G + row % a.G) * a.o_head;
+            float* part = shared ? a.part + (int64_t)blockIdx.x * (DP + 2) * 2 * BM + x * BM + row : nullptr;
             const bool odd = nx > 0 && *odd_v != 0;
+            if (part != nullptr && live) {
+                part[0] = ref;
+                part[2 * BM] = l;
+            }
 #pragma unroll 1
             for (int d = 0; d < DP; d += 32) {
                 uint32_t r[32];
@@ -596,22 +703,27 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 }
                 if (live) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) r[e] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(r[e]) * inv);
+                    for (int e = 0; e < 32; ++e) r[e] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(r[e]) * inv);
                     if (odd) {      // infinities and NaNs that were taken out of V, back to the rows that see them
-                        const __nv_bfloat16* vp = a.v + (a.cu_k != nullptr ? 0 : (int64_t)s * a.v_seq) + (int64_t)kvh * a.v_head + (int64_t)k0 * a.v_row;
-                        for (int kk = seen_by_all; kk < cnt; ++kk)
+                        const __nv_bfloat16* vp = a.v + (a.cu_k != nullptr ? 0 : (int64_t)later[6] * a.v_seq) + (int64_t)head * a.v_head + (int64_t)later[3] * a.v_row;
+                        for (int kk = later[4]; kk < cnt; ++kk)
 #pragma unroll
                             for (int e = 0; e < 32; ++e) {
                                 const float y = d + e < a.D ? __bfloat162float(vp[(int64_t)kk * a.v_row + d + e]) : 0.f;
                                 if (!(fabsf(y) <= 3.4e38f)) r[e] = __float_as_uint(__uint_as_float(r[e]) + y);
                             }
                     }
-                    uint32_t h[16];
+                    if (part != nullptr) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) h[e] = bf2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
+                        for (int e = 0; e < 32; ++e) part[(2 + d + e) * 2 * BM] = __uint_as_float(r[e]);
+                    } else {
+                        uint32_t h[16];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (d + 8 * e < a.D) *reinterpret_cast<uint4*>(dst + d + 8 * e) = make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
+                        for (int e = 0; e < 16; ++e) h[e] = bf2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (d + 8 * e < a.D) *reinterpret_cast<uint4*>(dst + d + 8 * e) = make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
+                    }
                 }
             }
         }
@@ -630,10 +742,91 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     if (threadIdx.x == 0 && *abort_flag != 0 && a.status != nullptr) atomicExch(a.status, HXQ_E_TIMEOUT);
 }
 
+// The shares' results of one row: out = sum_p 2^((m_p - M) sc) o_p / sum_p 2^((m_p - M) sc) l_p.  A CTA has 32 rows of a
+// tile, a lane each (in memory the rows are innermost), and kJoin dimensions; its warps take every eighth share and meet in
+// shared memory.
+constexpr int kJoin = 16;
+template <int DP>
+__global__ void __launch_bounds__(256) join_kernel(const Args a) {
+    __shared__ float meet[8][2 + kJoin][32];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int d = blockIdx.x % (DP / kJoin) * kJoin, group = blockIdx.x / (DP / kJoin) % a.groups, item = blockIdx.x / (DP / kJoin) / a.groups;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    Seq seq;
+    int s, ct, kvh;
+    if (!find_item(a, item, seq, s, ct, kvh)) return;
+    const int used = find_share(a, seq.lq, seq.lk, ct * 2 * a.tpg).used;
+    if (used == 1) return;              // written already
+    const int x = group >> 2, first = (2 * ct + x) * a.tpg, left = seq.lq - first, rows = a.G * (left < a.tpg ? left : a.tpg);
+    const int in = (group & 3) * 32 + lane;
+    float m = -INFINITY, l = 0.f, o[kJoin] = {};
+    if (in < rows) {
+        const float* part = a.part + (int64_t)item * a.splits * (DP + 2) * 2 * BM + x * BM + in;
+#pragma unroll 2
+        for (int p = warp; p < used; p += 8) {
+            const float* q = part + (int64_t)p * (DP + 2) * 2 * BM;
+            float v[kJoin];
+            const float ref = q[0], sum = q[2 * BM];
+#pragma unroll
+            for (int e = 0; e < kJoin; ++e) v[e] = q[(2 + d + e) * 2 * BM];
+            const float top = fmaxf(m, ref), c = m == -INFINITY ? 0.f : ex2((m - top) * a.scale_log2), w = ref == -INFINITY ? 0.f : ex2((ref - top) * a.scale_log2);
+            m = top;
+            l = c * l + w * sum;        // (NaN, a row's that sees one, stays one whatever the weights)
+#pragma unroll
+            for (int e = 0; e < kJoin; ++e) o[e] = c * o[e] + w * v[e];
+        }
+    }
+    meet[warp][0][lane] = m;
+    meet[warp][1][lane] = l;
+#pragma unroll
+    for (int e = 0; e < kJoin; ++e) meet[warp][2 + e][lane] = o[e];
+    __syncthreads();
+    if (in >= rows || d + 2 * warp >= a.D) return;        // a warp, two dimensions
+    float top = -INFINITY;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) top = fmaxf(top, meet[p][0][lane]);
+    float sum = 0.f, y0 = 0.f, y1 = 0.f;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+        const float w = meet[p][0][lane] == -INFINITY ? 0.f : ex2((meet[p][0][lane] - top) * a.scale_log2);
+        sum += w * meet[p][1][lane];
+        y0 += w * meet[p][2 + 2 * warp][lane];
+        y1 += w * meet[p][3 + 2 * warp][lane];
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    __nv_bfloat16* dst = a.out + (int64_t)(seq.q0 + first + in / a.G) * a.o_tok + (int64_t)(kvh * a.G + in % a.G) * a.o_head + d + 2 * warp;
+    *reinterpret_cast<uint32_t*>(dst) = sum == 0.f ? 0u : bf2(y0 * inv, y1 * inv);
+}
+
 // ---- host side ---------------------------------------------------------------------
 
+struct Plan {
+    int tpg, n_ct, items, splits, groups;
+};
+// Items: the tokens' tiles, one more for each sequence's last.  Few of them before many keys leave SMs idle: then their key tiles are
+// shared out, to as many CTAs as there are SMs for (16 tokens behind 32768 keys, 28 query and 4 KV heads: 4 items of 512 tiles).
+// max_q has no say in it: it would in the result's last bits.
+static bool make_plan(const hxq_attn* p, Plan& plan) {
+    plan.tpg = BM / (p->nq / p->nkv);
+    const int64_t max_q = p->max_q < p->Tq ? p->max_q : p->Tq, rows = 2 * plan.tpg;
+    plan.n_ct = (int)((max_q + rows - 1) / rows);
+    const int64_t all = (int64_t)p->Tq / rows + p->S, most = (int64_t)plan.n_ct * p->S;
+    const int64_t n = (all < most ? all : most) * p->nkv;
+    const int64_t keys = p->cu_k == p->cu_q && max_q < p->Tk ? max_q : p->Tk;        // of one sequence, at most
+    const int64_t steps = (keys + BN - 1) / BN, parts = steps <= kAlone ? 1 : (steps + kShare - 1) / kShare, room = 148 / (all * p->nkv);
+    const int64_t splits = parts < room ? parts : room;
+    plan.items = (int)n;
+    plan.groups = max_q > plan.tpg ? 8 : (int)((max_q * (p->nq / p->nkv) + 31) / 32);
+    plan.splits = splits > 1 ? (int)splits : 1;
+    return n <= 0x7fffffffLL / 64;
+}
+static size_t part_bytes(const hxq_attn* p, const Plan& plan) {
+    return plan.splits == 1 ? 0 : (size_t)plan.items * plan.splits * 2 * BM * ((p->D <= 64 ? 64 : 128) + 2) * sizeof(float);
+}
+
 template <int DP>
-static int run(const hxq_attn* p, int32_t* status, cudaStream_t stream) {
+static int run(const hxq_attn* p, const Plan& plan, void* workspace, int32_t* status, cudaStream_t stream) {
     using Z = Sizes<DP>;
     Args a;
     a.cu_q = p->cu_q; a.cu_k = p->cu_k; a.k_len = p->k_len;
@@ -642,12 +835,12 @@ static int run(const hxq_attn* p, int32_t* status, cudaStream_t stream) {
     a.status = status;
     a.v_seq = p->v_seq; a.v_head = p->v_head; a.v_row = p->v_row; a.o_tok = p->o_tok; a.o_head = p->o_head;
     a.Tq = p->Tq; a.Tk = p->Tk; a.S = p->S; a.nkv = p->nkv; a.G = p->nq / p->nkv; a.D = p->D; a.causal = p->causal != 0;
-    a.tpg = BM / a.G;
+    a.tpg = plan.tpg;
+    a.n_ct = plan.n_ct;
+    a.splits = plan.splits;
+    a.groups = plan.groups;
+    a.part = reinterpret_cast<float*>(workspace);
     a.scale_log2 = p->scale * 1.4426950408889634f;
-    const int64_t max_q = p->max_q < p->Tq ? p->max_q : p->Tq;
-    a.n_ct = (int)((max_q + 2 * a.tpg - 1) / (2 * a.tpg));
-    const int64_t grid = (int64_t)a.n_ct * a.nkv * a.S;
-    if (grid > 0x7fffffffLL) return HXQ_E_SHAPE;
 
     CUtensorMap mq, mk, mv;
     // (the stride of a dimension of one element is never used, but has to be a valid one)
@@ -674,7 +867,7 @@ static int run(const hxq_attn* p, int32_t* status, cudaStream_t stream) {
         attr_set[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid);
+    cfg.gridDim = dim3((unsigned)(plan.items * plan.splits));
     cfg.blockDim = dim3(NUM_THREADS);
     cfg.dynamicSmemBytes = Z::kSmem;
     cfg.stream = stream;
@@ -683,13 +876,20 @@ static int run(const hxq_attn* p, int32_t* status, cudaStream_t stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attn_prompt_kernel<DP>, mq, mk, mv, a) == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, attn_prompt_kernel<DP>, mq, mk, mv, a);
+    if (e == cudaSuccess && plan.splits > 1) {
+        cfg.gridDim = dim3((unsigned)(plan.items * plan.groups * (DP / kJoin)));
+        cfg.blockDim = dim3(256);
+        cfg.dynamicSmemBytes = 0;
+        e = cudaLaunchKernelEx(&cfg, join_kernel<DP>, a);
+    }
+    return e == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
 }
 
 }  // namespace attnp
 }  // namespace hxq
 
-extern "C" int hxq_attn_prompt(const hxq_attn* p, int32_t* status_word, hxq_stream_t stream) {
+static int check(const hxq_attn* p) {
     if (!p || !p->q || !p->k || !p->v || !p->out || !p->cu_q || (!p->cu_k) == (!p->k_len)) return HXQ_E_ARG;
     if (p->Tq < 0 || p->Tk < 0 || p->S <= 0 || p->max_q < 0 || !(p->scale > 0.f) || !(p->scale <= 3.4e38f)) return HXQ_E_ARG;
     if (p->nq <= 0 || p->nkv <= 0 || p->nq % p->nkv != 0 || p->nq / p->nkv > 64) return HXQ_E_SHAPE;
@@ -698,7 +898,22 @@ extern "C" int hxq_attn_prompt(const hxq_attn* p, int32_t* status_word, hxq_stre
     for (int64_t s : strides)
         if (s < 0 || s >= (int64_t(1) << 38) || s % 8 != 0) return HXQ_E_ALIGN;
     if (!hxq::aligned_to(p->q, 16) || !hxq::aligned_to(p->k, 16) || !hxq::aligned_to(p->v, 16) || !hxq::aligned_to(p->out, 16)) return HXQ_E_ALIGN;
-    if (p->Tq == 0 || p->max_q == 0) return HXQ_OK;
+    return HXQ_OK;
+}
+
+extern "C" size_t hxq_attn_prompt_workspace_bytes(const hxq_attn* p) {
+    hxq::attnp::Plan plan;
+    return check(p) == HXQ_OK && hxq::attnp::make_plan(p, plan) ? hxq::attnp::part_bytes(p, plan) : 0;
+}
+
+extern "C" int hxq_attn_prompt(const hxq_attn* p, void* workspace, size_t workspace_bytes, int32_t* status_word, hxq_stream_t stream) {
+    const int bad = check(p);
+    if (bad != HXQ_OK) return bad;
+    hxq::attnp::Plan plan;
+    if (!hxq::attnp::make_plan(p, plan)) return HXQ_E_SHAPE;
+    if (plan.items == 0) return HXQ_OK;
+    const size_t need = hxq::attnp::part_bytes(p, plan);
+    if (need > 0 && (!workspace || !hxq::aligned_to(workspace, 8) || workspace_bytes < need)) return HXQ_E_WORKSPACE;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    return p->D <= 64 ? hxq::attnp::run<64>(p, status_word, st) : hxq::attnp::run<128>(p, status_word, st);
+    return p->D <= 64 ? hxq::attnp::run<64>(p, plan, workspace, status_word, st) : hxq::attnp::run<128>(p, plan, workspace, status_word, st);
 }

@@ -63,5 +63,7 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Te
     p = _lib.HxqAttn(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), *k3, *v3, out.stride(0),
                      out.stride(1), cu_q.data_ptr(), None if slabs else cu_k.data_ptr(), k_len.data_ptr() if slabs else None,
                      T, rows, S, min(max_q, T), nq, nkv, D, int(causal), scale)
-    _call(dev, "hxq_attn_prompt", C.byref(p), _status_word(dev).data_ptr())
+    nb = _lib.lib().hxq_attn_prompt_workspace_bytes(C.byref(p))
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None       # for this call alone: captured graphs do not share it
+    _call(dev, "hxq_attn_prompt", C.byref(p), None if ws is None else ws.data_ptr(), nb, _status_word(dev).data_ptr())
     return out

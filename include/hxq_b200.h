@@ -245,7 +245,8 @@ int32_t hxq_attn_decode_span(int32_t B, int32_t nkv, int32_t max_len);
  * cu_q, cu_k (int32 [S + 1], ascending) and k_len (int64 [S]) are DEVICE arrays, exactly one of cu_k and k_len given;
  * max_q: no sequence has more queries (those past it are not computed).  Rows of out that belong to no sequence are
  * left as they are.  Strides in elements, multiples of 8; pointers 16-byte aligned; D % 8 == 0, 8 <= D <= 128;
- * nq / nkv <= 64; scale > 0.  status_word as in hxq_gemm.
+ * nq / nkv <= 64; scale > 0.  status_word as in hxq_gemm.  Few queries before many keys split the keys among
+ * thread blocks: workspace is hxq_attn_prompt_workspace_bytes() of plain scratch (0: none needed).
  */
 typedef struct hxq_attn {
     const void *q, *k, *v;
@@ -260,7 +261,8 @@ typedef struct hxq_attn {
     int32_t Tq, Tk, S, max_q, nq, nkv, D, causal;
     float scale;
 } hxq_attn;
-int hxq_attn_prompt(const hxq_attn* p, int32_t* status_word, hxq_stream_t stream);
+size_t hxq_attn_prompt_workspace_bytes(const hxq_attn* p);
+int hxq_attn_prompt(const hxq_attn* p, void* workspace, size_t workspace_bytes, int32_t* status_word, hxq_stream_t stream);
 
 /*
  * ---- key/value cache held in 8 bits (no counterpart in the reference, which keeps the framework's

@@ -226,3 +226,67 @@ def test_prompt_refuses():
         with pytest.raises(kind):
             call()
     assert attn_prompt(q[:0], k[:0], v[:0], out[:0], torch.zeros(2, dtype=torch.int32, device=dev), 0, 0.1).shape[0] == 0
+
+
+@pytest.mark.parametrize("nq,nkv,D", [(28, 4, 128), (4, 2, 64), (9, 3, 72), (64, 1, 128)])
+@pytest.mark.parametrize("lens,keys", [([1], [5000]), ([16], [513]), ([7], [512]), ([130], [1025]), ([3, 40], [4097, 90]), ([2, 1, 1], [1600, 0, 7]), ([700], [1300])])
+def test_few_queries_before_many_keys(nq, nkv, D, lens, keys):
+    """Where the keys are shared out among thread blocks; a longer slab, or a larger max_q, changes no bit."""
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, T, S, rows = _dev(), sum(lens), len(lens), max(keys) + 9
+    g = torch.Generator(device=dev).manual_seed(T + D)
+    q = torch.randn(T, nq, D, device=dev, generator=g).bfloat16()
+    kc = torch.randn(S, nkv, rows, D, device=dev, generator=g).bfloat16()
+    vc = torch.randn(S, nkv, rows, D, device=dev, generator=g).bfloat16()
+    for s, n in enumerate(keys):
+        kc[s, :, n:], vc[s, :, n:] = float("nan"), float("inf")
+    longer = [torch.cat([c, torch.full((S, nkv, 20000, D), float("nan"), device=dev, dtype=torch.bfloat16)], 2) for c in (kc, vc)]
+    cu = [sum(lens[:s]) for s in range(S + 1)]
+    cu_d, len_d = torch.tensor(cu, dtype=torch.int32, device=dev), torch.tensor(keys, device=dev)
+    for causal in (True, False):
+        out, again = (torch.empty(T, nq, D, device=dev, dtype=torch.bfloat16) for _ in range(2))
+        attn_prompt(q, kc, vc, out, cu_d, max(lens), 0.2, k_len=len_d, causal=causal)
+        attn_prompt(q, *longer, again, cu_d, max(lens) + 300, 0.2, k_len=len_d, causal=causal)
+        assert torch.equal(out, again)
+        for s, (a, b) in enumerate(zip(cu, cu[1:])):
+            n = keys[s]
+            _compare(out[a:b], _want(q[a:b], kc[s, :, :n].transpose(0, 1), vc[s, :, :n].transpose(0, 1), 0.2, causal), (causal, s))
+
+
+@pytest.mark.parametrize("at", [0, 700, 2990, 2999])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_bad_values_in_a_share_of_the_keys(at, bad):
+    """Ten queries behind 2990 keys, the keys in shares: a bad value of V reaches its dimension, one of K the whole row."""
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, nq, nkv, D, T, n = _dev(), 14, 2, 128, 10, 3000
+    g = torch.Generator(device=dev).manual_seed(at)
+    q = torch.randn(T, nq, D, device=dev, generator=g).bfloat16()
+    kc, vc = (torch.randn(1, nkv, n, D, device=dev, generator=g).bfloat16() for _ in range(2))
+    vc[0, 1, at, 5] = bad
+    cu, k_len = torch.tensor([0, T], dtype=torch.int32, device=dev), torch.tensor([n], device=dev)
+    out = torch.empty(T, nq, D, device=dev, dtype=torch.bfloat16)
+    attn_prompt(q, kc, vc, out, cu, T, D ** -0.5, k_len=k_len)
+    _compare(out, _want(q, kc[0].transpose(0, 1), vc[0].transpose(0, 1), D ** -0.5, True), at)
+    vc.nan_to_num_(0.0, 0.0, 0.0)
+    kc[0, 0, at, 2] = float("nan")
+    attn_prompt(q, kc, vc, out, cu, T, D ** -0.5, k_len=k_len)
+    _compare(out, _want(q, kc[0].transpose(0, 1), vc[0].transpose(0, 1), D ** -0.5, True), at)
+
+
+@pytest.mark.parametrize("nq,nkv,D,lens", [(28, 4, 128, [900, 37, 1, 300]), (4, 2, 64, [2000])])
+def test_the_same_bits_every_time(nq, nkv, D, lens):
+    """Rows whose maxima keep growing, so that outputs are rescaled up to the last step: sixty calls at different moments."""
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, T = _dev(), sum(lens)
+    g = torch.Generator(device=dev).manual_seed(T)
+    q, k, v = (torch.randn(T, n, D, device=dev, generator=g).bfloat16() for n in (nq, nkv, nkv))
+    q = q.abs()
+    k *= torch.linspace(0.0, 40.0, T, device=dev)[:, None, None].bfloat16()
+    k.abs_()
+    cu = torch.tensor([sum(lens[:s]) for s in range(len(lens) + 1)], dtype=torch.int32, device=dev)
+    outs = [torch.empty(T, nq, D, device=dev, dtype=torch.bfloat16) for _ in range(60)]
+    for o in outs:
+        attn_prompt(q, k, v, o, cu, max(lens), D ** -0.5)
+    assert all(torch.equal(outs[0], o) for o in outs)
+    a, b = int(cu[0]), int(cu[1])
+    _compare(outs[0][a:b], _want(q[a:b], k[a:b], v[a:b], D ** -0.5, True), "the first")
