@@ -123,7 +123,7 @@ __device__ __forceinline__ Share find_share(const Args& a, int lq, int keys, int
 }
 // Item i: two tiles' tokens (from ct * 2 * tpg on) of one sequence and KV head.  The items of all sequences stand in a row by
 // falling ct, the longest work (of causal attention) first, with no gaps for sequences that are shorter than others.
-// Every warp finds its item for itself: F(c), the number of items with ct >= c of one head, falls in c.
+// A warp finds the item: F(c), the number of items with ct >= c of one head, falls in c.
 __device__ __forceinline__ bool find_item(const Args& a, int i, Seq& q, int& s, int& ct, int& kvh) {
     const int lane = threadIdx.x & 31;
     kvh = i % a.nkv;
@@ -138,15 +138,19 @@ __device__ __forceinline__ bool find_item(const Args& a, int i, Seq& q, int& s, 
         ct = items(q.lq) - 1 - i;
         return ct >= 0;
     }
-    const Seq mine = sequence(a, lane);
-    const int my_items = items(mine.lq);
+    constexpr int HELD = 4;     // sequences a lane keeps (their loads run together); more are read again
+    int held[HELD];
+#pragma unroll
+    for (int b = 0; b < HELD; ++b) held[b] = 32 * b < a.S ? items(sequence(a, 32 * b + lane).lq) : 0;
     auto from = [&](int c) {
-        int sum = __reduce_add_sync(0xffffffffu, my_items > c ? my_items - c : 0);
-        for (int b = 32; b < a.S; b += 32) {
+        int sum = 0;
+#pragma unroll
+        for (int b = 0; b < HELD; ++b) sum += held[b] > c ? held[b] - c : 0;
+        for (int b = 32 * HELD; b < a.S; b += 32) {
             const int n = items(sequence(a, b + lane).lq);
-            sum += __reduce_add_sync(0xffffffffu, n > c ? n - c : 0);
+            sum += n > c ? n - c : 0;
         }
-        return sum;
+        return __reduce_add_sync(0xffffffffu, sum);
     };
     if (from(0) <= i) return false;
     int lo = 0, hi = a.n_ct, before = 0;        // F(lo) > i >= F(hi) = before
@@ -157,7 +161,7 @@ __device__ __forceinline__ bool find_item(const Args& a, int i, Seq& q, int& s, 
     ct = lo;
     i -= before;                                // the i-th of the sequences that are long enough
     for (int b = 0; b < a.S; b += 32) {
-        const Seq here = b == 0 ? mine : sequence(a, b + lane);
+        const Seq here = sequence(a, b + lane);
         uint32_t has = __ballot_sync(0xffffffffu, items(here.lq) > lo);
         const int n = __popc(has);
         if (i < n) {
@@ -352,21 +356,83 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_done + 4);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile int* odd_v = abort_flag + 1;       // a V tile held an infinity or a NaN that some row does not see
-    volatile int* later = odd_v + 1;            // what only the end needs: out of the softmax's registers
-    static_assert((4 * kMaxStages + 13) * 8 + 12 + 7 * 4 <= kBarBytes, "barrier area");
+    volatile int* job = odd_v + 1;              // [8] this CTA's sequence, first token and head
+    static_assert((4 * kMaxStages + 13) * 8 + 12 + 8 * 4 <= kBarBytes, "barrier area");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-
+    const int rows = a.G * a.tpg;               // of a tile; the rest is zero
     const int item = a.splits == 1 ? blockIdx.x : blockIdx.x / a.splits, share = blockIdx.x - item * a.splits;
-    Seq seq;
-    int s, ct, kvh;
-    if (!find_item(a, item, seq, s, ct, kvh)) return;
-    const int q0 = seq.q0, lq = seq.lq, all_keys = seq.lk, i0 = ct * 2 * a.tpg;
+    // The warp that loads looks for what this CTA is for, and loads the first tiles, while others set up.
+    if (warp == SM_WARPS) {
+        constexpr int BARS = 4 * kMaxStages + 13, CLEAN = 3 * kMaxStages, P_READY = 4 * kMaxStages + 5;
+        for (int i = lane; i < BARS; i += 32)
+            sm100::mbar_init(full + i, i >= CLEAN && i < CLEAN + kMaxStages ? 2 : (i >= P_READY && i < P_READY + 4 ? SM_WARPS / 2 : 1));
+        if (lane == 0) {
+            *abort_flag = 0;
+            *odd_v = 0;
+            sm100::prefetch_tensormap(&map_q);
+            sm100::prefetch_tensormap(&map_k);
+            sm100::prefetch_tensormap(&map_v);
+        }
+        sm100::fence_barrier_init();
+        __syncwarp();
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (warp == SM_WARPS) {
+        Seq seq;
+        int s, ct, kvh;
+        bool found = find_item(a, item, seq, s, ct, kvh);
+        if (found && lane == 0) {
+            const Share sh = find_share(a, seq.lq, seq.lk, ct * 2 * a.tpg);
+            found = share < sh.used;
+            const int i0 = ct * 2 * a.tpg, last = i0 + 2 * a.tpg < seq.lq ? i0 + 2 * a.tpg - 1 : seq.lq - 1, skip = share * sh.per * BN;
+            int n = reach(a, seq.lq, seq.lk, last) - skip;
+            if (sh.used > 1 && n > sh.per * BN) n = sh.per * BN;
+            if (found && n > 0) {
+                sm100::mbar_arrive_expect_tx(&full[0], n > BN ? 2 * TILE : TILE);
+                for (int t = 0; t < (n > BN ? 2 : 1); ++t)
+                    for (int h = 0; h < DP / 64; ++h)
+                        tma_load_4d(sm100::smem_u32(ring + t * TILE + h * HALF), &map_k, &full[0], 64 * h, seq.k0 + skip + t * BN, kvh, a.cu_k != nullptr ? 0 : s);
+                sm100::mbar_arrive_expect_tx(q_full, 2u * (DP / 64) * (uint32_t)rows * 128u);
+                for (int x = 0; x < 2; ++x)
+                    for (int h = 0; h < DP / 64; ++h)
+                        tma_load_3d(sm100::smem_u32(smem + x * QT + h * QHALF), &map_q, q_full, 64 * h, kvh * a.G, seq.q0 + i0 + x * a.tpg);
+            }
+        }
+        if (lane == 0) {
+            job[0] = found;
+            job[1] = seq.q0;
+            job[2] = seq.lq;
+            job[3] = seq.k0;
+            job[4] = seq.lk;
+            job[5] = s;
+            job[6] = ct * 2 * a.tpg;
+            job[7] = kvh;
+        }
+    } else if (warp == SM_WARPS + 1) {
+        sm100::tmem_alloc(tmem_slot, 512);
+        sm100::tmem_relinquish();
+    } else {        // rows of the Q tiles that no token fills
+        const int idle = (BM - rows) * 8, i0 = threadIdx.x - (warp > SM_WARPS ? 64 : 0);
+        for (int part = 0; part < 2 * (DP / 64); ++part)
+            for (int i = i0; i < idle; i += NUM_THREADS - 64)
+                *reinterpret_cast<uint4*>(smem + part * QHALF + (rows + (i >> 3)) * 128 + (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    sm100::fence_proxy_async_smem();
+    sm100::tc_fence_before_sync();
+    __syncthreads();
+    sm100::tc_fence_after_sync();
+    // The next kernel may come in only now: one that took tensor memory before this CTA did would keep it waiting.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;       // S of tile 0: two buffers of 64 columns; of tile 1; O of either, 128 columns each
+    if (job[0] == 0) {
+        if (warp == SM_WARPS + 1) sm100::tmem_dealloc(tmem, 512);
+        return;
+    }
+    const int q0 = job[1], lq = job[2], all_keys = job[4], s = job[5], i0 = job[6], kvh = job[7];
     const Share sh = find_share(a, lq, all_keys, i0);
-    if (share >= sh.used) return;
     const int skip = share * sh.per * BN, lk = all_keys - skip;        // keys before this CTA's first, and from it on
-    const int k0 = seq.k0 + skip;
+    const int k0 = job[3] + skip;
     auto count = [&](int i) {           // of this CTA's keys, those that token i sees
         const int n = reach(a, lq, all_keys, i) - skip;
         return n < 0 ? 0 : (sh.used > 1 && n > sh.per * BN ? sh.per * BN : n);
@@ -379,75 +445,26 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     const int n0 = steps(0), n1 = steps(1), n = n0 > n1 ? n0 : n1;
     const int seen_by_all = count(i0);          // keys that every token of this CTA sees
     const int jc = seen_by_all / BN;            // V tiles from here on are looked at
-    const int rows = a.G * a.tpg;               // of a tile; the rest is zero
-
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < NS; ++i) {
-            sm100::mbar_init(&full[i], 1);
-            sm100::mbar_init(&empty[i], 1);
-            sm100::mbar_init(&raw[i], 1);
-            sm100::mbar_init(&clean[i], 2);
-        }
-        sm100::mbar_init(q_full, 1);
-        for (int i = 0; i < 4; ++i) {
-            sm100::mbar_init(&s_full[i], 1);
-            sm100::mbar_init(&p_ready[i], SM_WARPS / 2);
-        }
-        for (int i = 0; i < 4; ++i) sm100::mbar_init(&o_done[i], 1);
-        *abort_flag = 0;
-        *odd_v = 0;
-        later[0] = q0 + i0;
-        later[1] = lq - i0;
-        later[2] = kvh;
-        later[3] = k0;
-        later[4] = seen_by_all;
-        later[5] = sh.used;
-        later[6] = s;
-        sm100::fence_barrier_init();
-        sm100::prefetch_tensormap(&map_q);
-        sm100::prefetch_tensormap(&map_k);
-        sm100::prefetch_tensormap(&map_v);
-    }
-    if (warp == SM_WARPS + 1) {
-        sm100::tmem_alloc(tmem_slot, 512);
-        sm100::tmem_relinquish();
-    }
-    // rows of the Q tiles that no token fills
-    for (int i = threadIdx.x; i < 2 * (DP / 64) * (BM - rows) * 8; i += NUM_THREADS) {
-        const int part = i / ((BM - rows) * 8), rem = i - part * (BM - rows) * 8;
-        *reinterpret_cast<uint4*>(smem + part * QHALF + (rows + (rem >> 3)) * 128 + (rem & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-    }
-    sm100::fence_proxy_async_smem();
-    sm100::tc_fence_before_sync();
-    __syncthreads();
-    sm100::tc_fence_after_sync();
-    // The next kernel may come in only now: one that took tensor memory before this CTA did would keep it waiting.
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const uint32_t tmem = *tmem_slot;       // S of tile 0: two buffers of 64 columns; of tile 1; O of either, 128 columns each
     bool ok = true;
 
     static_assert(32 * SM_WARPS * kRegsSoftmax + 128 * kRegsOther <= NUM_THREADS * kRegsLaunch, "no more registers than the launch brings");
     if (warp >= SM_WARPS) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     if (warp == SM_WARPS) {
-        // ------------------------------------------------------------ loads, in the order of their use: K0 K1 | V0 K2 | V1 K3 | ...
+        // ------------------------------------------------------------ loads, in the order of their use: K0 K1 (above) | V0 K2 | V1 K3 | ...
         if (lane == 0 && n > 0) {
-            sm100::mbar_arrive_expect_tx(q_full, 2u * (DP / 64) * (uint32_t)rows * 128u);
-            for (int x = 0; x < 2; ++x)
-                for (int h = 0; h < DP / 64; ++h)
-                    tma_load_3d(sm100::smem_u32(smem + x * QT + h * QHALF), &map_q, q_full, 64 * h, kvh * a.G, q0 + i0 + x * a.tpg);
             const int slab = a.cu_k != nullptr ? 0 : s;
-            int slot = 0;
+            int slot = 1;
             uint32_t ph = 1;
-            for (int i = -1; i < n; ++i) {          // stage i + 1: V of step i (K of step 0 at the start) and K of step i + 2
+            for (int i = 0; i < n; ++i) {           // stage i + 1: V of step i and K of step i + 2
                 ok = bar_wait(&empty[slot], ph, abort_flag);
                 if (!ok) break;
-                const bool two = i < 0 ? n > 1 : i + 2 < n;
-                uint64_t* bar = i >= 0 && i >= jc ? &raw[slot] : &full[slot];
+                const bool two = i + 2 < n;
+                uint64_t* bar = i >= jc ? &raw[slot] : &full[slot];
                 sm100::mbar_arrive_expect_tx(bar, two ? 2 * TILE : TILE);
                 const uint32_t dst = sm100::smem_u32(ring + slot * 2 * TILE);
                 for (int h = 0; h < DP / 64; ++h)
-                    tma_load_4d(dst + h * HALF, i < 0 ? &map_k : &map_v, bar, 64 * h, k0 + (i < 0 ? 0 : i) * BN, kvh, slab);
+                    tma_load_4d(dst + h * HALF, &map_v, bar, 64 * h, k0 + i * BN, kvh, slab);
                 if (two)
                     for (int h = 0; h < DP / 64; ++h) tma_load_4d(dst + TILE + h * HALF, &map_k, bar, 64 * h, k0 + (i + 2) * BN, kvh, slab);
                 if (++slot == NS) { slot = 0; ph ^= 1u; }
@@ -551,23 +568,34 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             char* tile = ring + slot * 2 * TILE;
             const int from = seen_by_all - j * BN > 0 ? seen_by_all - j * BN : 0;         // rows before it are everybody's
             bool odd = false;
-            for (int i = (warp - SM_WARPS - 2) * 32 + lane; i < (DP / 64) * (BN - from) * 8; i += 64) {
-                const int part = i / ((BN - from) * 8), rem = i - part * (BN - from) * 8;
-                const int row = from + (rem >> 3);
-                uint4* p = reinterpret_cast<uint4*>(tile + part * HALF + row * 128 + (rem & 7) * 16);
-                if (j * BN + row >= lk) {
-                    *p = make_uint4(0u, 0u, 0u, 0u);
-                } else {
-                    uint4 w = *p;
-                    uint32_t* e = &w.x;
-                    bool hit = false;
+            // a lane's column of 16 bytes, in rows eight apart, four rows of both halves at a time
+            for (int row0 = from + (warp - SM_WARPS - 2) * 4 + (lane >> 3); row0 < BN; row0 += 32) {
+                uint4 w[4][DP / 64];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {        // exponent of all ones
-                        if ((e[c] & 0x7f80u) == 0x7f80u) { e[c] &= 0xffff0000u; hit = true; }
-                        if ((e[c] & 0x7f800000u) == 0x7f800000u) { e[c] &= 0xffffu; hit = true; }
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int h = 0; h < DP / 64; ++h)
+                        if (row0 + 8 * i < BN) w[i][h] = *reinterpret_cast<const uint4*>(tile + h * HALF + (row0 + 8 * i) * 128 + (lane & 7) * 16);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int h = 0; h < DP / 64; ++h) {
+                        const int row = row0 + 8 * i;
+                        if (row >= BN) continue;
+                        uint4* p = reinterpret_cast<uint4*>(tile + h * HALF + row * 128 + (lane & 7) * 16);
+                        if (j * BN + row >= lk) {
+                            *p = make_uint4(0u, 0u, 0u, 0u);
+                            continue;
+                        }
+                        uint32_t* e = &w[i][h].x;
+                        bool hit = false;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {        // exponent of all ones
+                            if ((e[c] & 0x7f80u) == 0x7f80u) { e[c] &= 0xffff0000u; hit = true; }
+                            if ((e[c] & 0x7f800000u) == 0x7f800000u) { e[c] &= 0xffffu; hit = true; }
+                        }
+                        if (hit) { *p = w[i][h]; odd = true; }
                     }
-                    if (hit) { *p = w; odd = true; }
-                }
             }
             if (odd) *odd_v = 1;
             sm100::fence_proxy_async_smem();
@@ -681,13 +709,14 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (ok && nx > 0) ok = __all_sync(0xffffffffu, bar_wait(&o_done[2 * x + 1], 0, abort_flag));
         if (ok) {
             sm100::tc_fence_after_sync();
-            const int at = x * a.tpg + row / a.G, head = later[2], shared = later[5] > 1;      // at: token of this CTA
-            const bool live = row < a.G * a.tpg && at < later[1];
-            const float inv = shared ? 1.f : (l == 0.f ? 0.f : 1.f / l);
-            __nv_bfloat16* dst = a.out + (int64_t)(later[0] + at) * a.o_tok + (int64_t)(head * a.G + row % a.G) * a.o_head;
-            float* part = shared ? a.part + (int64_t)blockIdx.x * (DP + 2) * 2 * BM + x * BM + row : nullptr;
+            const int tok = job[6] + x * a.tpg + row / a.G, head = job[7];
+            const bool live = row < a.G * a.tpg && tok < job[2], shared = a.splits > 1 && find_share(a, job[2], job[4], job[6]).used > 1;
+            const float inv = shared ? 1.f : 1.f / l;
             const bool odd = nx > 0 && *odd_v != 0;
-            if (part != nullptr && live) {
+            __nv_bfloat16* dst = a.out + (int64_t)(job[1] + tok) * a.o_tok + (int64_t)(head * a.G + row % a.G) * a.o_head;
+            float* part = a.part + (int64_t)blockIdx.x * (DP + 2) * 2 * BM + x * BM + row;
+            char* stage = smem + warp * (32 * DP * 2);      // 32 rows; Q has been read: the tile's last product has retired
+            if (shared && live) {
                 part[0] = ref;
                 part[2 * BM] = l;
             }
@@ -697,33 +726,49 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 if (nx > 0) {
                     sm100::tmem_ld_32x32(to + d, r);
                     tmem_ld_wait(r);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) r[e] = 0u;
                 }
-                if (live) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) r[e] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(r[e]) * inv);
-                    if (odd) {      // infinities and NaNs that were taken out of V, back to the rows that see them
-                        const __nv_bfloat16* vp = a.v + (a.cu_k != nullptr ? 0 : (int64_t)later[6] * a.v_seq) + (int64_t)head * a.v_head + (int64_t)later[3] * a.v_row;
-                        for (int kk = later[4]; kk < cnt; ++kk)
+                for (int e = 0; e < 32; ++e) r[e] = nx == 0 || l == 0.f ? 0u : __float_as_uint(__uint_as_float(r[e]) * inv);
+                if (odd && live) {      // infinities and NaNs that were taken out of V, back to the rows that see them
+                    const __nv_bfloat16* vp = a.v + (a.cu_k != nullptr ? 0 : (int64_t)job[5] * a.v_seq) + (int64_t)head * a.v_head + (int64_t)k0 * a.v_row;
+                    for (int kk = seen_by_all; kk < cnt; ++kk)
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                const float y = d + e < a.D ? __bfloat162float(vp[(int64_t)kk * a.v_row + d + e]) : 0.f;
-                                if (!(fabsf(y) <= 3.4e38f)) r[e] = __float_as_uint(__uint_as_float(r[e]) + y);
-                            }
-                    }
-                    if (part != nullptr) {
+                        for (int e = 0; e < 32; ++e) {
+                            const float y = d + e < a.D ? __bfloat162float(vp[(int64_t)kk * a.v_row + d + e]) : 0.f;
+                            if (!(fabsf(y) <= 3.4e38f)) r[e] = __float_as_uint(__uint_as_float(r[e]) + y);
+                        }
+                }
+                if (shared) {
+                    if (live) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e) part[(2 + d + e) * 2 * BM] = __uint_as_float(r[e]);
-                    } else {
-                        uint32_t h[16];
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) h[e] = bf2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
+                    }
+                } else if (nx == 0) {               // (Q may still be landing)
+                    if (live) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (d + 8 * e < a.D) *reinterpret_cast<uint4*>(dst + d + 8 * e) = make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]);
+                            if (d + 8 * e < a.D) *reinterpret_cast<uint4*>(dst + d + 8 * e) = make_uint4(0u, 0u, 0u, 0u);
                     }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        *reinterpret_cast<uint4*>(stage + lane * (DP * 2) + (((d >> 3) + e) ^ (lane & 7)) * 16) =
+                            make_uint4(bf2(__uint_as_float(r[8 * e]), __uint_as_float(r[8 * e + 1])), bf2(__uint_as_float(r[8 * e + 2]), __uint_as_float(r[8 * e + 3])),
+                                       bf2(__uint_as_float(r[8 * e + 4]), __uint_as_float(r[8 * e + 5])), bf2(__uint_as_float(r[8 * e + 6]), __uint_as_float(r[8 * e + 7])));
+                }
+            }
+            // Rows by way of shared memory: a store of 16 bytes to each of 32 rows is 32 half sectors, and was the longest part of
+            // a short CTA.
+            if (!shared && nx > 0) {
+                __syncwarp();
+                constexpr int PER = DP / 8, AT_ONCE = 32 / PER;     // lanes to a row, rows to a store
+                const int64_t mine = live ? dst - a.out : -1;
+#pragma unroll 4
+                for (int i = 0; i < PER; ++i) {
+                    const int from = i * AT_ONCE + lane / PER, c = lane % PER;
+                    const int64_t off = __shfl_sync(0xffffffffu, mine, from);
+                    const uint4 w = *reinterpret_cast<const uint4*>(stage + from * (DP * 2) + (c ^ (from & 7)) * 16);
+                    if (off >= 0 && 8 * c < a.D) *reinterpret_cast<uint4*>(a.out + off + 8 * c) = w;
                 }
             }
         }
