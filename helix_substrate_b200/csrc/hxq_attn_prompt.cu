@@ -720,7 +720,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 part[0] = ref;
                 part[2 * BM] = l;
             }
-#pragma unroll 1
+#pragma unroll 2
             for (int d = 0; d < DP; d += 32) {
                 uint32_t r[32];
                 if (nx > 0) {
@@ -763,7 +763,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 __syncwarp();
                 constexpr int PER = DP / 8, AT_ONCE = 32 / PER;     // lanes to a row, rows to a store
                 const int64_t mine = live ? dst - a.out : -1;
-#pragma unroll 4
+#pragma unroll 8
                 for (int i = 0; i < PER; ++i) {
                     const int from = i * AT_ONCE + lane / PER, c = lane % PER;
                     const int64_t off = __shfl_sync(0xffffffffu, mine, from);

@@ -538,7 +538,9 @@ __global__ void __launch_bounds__(32 * kWarps, kDecodeCtas) decode_kernel(const 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int D = FULL ? DP : a.c.D;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(ring_smem) + (uint32_t)(warp * RING);
-    pdl_enter();
+    // In this order: the joining launch, which comes in now, reads the positions before it waits for this one.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     int b, kvh, units;
     int64_t flat = 0, flat_end = 0, pair0 = 0;     // this CTA's places, and the place at which the pair starts
     if (CLUSTER) {
@@ -926,34 +928,67 @@ __global__ void __launch_bounds__(32 * kWarps, kDecodeCtas) decode_kernel(const 
 }
 
 // Joins the partial results of the pairs that more than one CTA had a segment of:
-// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c; sequences with nothing to see get zeros.  A long context has a
-// hundred partial results and more: four groups of threads take every fourth, several loads in flight each.
-constexpr int kJoin = 4;
+// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c; sequences with nothing to see get zeros.  kFew results are one round
+// trip to memory.  A long context has a hundred and more, and a large CTA.
+// (32 sequences: 128 threads a CTA, so that all CTAs are there and have found their pairs when the last result is written, and
+// one round trip: 10 -> 3 us.)
+constexpr int kJoin = 8, kFew = 8, kHeld = 28;
+static_assert(kJoin * kMaxD >= kDecodeCtas * 148 + 1, "a thread to a result");
 __global__ void __launch_bounds__(kJoin * kMaxD) combine_kernel(const DecodeArgs a) {
     __shared__ float w_s[kDecodeCtas * 148 + 1], o_s[kJoin][kMaxD], red[2][kJoin * kMaxD / 32];
     const int kvh = blockIdx.x, hd = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, D = a.c.D;
     const int d = tid & (kMaxD - 1), j = tid / kMaxD, lane = tid & 31, warp = tid >> 5;
-    pdl_enter();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     int64_t total;
     const Share at = find(a, 0, b, total);
+    const int64_t s = at.before * a.c.nkv + (int64_t)kvh * (at.units + kPad), e = s + at.units;
+    const int c0 = (int)(s / at.per), n = at.units == 0 ? 0 : (int)((e - 1) / at.per) - c0 + 1;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     __nv_bfloat16* out = a.out + (int64_t)b * a.ld_out + ((int64_t)kvh * a.G + hd) * D;
-    if (at.units == 0) {
+    if (n == 0) {
         if (tid < D) out[tid] = __float2bfloat16_rn(0.f);
         return;
     }
-    const int64_t s = at.before * a.c.nkv + (int64_t)kvh * (at.units + kPad), e = s + at.units;
-    const int c0 = (int)(s / at.per), n = (int)((e - 1) / at.per) - c0 + 1;
     if (n == 1) return;           // one CTA had it all and wrote it
     // the CTA that a pair starts in has it in its first slot if it starts there, too, the others always
     const int64_t step = 2 * (int64_t)a.G * (D + 2);
     const float* base = a.part + c0 * step + (int64_t)hd * (D + 2);
     const int64_t skip = s == c0 * at.per ? 0 : step / 2;
     auto part = [&](int c) { return base + c * step + (c == 0 ? skip : 0); };
-    float mx = -INFINITY;
-    for (int c = tid; c < n; c += kJoin * kMaxD) {
-        w_s[c] = part(c)[0];
-        mx = fmaxf(mx, w_s[c]);
+    if (n <= kFew || blockDim.x < kJoin * kMaxD) {
+        if (tid >= D) return;
+        float top = -INFINITY, lv = 0.f, ov = 0.f;
+        for (int at0 = 0; at0 < n; at0 += kFew) {
+            float m[kFew], l[kFew], o[kFew], mx = top;
+#pragma unroll
+            for (int i = 0; i < kFew; ++i) {
+                const int c = at0 + i;
+                m[i] = c < n ? part(c)[0] : -INFINITY;
+                l[i] = c < n ? part(c)[1] : 0.f;
+                o[i] = c < n ? part(c)[2 + tid] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < kFew; ++i) mx = fmaxf(mx, m[i]);
+            const float ref = mx == -INFINITY ? 0.f : mx, corr = ex2(top - ref);
+            lv *= corr;
+            ov *= corr;
+#pragma unroll
+            for (int i = 0; i < kFew; ++i) {
+                const float w = ex2(m[i] - ref);
+                lv += w * l[i];
+                ov += w * o[i];
+            }
+            top = mx;
+        }
+        out[tid] = __float2bfloat16_rn(ov / lv);
+        return;
     }
+    // a thread to a result's maximum and sum, a group of threads to every kJoin-th result's outputs, all under way at once
+    float v[kHeld], m = -INFINITY, l = 0.f;
+    if (tid < n) { m = part(tid)[0]; l = part(tid)[1]; }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) v[i] = d < D && j + kJoin * i < n ? part(j + kJoin * i)[2 + d] : 0.f;
+    float mx = m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     if (lane == 0) red[0][warp] = mx;
@@ -961,28 +996,29 @@ __global__ void __launch_bounds__(kJoin * kMaxD) combine_kernel(const DecodeArgs
     mx = red[0][0];
 #pragma unroll
     for (int w = 1; w < kJoin * kMaxD / 32; ++w) mx = fmaxf(mx, red[0][w]);
-    const float ref = mx == -INFINITY ? 0.f : mx;
-    float l = 0.f;
-    for (int c = tid; c < n; c += kJoin * kMaxD) {
-        const float w = ex2(w_s[c] - ref);
-        w_s[c] = w;
-        l += w * part(c)[1];
-    }
+    const float weight = ex2(m - (mx == -INFINITY ? 0.f : mx));
+    if (tid < n) w_s[tid] = weight;
+    l *= weight;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     if (lane == 0) red[1][warp] = l;
     __syncthreads();
     float o = 0.f;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        if (j + kJoin * i < n) o += w_s[j + kJoin * i] * v[i];
     if (d < D)
 #pragma unroll 8
-        for (int c = j; c < n; c += kJoin) o += w_s[c] * part(c)[2 + d];
+        for (int c = j + kJoin * kHeld; c < n; c += kJoin) o += w_s[c] * part(c)[2 + d];
     o_s[j][d] = o;
     __syncthreads();
     if (tid < D) {
-        float lv = 0.f;
+        float lv = 0.f, ov = 0.f;
 #pragma unroll
         for (int w = 0; w < kJoin * kMaxD / 32; ++w) lv += red[1][w];
-        out[d] = __float2bfloat16_rn((o_s[0][d] + o_s[1][d] + o_s[2][d] + o_s[3][d]) / lv);
+#pragma unroll
+        for (int w = 0; w < kJoin; ++w) ov += o_s[w][d];
+        out[d] = __float2bfloat16_rn(ov / lv);
     }
 }
 
@@ -1144,6 +1180,8 @@ extern "C" int hxq_attn_decode_kv8(const hxq_kv8* cache, const void* q, int64_t 
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
     if (clustered) return run_decode<true>(a, stream) == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
     cudaError_t e = run_decode<false>(a, stream);
-    if (e == cudaSuccess) e = launch_pdl(combine_kernel, dim3(cache->nkv, a.G, B), dim3(kJoin * kMaxD), stream, 0, a);
+    // (about ctas / (B nkv) results a pair)
+    const bool few = (int64_t)a.ctas <= (int64_t)B * cache->nkv * (kFew - 2);
+    if (e == cudaSuccess) e = launch_pdl(combine_kernel, dim3(cache->nkv, a.G, B), dim3(few ? kMaxD : kJoin * kMaxD), stream, 0, a);
     return e == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
 }
