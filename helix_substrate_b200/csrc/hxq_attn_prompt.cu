@@ -53,19 +53,20 @@ namespace attnp {
 
 constexpr int BM = 128;                     // rows of a tile
 constexpr int BN = 64;                      // keys of a step
-constexpr int SM_WARPS = 8;                 // softmax: four per tile
-constexpr int NUM_THREADS = 32 * (SM_WARPS + 4);
 constexpr int kMaxStages = 8;
 constexpr int kBarBytes = 768;
-constexpr int kShare = 8, kAlone = 16;       // key tiles: that a CTA of a shared item has at least; up to which an item is not shared
+constexpr int kMany = 4 * 148;              // items of two tiles from which on the tiles stay together
+constexpr int kShare = 8;                   // key tiles that a CTA of a shared item has at least
 constexpr int kPolyOf4 = 1;                 // of four pairs of weights, how many are made on the multiply-add units
-constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 88;      // of a thread: at launch, and after the roles have parted
 
-template <int DP>
+template <int DP, int TILES>
 struct Sizes {
-    static constexpr int kQ = BM * DP * 2, kTile = BN * DP * 2;      // a Q tile, a K or V tile
-    static constexpr int kStages = DP == 128 ? 5 : 8;                // of two tiles: the first two of K, then one of V and one of K
-    static constexpr int kSmem = 2 * kQ + 2 * kStages * kTile + kBarBytes;
+    static constexpr int kSoftmaxWarps = 4 * TILES, kThreads = 32 * (kSoftmaxWarps + 4);
+    static constexpr int kRegsLaunch = TILES == 2 ? 168 : 128;                // of a thread: at launch, and after the roles have parted
+    static constexpr int kRegsSoftmax = TILES == 2 ? 208 : 192, kRegsOther = TILES == 2 ? 88 : 64;
+    static constexpr int kQ = BM * DP * 2, kTile = BN * DP * 2;               // a Q tile, a K or V tile
+    static constexpr int kStages = TILES == 2 ? (DP == 128 ? 5 : 8) : (DP == 128 ? 2 : 6);      // of two tiles: the first two of K, then one of V and one of K
+    static constexpr int kSmem = TILES * kQ + 2 * kStages * kTile + kBarBytes;
 };
 
 struct Args {
@@ -76,7 +77,7 @@ struct Args {
     int32_t* status;
     int64_t v_seq, v_head, v_row, o_tok, o_head;
     float* part;            // splits > 1: [items][splits][DP + 2][2 * BM]: reference point, sum, output before the division
-    int32_t Tq, Tk, S, nkv, G, D, tpg, n_ct, causal, splits, groups;       // groups of 32 rows of an item that any token can fill
+    int32_t Tq, Tk, S, nkv, G, D, tpg, rows, n_ct, causal, splits, alone, groups;     // rows: tokens of an item; alone: key tiles up to which a sequence's items are not shared; groups of 32 rows of an item that any token can fill
     float scale_log2;
 };
 
@@ -114,14 +115,13 @@ struct Share {
     int used, per;
 };
 __device__ __forceinline__ Share find_share(const Args& a, int lq, int keys, int i0) {
-    if (a.splits == 1) return {1, 0};
-    const int last = i0 + 2 * a.tpg < lq ? i0 + 2 * a.tpg - 1 : lq - 1;
+    if (a.splits == 1 || keys <= a.alone * BN) return {1, 0};
+    const int last = i0 + a.rows < lq ? i0 + a.rows - 1 : lq - 1;
     const int total = (reach(a, lq, keys, last) + BN - 1) / BN, each = (total + a.splits - 1) / a.splits;
-    if (total <= kAlone) return {1, 0};
     const int per = each > kShare ? each : kShare;
-    return {(total + per - 1) / per, per};
+    return {total > 0 ? (total + per - 1) / per : 1, per};
 }
-// Item i: two tiles' tokens (from ct * 2 * tpg on) of one sequence and KV head.  The items of all sequences stand in a row by
+// Item i: a CTA's tokens (from ct * rows on) of one sequence and KV head.  The items of all sequences stand in a row by
 // falling ct, the longest work (of causal attention) first, with no gaps for sequences that are shorter than others.
 // A warp finds the item: F(c), the number of items with ct >= c of one head, falls in c.
 __device__ __forceinline__ bool find_item(const Args& a, int i, Seq& q, int& s, int& ct, int& kvh) {
@@ -129,7 +129,7 @@ __device__ __forceinline__ bool find_item(const Args& a, int i, Seq& q, int& s, 
     kvh = i % a.nkv;
     i /= a.nkv;
     auto items = [&](int lq) {
-        const int n = (lq + 2 * a.tpg - 1) / (2 * a.tpg);
+        const int n = (lq + a.rows - 1) / a.rows;
         return n < a.n_ct ? n : a.n_ct;
     };
     if (a.S == 1) {             // (0.7 us less, of 5)
@@ -331,11 +331,12 @@ __device__ __forceinline__ uint64_t make_desc_mn_sw128(uint32_t smem_addr, uint3
     return d;
 }
 
-template <int DP>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
+template <int DP, int TILES>
+__global__ void __launch_bounds__(Sizes<DP, TILES>::kThreads, 3 - TILES)
 attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v, const Args a) {
-    using Z = Sizes<DP>;
+    using Z = Sizes<DP, TILES>;
+    constexpr int SM_WARPS = Z::kSoftmaxWarps, NUM_THREADS = Z::kThreads;
     constexpr int NS = Z::kStages, QT = Z::kQ, TILE = Z::kTile;
     constexpr int QHALF = BM * 128, HALF = BN * 128;      // 64 of the dimensions of a Q tile, of a K or V tile
     extern __shared__ __align__(1024) char smem[];        // (no room for slack: the swizzled tiles need that alignment, checked here)
@@ -343,7 +344,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (threadIdx.x == 0 && a.status != nullptr) atomicExch(a.status, HXQ_E_ALIGN);
         return;
     }
-    char* ring = smem + 2 * QT;
+    char* ring = smem + TILES * QT;
     uint64_t* full = reinterpret_cast<uint64_t*>(ring + NS * 2 * TILE);      // [NS] a stage has landed, ready for its products
     uint64_t* empty = full + kMaxStages;        // [NS] its products have retired
     uint64_t* raw = empty + kMaxStages;         // [NS] a stage whose V tile is to be cleaned has landed (full is not signalled) ...
@@ -366,7 +367,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     if (warp == SM_WARPS) {
         constexpr int BARS = 4 * kMaxStages + 13, CLEAN = 3 * kMaxStages, P_READY = 4 * kMaxStages + 5;
         for (int i = lane; i < BARS; i += 32)
-            sm100::mbar_init(full + i, i >= CLEAN && i < CLEAN + kMaxStages ? 2 : (i >= P_READY && i < P_READY + 4 ? SM_WARPS / 2 : 1));
+            sm100::mbar_init(full + i, i >= CLEAN && i < CLEAN + kMaxStages ? 2 : (i >= P_READY && i < P_READY + 4 ? 4 : 1));
         if (lane == 0) {
             *abort_flag = 0;
             *odd_v = 0;
@@ -383,9 +384,9 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         int s, ct, kvh;
         bool found = find_item(a, item, seq, s, ct, kvh);
         if (found && lane == 0) {
-            const Share sh = find_share(a, seq.lq, seq.lk, ct * 2 * a.tpg);
+            const Share sh = find_share(a, seq.lq, seq.lk, ct * a.rows);
             found = share < sh.used;
-            const int i0 = ct * 2 * a.tpg, last = i0 + 2 * a.tpg < seq.lq ? i0 + 2 * a.tpg - 1 : seq.lq - 1, skip = share * sh.per * BN;
+            const int i0 = ct * a.rows, last = i0 + a.rows < seq.lq ? i0 + a.rows - 1 : seq.lq - 1, skip = share * sh.per * BN;
             int n = reach(a, seq.lq, seq.lk, last) - skip;
             if (sh.used > 1 && n > sh.per * BN) n = sh.per * BN;
             if (found && n > 0) {
@@ -393,8 +394,8 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 for (int t = 0; t < (n > BN ? 2 : 1); ++t)
                     for (int h = 0; h < DP / 64; ++h)
                         tma_load_4d(sm100::smem_u32(ring + t * TILE + h * HALF), &map_k, &full[0], 64 * h, seq.k0 + skip + t * BN, kvh, a.cu_k != nullptr ? 0 : s);
-                sm100::mbar_arrive_expect_tx(q_full, 2u * (DP / 64) * (uint32_t)rows * 128u);
-                for (int x = 0; x < 2; ++x)
+                sm100::mbar_arrive_expect_tx(q_full, (uint32_t)TILES * (DP / 64) * (uint32_t)rows * 128u);
+                for (int x = 0; x < TILES; ++x)
                     for (int h = 0; h < DP / 64; ++h)
                         tma_load_3d(sm100::smem_u32(smem + x * QT + h * QHALF), &map_q, q_full, 64 * h, kvh * a.G, seq.q0 + i0 + x * a.tpg);
             }
@@ -406,15 +407,15 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
             job[3] = seq.k0;
             job[4] = seq.lk;
             job[5] = s;
-            job[6] = ct * 2 * a.tpg;
+            job[6] = ct * a.rows;
             job[7] = kvh;
         }
     } else if (warp == SM_WARPS + 1) {
-        sm100::tmem_alloc(tmem_slot, 512);
+        sm100::tmem_alloc(tmem_slot, 256 * TILES);
         sm100::tmem_relinquish();
     } else {        // rows of the Q tiles that no token fills
         const int idle = (BM - rows) * 8, i0 = threadIdx.x - (warp > SM_WARPS ? 64 : 0);
-        for (int part = 0; part < 2 * (DP / 64); ++part)
+        for (int part = 0; part < TILES * (DP / 64); ++part)
             for (int i = i0; i < idle; i += NUM_THREADS - 64)
                 *reinterpret_cast<uint4*>(smem + part * QHALF + (rows + (i >> 3)) * 128 + (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
     }
@@ -426,7 +427,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tmem = *tmem_slot;       // S of tile 0: two buffers of 64 columns; of tile 1; O of either, 128 columns each
     if (job[0] == 0) {
-        if (warp == SM_WARPS + 1) sm100::tmem_dealloc(tmem, 512);
+        if (warp == SM_WARPS + 1) sm100::tmem_dealloc(tmem, 256 * TILES);
         return;
     }
     const int q0 = job[1], lq = job[2], all_keys = job[4], s = job[5], i0 = job[6], kvh = job[7];
@@ -442,14 +443,14 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (first >= lq) return 0;
         return (count(first + a.tpg < lq ? first + a.tpg - 1 : lq - 1) + BN - 1) / BN;
     };
-    const int n0 = steps(0), n1 = steps(1), n = n0 > n1 ? n0 : n1;
+    const int n0 = steps(0), n1 = TILES == 2 ? steps(1) : 0, n = n0 > n1 ? n0 : n1;
     const int seen_by_all = count(i0);          // keys that every token of this CTA sees
     const int jc = seen_by_all / BN;            // V tiles from here on are looked at
     bool ok = true;
 
-    static_assert(32 * SM_WARPS * kRegsSoftmax + 128 * kRegsOther <= NUM_THREADS * kRegsLaunch, "no more registers than the launch brings");
+    static_assert(32 * SM_WARPS * Z::kRegsSoftmax + 128 * Z::kRegsOther <= NUM_THREADS * Z::kRegsLaunch, "no more registers than the launch brings");
     if (warp >= SM_WARPS) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Z::kRegsOther));
     if (warp == SM_WARPS) {
         // ------------------------------------------------------------ loads, in the order of their use: K0 K1 (above) | V0 K2 | V1 K3 | ...
         if (lane == 0 && n > 0) {
@@ -520,13 +521,13 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 if (cleaned) clean_ph ^= 1u << here; else full_ph ^= 1u << here;
                 stage = here + 1 == NS ? 0 : here + 1;
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
+                for (int x = 0; x < TILES; ++x) {
                     const int nx = x ? un1 : un0;
                     const bool live = PLAIN || j < nx;
                     if (live && !p_done) ok = bar_wait(p_at + (uint32_t)(8 * (2 * x + buf)), p_phase, abort_flag) && ok;
                     sm100::tc_fence_after_sync();
-                    // the next looks: at the other tile's weights of this step, or this tile's of the next and the next stage
-                    if (x == 0) {
+                    // the next looks: at the other tile's weights of this step, or the first's of the next and the next stage
+                    if (x + 1 < TILES) {
                         p_done = peek(p_at + (uint32_t)(8 * (2 + buf)), p_phase);
                     } else {
                         const bool next_cleaned = !PLAIN && j + 1 >= ujc;
@@ -536,7 +537,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                     if (live) {
 #pragma unroll
                         for (int k = 0; k < BN / 16; ++k)
-                            umma_ts(leader, ut + (uint32_t)(256 + 128 * x), ut + (uint32_t)(128 * x + 64 * buf + 8 * k), dv + at / 16 + (uint32_t)(k * (2048 / 16)), idesc_o,
+                            umma_ts(leader, ut + (uint32_t)(128 * TILES + 128 * x), ut + (uint32_t)(128 * x + 64 * buf + 8 * k), dv + at / 16 + (uint32_t)(k * (2048 / 16)), idesc_o,
                                     (j > 0 || k > 0) ? 1u : 0u);
                         if (!PLAIN && j + 2 >= nx) commit(leader, o_at + (uint32_t)(16 * x) + (j + 1 == nx ? 8u : 0u));
                     }
@@ -546,7 +547,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 ok = __all_sync(0xffffffffu, ok);
             };
             int j = 0;
-            const int plain = min(min(un0, un1) - 2, ujc);
+            const int plain = min((TILES == 2 ? min(un0, un1) : un0) - 2, ujc);
             for (; j + 2 <= plain && ok; j += 2) {
                 step(j, std::true_type{}, std::integral_constant<int, 0>{});
                 if (ok) step(j + 1, std::true_type{}, std::integral_constant<int, 1>{});
@@ -605,13 +606,13 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     }
     } else {
         // ------------------------------------------------------------ softmax and epilogue: TMEM lane == row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Z::kRegsSoftmax));
         const int x = warp >> 2, row = 32 * (warp & 3) + lane;
         const int nx = x ? n1 : n0;
         const int cnt = count(i0 + x * a.tpg + row / a.G);
         const int seen = nx > 0 ? count(i0 + x * a.tpg) : 0;        // keys that every row of the tile sees
         const uint32_t t_lane = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-        const uint32_t to = t_lane + 256u + 128u * x;
+        const uint32_t to = t_lane + 128u * TILES + 128u * x;
         const float sc = a.scale_log2;
         float ref = -INFINITY, l = 0.f;         // in units of S
         float first = 0.f, bias = 0.f;
@@ -710,7 +711,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (ok) {
             sm100::tc_fence_after_sync();
             const int tok = job[6] + x * a.tpg + row / a.G, head = job[7];
-            const bool live = row < a.G * a.tpg && tok < job[2], shared = a.splits > 1 && find_share(a, job[2], job[4], job[6]).used > 1;
+            const bool live = row < a.G * a.tpg && tok < job[2], shared = TILES == 2 && a.splits > 1 && find_share(a, job[2], job[4], job[6]).used > 1;
             const float inv = shared ? 1.f : 1.f / l;
             const bool odd = nx > 0 && *odd_v != 0;
             __nv_bfloat16* dst = a.out + (int64_t)(job[1] + tok) * a.o_tok + (int64_t)(head * a.G + row % a.G) * a.o_head;
@@ -782,7 +783,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
     __syncthreads();
     if (warp == SM_WARPS + 1) {
         sm100::tc_fence_after_sync();
-        sm100::tmem_dealloc(tmem, 512);
+        sm100::tmem_dealloc(tmem, 256 * TILES);
     }
     if (threadIdx.x == 0 && *abort_flag != 0 && a.status != nullptr) atomicExch(a.status, HXQ_E_TIMEOUT);
 }
@@ -801,7 +802,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a) {
     Seq seq;
     int s, ct, kvh;
     if (!find_item(a, item, seq, s, ct, kvh)) return;
-    const int used = find_share(a, seq.lq, seq.lk, ct * 2 * a.tpg).used;
+    const int used = find_share(a, seq.lq, seq.lk, ct * a.rows).used;
     if (used == 1) return;              // written already
     const int x = group >> 2, first = (2 * ct + x) * a.tpg, left = seq.lq - first, rows = a.G * (left < a.tpg ? left : a.tpg);
     const int in = (group & 3) * 32 + lane;
@@ -847,32 +848,39 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a) {
 // ---- host side ---------------------------------------------------------------------
 
 struct Plan {
-    int tpg, n_ct, items, splits, groups;
+    int tpg, rows, n_ct, items, splits, alone, groups;
 };
-// Items: the tokens' tiles, one more for each sequence's last.  Few of them before many keys leave SMs idle: then their key tiles are
-// shared out, to as many CTAs as there are SMs for (16 tokens behind 32768 keys, 28 query and 4 KV heads: 4 items of 512 tiles).
-// max_q has no say in it: it would in the result's last bits.
+// Items: the tokens' tiles, two to a CTA, and one more for each sequence's last.
+// Few of them before many keys leave SMs idle: then their key tiles are shared out, to as many CTAs (room) as there are SMs
+// for.  Sharing costs a launch and the shares' way through memory, and pays from some number of key tiles on, the sooner the more
+// room there is (28 + 4 heads, 16 queries, room 37, behind 32768 keys: 360 -> 28 us; 256, room 4: 349 -> 145, but 19 -> 28
+// behind 1024; 512, room 2: 352 -> 276, but 50 -> 63 behind 4096).  max_q has no say in any of this: it would in the result's last bits.
+// Items that stay whole have one tile each and come two to an SM, where one's start and end pass behind the other's products
+// (813 tokens behind 8111: 106 -> 95 us; 908 tokens of 3 heads: 18.9 -> 13.8 us), unless there are so many that these matter less than
+// keys and values read twice as often (16384 tokens: 1543 us together, 1636 apart).
 static bool make_plan(const hxq_attn* p, Plan& plan) {
     plan.tpg = BM / (p->nq / p->nkv);
-    const int64_t max_q = p->max_q < p->Tq ? p->max_q : p->Tq, rows = 2 * plan.tpg;
-    plan.n_ct = (int)((max_q + rows - 1) / rows);
-    const int64_t all = (int64_t)p->Tq / rows + p->S, most = (int64_t)plan.n_ct * p->S;
-    const int64_t n = (all < most ? all : most) * p->nkv;
+    const int64_t max_q = p->max_q < p->Tq ? p->max_q : p->Tq;
+    const int64_t all = ((int64_t)p->Tq / (2 * plan.tpg) + p->S) * p->nkv, room = 148 / all;
     const int64_t keys = p->cu_k == p->cu_q && max_q < p->Tk ? max_q : p->Tk;        // of one sequence, at most
-    const int64_t steps = (keys + BN - 1) / BN, parts = steps <= kAlone ? 1 : (steps + kShare - 1) / kShare, room = 148 / (all * p->nkv);
-    const int64_t splits = parts < room ? parts : room;
+    const int64_t steps = (keys + BN - 1) / BN, parts = (steps + kShare - 1) / kShare;
+    plan.alone = room > 1 ? 16 + (int)(384 / (room * room)) : 0;
+    plan.splits = room > 1 && steps > plan.alone ? (int)(parts < room ? parts : room) : 1;
+    plan.rows = plan.splits > 1 || all >= kMany ? 2 * plan.tpg : plan.tpg;
+    const int64_t n_ct = (max_q + plan.rows - 1) / plan.rows;
+    const int64_t some = (int64_t)p->Tq / plan.rows + p->S, most = n_ct * p->S, n = (some < most ? some : most) * p->nkv;
+    plan.n_ct = (int)n_ct;
     plan.items = (int)n;
     plan.groups = max_q > plan.tpg ? 8 : (int)((max_q * (p->nq / p->nkv) + 31) / 32);
-    plan.splits = splits > 1 ? (int)splits : 1;
-    return n <= 0x7fffffffLL / 64;
+    return n <= 0x7fffffffLL / 128;
 }
 static size_t part_bytes(const hxq_attn* p, const Plan& plan) {
     return plan.splits == 1 ? 0 : (size_t)plan.items * plan.splits * 2 * BM * ((p->D <= 64 ? 64 : 128) + 2) * sizeof(float);
 }
 
-template <int DP>
-static int run(const hxq_attn* p, const Plan& plan, void* workspace, int32_t* status, cudaStream_t stream) {
-    using Z = Sizes<DP>;
+template <int DP, int TILES>
+static int run_tiles(const hxq_attn* p, const Plan& plan, void* workspace, int32_t* status, cudaStream_t stream) {
+    using Z = Sizes<DP, TILES>;
     Args a;
     a.cu_q = p->cu_q; a.cu_k = p->cu_k; a.k_len = p->k_len;
     a.v = reinterpret_cast<const __nv_bfloat16*>(p->v);
@@ -881,8 +889,10 @@ static int run(const hxq_attn* p, const Plan& plan, void* workspace, int32_t* st
     a.v_seq = p->v_seq; a.v_head = p->v_head; a.v_row = p->v_row; a.o_tok = p->o_tok; a.o_head = p->o_head;
     a.Tq = p->Tq; a.Tk = p->Tk; a.S = p->S; a.nkv = p->nkv; a.G = p->nq / p->nkv; a.D = p->D; a.causal = p->causal != 0;
     a.tpg = plan.tpg;
+    a.rows = plan.rows;
     a.n_ct = plan.n_ct;
     a.splits = plan.splits;
+    a.alone = plan.alone;
     a.groups = plan.groups;
     a.part = reinterpret_cast<float*>(workspace);
     a.scale_log2 = p->scale * 1.4426950408889634f;
@@ -907,13 +917,13 @@ static int run(const hxq_attn* p, const Plan& plan, void* workspace, int32_t* st
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return HXQ_E_DEVICE;
     if (!attr_set[dev]) {
         cudaFuncAttributes fa;        // the warps' exchange of registers counts on what the launch brings
-        if (cudaFuncGetAttributes(&fa, attn_prompt_kernel<DP>) != cudaSuccess || fa.numRegs < kRegsLaunch) return HXQ_E_DEVICE;
-        if (cudaFuncSetAttribute(attn_prompt_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::kSmem) != cudaSuccess) return HXQ_E_DEVICE;
+        if (cudaFuncGetAttributes(&fa, attn_prompt_kernel<DP, TILES>) != cudaSuccess || fa.numRegs < Z::kRegsLaunch) return HXQ_E_DEVICE;
+        if (cudaFuncSetAttribute(attn_prompt_kernel<DP, TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::kSmem) != cudaSuccess) return HXQ_E_DEVICE;
         attr_set[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(plan.items * plan.splits));
-    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.blockDim = dim3(Z::kThreads);
     cfg.dynamicSmemBytes = Z::kSmem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -921,7 +931,7 @@ static int run(const hxq_attn* p, const Plan& plan, void* workspace, int32_t* st
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, attn_prompt_kernel<DP>, mq, mk, mv, a);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, attn_prompt_kernel<DP, TILES>, mq, mk, mv, a);
     if (e == cudaSuccess && plan.splits > 1) {
         cfg.gridDim = dim3((unsigned)(plan.items * plan.groups * (DP / kJoin)));
         cfg.blockDim = dim3(256);
@@ -929,6 +939,10 @@ static int run(const hxq_attn* p, const Plan& plan, void* workspace, int32_t* st
         e = cudaLaunchKernelEx(&cfg, join_kernel<DP>, a);
     }
     return e == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
+}
+template <int DP>
+static int run(const hxq_attn* p, const Plan& plan, void* workspace, int32_t* status, cudaStream_t stream) {
+    return plan.rows == plan.tpg ? run_tiles<DP, 1>(p, plan, workspace, status, stream) : run_tiles<DP, 2>(p, plan, workspace, status, stream);
 }
 
 }  // namespace attnp

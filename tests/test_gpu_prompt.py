@@ -290,3 +290,42 @@ def test_the_same_bits_every_time(nq, nkv, D, lens):
     assert all(torch.equal(outs[0], o) for o in outs)
     a, b = int(cu[0]), int(cu[1])
     _compare(outs[0][a:b], _want(q[a:b], k[a:b], v[a:b], D ** -0.5, True), "the first")
+
+
+@pytest.mark.parametrize("nq,nkv,D", [(128, 4, 128), (128, 4, 64), (112, 16, 72)])
+def test_many_tiles(nq, nkv, D):
+    """So many rows that thread blocks take two tiles each; a sequence by itself, one tile each, gives the same bits."""
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, lens = _dev(), [800, 37, 0, 1, 256, 129, 300]
+    T = sum(lens)
+    g = torch.Generator(device=dev).manual_seed(D)
+    q = torch.randn(T, nq, D, device=dev, generator=g).bfloat16()
+    k, v = (torch.randn(T, nkv, D, device=dev, generator=g).bfloat16() for _ in range(2))
+    v[1000, 1, 3] = float("inf")
+    cu = [sum(lens[:s]) for s in range(len(lens) + 1)]
+    for causal in (True, False):
+        out = torch.empty(T, nq, D, device=dev, dtype=torch.bfloat16)
+        attn_prompt(q, k, v, out, torch.tensor(cu, dtype=torch.int32, device=dev), max(lens), D ** -0.5, causal=causal)
+        for a, b in zip(cu, cu[1:]):
+            if b == a:
+                continue
+            _compare(out[a:b], _want(q[a:b], k[a:b], v[a:b], D ** -0.5, causal), (causal, a, b))
+            alone = torch.empty(b - a, nq, D, device=dev, dtype=torch.bfloat16)
+            attn_prompt(q[a:b], k[a:b], v[a:b], alone, torch.tensor([0, b - a], dtype=torch.int32, device=dev), b - a, D ** -0.5, causal=causal)
+            assert torch.equal(alone.view(torch.int16), out[a:b].view(torch.int16)), (causal, a, b)
+
+
+def test_hundreds_of_sequences():
+    """More sequences than a warp's lanes hold at once, most of them short, one long, some empty."""
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, nq, nkv, D = _dev(), 6, 2, 64
+    lens = [(7 * s) % 23 for s in range(300)]
+    lens[170] = 500
+    T = sum(lens)
+    g = torch.Generator(device=dev).manual_seed(3)
+    q, k, v = (torch.randn(T, n, D, device=dev, generator=g).bfloat16() for n in (nq, nkv, nkv))
+    cu = [sum(lens[:s]) for s in range(len(lens) + 1)]
+    out = torch.full((T, nq, D), 7.0, device=dev, dtype=torch.bfloat16)
+    attn_prompt(q, k, v, out, torch.tensor(cu, dtype=torch.int32, device=dev), max(lens), 0.125)
+    want = torch.cat([_want(q[a:b], k[a:b], v[a:b], 0.125, True) for a, b in zip(cu, cu[1:]) if b > a])
+    _compare(out, want, "all")
