@@ -6,9 +6,9 @@
 //     out[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h / G]) v[j, h / G],   j < count(i),
 //     count(i) = lk - lq + i + 1 (causal) or lk;  a row with count(i) <= 0 is zero.
 //
-// One CTA takes two tiles of 128 rows.  A row is (token, head of the group): the G query heads of a KV head share
-// its keys, so a tile spans 128 / G tokens, the causal edge wastes that much less, and a short prompt fills its
-// tiles G times better than with a head per CTA.  Per 64 keys and tile, all on the tensor cores (tcgen05):
+// A tile is 128 rows.  A row is (token, head of the group): the G query heads of a KV head share its keys, so a tile
+// spans 128 / G tokens, the causal edge wastes that much less, and a short prompt fills its tiles G times better than
+// with a head per CTA.  Per 64 keys and tile, all on the tensor cores (tcgen05):
 //
 //     S = Q K^T       both operands in shared memory (TMA, 128-byte swizzle), S in tensor memory
 //     P = 2^(scale' S - m)      one thread per row, in registers: running maximum m and sum; P goes back to tensor
@@ -16,16 +16,20 @@
 //     O += P V        A operand from tensor memory, V as it lies in memory (its rows are the contraction), O in
 //                     tensor memory for the whole row
 //
-// Roles: warps 0-3 and 4-7 are the two tiles' softmax and epilogue, warp 8 feeds K and V through a ring of
-// 64-row tiles, warp 9 issues the MMAs, warps 10 and 11 clean V tiles.  P is rounded to bf16, V's type (the MMA takes no
-// other beside it): 2^-9 at most per weight, as much as the output's own rounding; the sum that divides takes the weights
-// before rounding.
+// Roles: four warps a tile are its softmax and epilogue, one warp feeds K and V through a ring, one issues the MMAs, two
+// clean V tiles.  P is rounded to bf16, V's type (the MMA takes no other beside it): 2^-9 at most per weight, as much as
+// the output's own rounding; the sum that divides takes the weights before rounding.
 //
-// A step's products, its softmax and the signals between them (about 1000 cycles of the last two thirds each) depend on
-// one another, and two tiles alone do not hide that: with 128 keys a step, S of the next waiting for P V of this one,
-// a step took 3900 cycles, its MMAs 2048.  So S has two buffers a tile, of 64 keys, tensor memory being full with them
-// and O: the next step's scores are there when a warp comes for them.  (Products of 64 keys cost a third more, 670 cycles a
-// step and tile instead of 512: a Q tile is read from shared memory for half the work.)
+// Bound by the tensor cores for long prompts, by each CTA's start and end for short ones.  A step's products, its softmax
+// and the signals between them depend on one another (about 1000 cycles of the last two each), so two tiles take turns, in one
+// CTA or in two on an SM, and S has two buffers a tile, of 64 keys, tensor memory being full with them and O: the next step's
+// scores are there when a warp comes for them.  (Products of 64 keys cost a third more, 670 cycles a step and tile instead of 512: a
+// Q tile is read from shared memory for half the work.  With 128 keys a step and one buffer, S of the next waiting for P V of
+// this one, a step took 3900 cycles, its products 2048.)  Both tiles' 64 keys take 1440 cycles, their products 1345.  16384
+// tokens of 28 + 4 heads of 128 take 1.54 to 1.63 ms, 1180 to 1250 TFLOP/s, at the 1.4 to 1.5 GHz that the power limit leaves.
+//
+// A CTA's start (finding its tokens 1 to 2 us, first loads and scores 1.3) and end (outputs by way of shared memory 2.5) cost
+// as much as ten to fifteen steps; of 2048 tokens and less they are half of the time.
 //
 // The reference point m moves only when the maximum has grown by more than 2^8: weights stay below 256, nothing
 // overflows, the result is the same, and O is rarely rescaled.
@@ -109,8 +113,8 @@ __device__ __forceinline__ int reach(const Args& a, int lq, int keys, int i) {  
     const int n = keys - lq + i + 1;
     return n > 0 ? n : 0;
 }
-// An item's key tiles are shared out among `used` CTAs, `per` tiles each.  Both follow from the item and a.splits, of which a larger
-// one than `used` changes nothing: the same bits from a slab of any length.
+// An item's key tiles are shared out among `used` CTAs, `per` tiles each, unless its sequence has few.  A larger a.splits than
+// `used` changes nothing: the same bits from a slab of any length.
 struct Share {
     int used, per;
 };
@@ -951,6 +955,7 @@ static int run(const hxq_attn* p, const Plan& plan, void* workspace, int32_t* st
 static int check(const hxq_attn* p) {
     if (!p || !p->q || !p->k || !p->v || !p->out || !p->cu_q || (!p->cu_k) == (!p->k_len)) return HXQ_E_ARG;
     if (p->Tq < 0 || p->Tk < 0 || p->S <= 0 || p->max_q < 0 || !(p->scale > 0.f) || !(p->scale <= 3.4e38f)) return HXQ_E_ARG;
+    if (p->Tq > 1 << 30 || p->Tk > 1 << 30) return HXQ_E_SHAPE;        // (coordinates past the end stay in 32 bits)
     if (p->nq <= 0 || p->nkv <= 0 || p->nq % p->nkv != 0 || p->nq / p->nkv > 64) return HXQ_E_SHAPE;
     if (p->D < 8 || p->D > 128 || p->D % 8 != 0) return HXQ_E_SHAPE;
     const int64_t strides[10] = {p->q_tok, p->q_head, p->k_seq, p->k_head, p->k_row, p->v_seq, p->v_head, p->v_row, p->o_tok, p->o_head};
@@ -971,6 +976,7 @@ extern "C" int hxq_attn_prompt(const hxq_attn* p, void* workspace, size_t worksp
     hxq::attnp::Plan plan;
     if (!hxq::attnp::make_plan(p, plan)) return HXQ_E_SHAPE;
     if (plan.items == 0) return HXQ_OK;
+    if (p->Tk == 0) return HXQ_E_SHAPE;
     const size_t need = hxq::attnp::part_bytes(p, plan);
     if (need > 0 && (!workspace || !hxq::aligned_to(workspace, 8) || workspace_bytes < need)) return HXQ_E_WORKSPACE;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

@@ -245,8 +245,8 @@ int32_t hxq_attn_decode_span(int32_t B, int32_t nkv, int32_t max_len);
  * cu_q, cu_k (int32 [S + 1], ascending) and k_len (int64 [S]) are DEVICE arrays, exactly one of cu_k and k_len given;
  * max_q: no sequence has more queries (those past it are not computed).  Rows of out that belong to no sequence are
  * left as they are.  Strides in elements, multiples of 8; pointers 16-byte aligned; D % 8 == 0, 8 <= D <= 128;
- * nq / nkv <= 64; scale > 0.  status_word as in hxq_gemm.  Few queries before many keys split the keys among
- * thread blocks: workspace is hxq_attn_prompt_workspace_bytes() of plain scratch (0: none needed).
+ * nq / nkv <= 64; Tq, Tk <= 2^30; scale > 0.  status_word as in hxq_gemm.  Few queries before many keys split the keys among
+ * thread blocks: workspace is hxq_attn_prompt_workspace_bytes() of 8-byte aligned scratch (0: none needed).
  */
 typedef struct hxq_attn {
     const void *q, *k, *v;
@@ -305,7 +305,7 @@ int hxq_rope_append_prompt_kv8(const hxq_kv8* cache, const void* qkv, int64_t ld
 
 /* hxq_attn_decode over an 8-bit cache: positions 0 .. pos[b] of slot b, the finished blocks from their codes, the
  * last one from the tail.  A position < 0 or >= max_len gives zeros.  nq / nkv <= 8.  workspace:
- * hxq_attn_decode_kv8_workspace_bytes() of plain scratch (0: none needed). */
+ * hxq_attn_decode_kv8_workspace_bytes() of 8-byte aligned scratch (0: none needed). */
 size_t hxq_attn_decode_kv8_workspace_bytes(int32_t B, int32_t nq, int32_t nkv, int32_t D, int32_t max_len);
 int hxq_attn_decode_kv8(const hxq_kv8* cache, const void* q, int64_t ld_q, const int64_t* pos, int32_t pos_stride,
                         void* out, int64_t ld_out, void* workspace, size_t workspace_bytes, int32_t B, int32_t nq,
