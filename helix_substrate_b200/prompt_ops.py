@@ -15,8 +15,7 @@ from .packed import _status_word
 
 
 def _heads(t: torch.Tensor, name: str, dev: torch.device, shape: tuple) -> None:
-    if not (t.dtype is torch.bfloat16 and t.device == dev and t.is_cuda and t.ndim == len(shape) and t.stride(-1) == 1
-            and all(w is None or n == w for n, w in zip(t.shape, shape))):
+    if not (t.dtype is torch.bfloat16 and t.device == dev and t.is_cuda and t.shape == shape and t.stride()[-1] == 1):
         raise TypeError(f"{name}: expected a CUDA bf16 tensor {tuple('*' if w is None else w for w in shape)} on {dev}, contiguous along "
                         f"its last dimension, got {t.dtype} {tuple(t.shape)} {t.stride()} on {t.device}")
 
@@ -34,16 +33,21 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Te
     slabs = k_len is not None
     if slabs and cu_k is not None:
         raise ValueError("keys lie packed (cu_k) or in slabs (k_len), not both")
-    _heads(q, "q", dev, (None, None, None))
-    T, nq, D = q.shape
+    q_shape, k_shape = q.shape, k.shape
+    _heads(q, "q", dev, q_shape if len(q_shape) == 3 else (None, None, None))
+    T, nq, D = q_shape
     S = cu_q.shape[0] - 1 if cu_q.ndim == 1 else -1
     if S < 1 or max_q < 0:
         raise ValueError(f"cu_q of shape {tuple(cu_q.shape)}, max_q {max_q}")
     _ints(cu_q, "cu_q", dev, torch.int32, S + 1)
-    _heads(k, "k", dev, (S, None, None, D) if slabs else (None, None, D))
-    _heads(v, "v", dev, tuple(k.shape))
-    _heads(out, "out", dev, (T, nq, D))
-    nkv, rows = (k.shape[1], k.shape[2]) if slabs else (k.shape[1], k.shape[0])
+    if slabs:
+        nkv, rows = k_shape[1:3] if len(k_shape) == 4 else (None, None)
+        _heads(k, "k", dev, (S, nkv, rows, D))
+    else:
+        rows, nkv = k_shape[:2] if len(k_shape) == 3 else (None, None)
+        _heads(k, "k", dev, (rows, nkv, D))
+    _heads(v, "v", dev, k_shape)
+    _heads(out, "out", dev, q_shape)
     if nkv < 1 or nq % nkv:
         raise ValueError(f"{nq} query heads over {nkv} KV heads")
     if slabs:
@@ -58,12 +62,13 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Te
         return out
     if rows == 0:
         raise ValueError("k and v have no rows")
-    ks, vs = k.stride(), v.stride()
-    k3, v3 = ((ks[0], ks[1], ks[2]), (vs[0], vs[1], vs[2])) if slabs else ((0, ks[1], ks[0]), (0, vs[1], vs[0]))
-    p = _lib.HxqAttn(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), *k3, *v3, out.stride(0),
-                     out.stride(1), cu_q.data_ptr(), None if slabs else cu_k.data_ptr(), k_len.data_ptr() if slabs else None,
-                     T, rows, S, min(max_q, T), nq, nkv, D, int(causal), scale)
-    nb = _lib.lib().hxq_attn_prompt_workspace_bytes(C.byref(p))
+    ks, vs, qs, os = k.stride(), v.stride(), q.stride(), out.stride()
+    if not slabs:
+        ks, vs = (0, ks[1], ks[0]), (0, vs[1], vs[0])
+    p = C.byref(_lib.HxqAttn(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qs[0], qs[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                             os[0], os[1], cu_q.data_ptr(), None if slabs else cu_k.data_ptr(), k_len.data_ptr() if slabs else None,
+                             T, rows, S, min(max_q, T), nq, nkv, D, int(causal), scale))
+    nb = _lib.lib().hxq_attn_prompt_workspace_bytes(p)
     ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None       # for this call alone: captured graphs do not share it
-    _call(dev, "hxq_attn_prompt", C.byref(p), None if ws is None else ws.data_ptr(), nb, _status_word(dev).data_ptr())
+    _call(dev, "hxq_attn_prompt", p, None if ws is None else ws.data_ptr(), nb, _status_word(dev).data_ptr())
     return out
