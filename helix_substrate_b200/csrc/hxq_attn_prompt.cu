@@ -25,11 +25,12 @@
 // CTA or in two on an SM, and S has two buffers a tile, of 64 keys, tensor memory being full with them and O: the next step's
 // scores are there when a warp comes for them.  (Products of 64 keys cost a third more, 670 cycles a step and tile instead of 512: a
 // Q tile is read from shared memory for half the work.  With 128 keys a step and one buffer, S of the next waiting for P V of
-// this one, a step took 3900 cycles, its products 2048.)  Both tiles' 64 keys take 1440 cycles, their products 1345.  16384
-// tokens of 28 + 4 heads of 128 take 1.54 to 1.63 ms, 1180 to 1250 TFLOP/s, at the 1.4 to 1.5 GHz that the power limit leaves.
+// this one, a step took 3900 cycles, its products 2048.)  Both tiles' 64 keys take 1530 to 1750 cycles, their products 1345; a
+// tile by itself takes 1241, its softmax's latency.  16384 tokens of 28 + 4 heads of 128 take 1.54 ms in a short run (1250
+// TFLOP/s), 1.80 in one of a second, at the 1.6 GHz that the power limit leaves.
 //
-// A CTA's start (finding its tokens 1 to 2 us, first loads and scores 1.3) and end (outputs by way of shared memory 2.5) cost
-// as much as ten to fifteen steps; of 2048 tokens and less they are half of the time.
+// A CTA's start (finding its tokens 1 to 2 us, first loads and scores 1.3) and end (V's edge 0.7, outputs by way of shared memory
+// 2.5) cost as much as seven steps; of 2048 tokens and less they are half of the time.
 //
 // The reference point m moves only when the maximum has grown by more than 2^8: weights stay below 256, nothing
 // overflows, the result is the same, and O is rarely rescaled.
@@ -481,7 +482,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         // what the loop computes is then known to be the same in every lane and stays in uniform registers, where the products
         // want it.  A barrier is looked at before the products in front of its use are issued, and waited for
         // only if it was not done then: issuing is in order, so a wait holds up what comes after it, 150 cycles and more even
-        // when there is nothing to wait for.  (670 cycles a step and tile, which is its products' time; with the loop inside an
+        // when there is nothing to wait for.  (Products alone 670 cycles a step and tile, their own time; with the loop inside an
         // "if (lane == 0)" 1000 and more, each descriptor being moved between register files, with four waits a step 1000.)
         const int un = __shfl_sync(0xffffffffu, n, 0), un0 = __shfl_sync(0xffffffffu, n0, 0), un1 = __shfl_sync(0xffffffffu, n1, 0);
         const int ujc = __shfl_sync(0xffffffffu, jc, 0);
