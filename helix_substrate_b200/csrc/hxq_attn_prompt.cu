@@ -60,6 +60,7 @@ constexpr int BM = 128;                     // rows of a tile
 constexpr int BN = 64;                      // keys of a step
 constexpr int kMaxStages = 8;
 constexpr int kBarBytes = 768;
+constexpr int kSorted = 128;                // sequences whose items stand in order of their work
 constexpr int kMany = 4 * 148;              // items of two tiles from which on the tiles stay together
 constexpr int kShare = 8;                   // key tiles that a CTA of a shared item has at least
 constexpr int kPolyOf4 = 1;                 // of four pairs of weights, how many are made on the multiply-add units
@@ -128,7 +129,9 @@ __device__ __forceinline__ Share find_share(const Args& a, int lq, int keys, int
 }
 // Item i: a CTA's tokens (from ct * rows on) of one sequence and KV head.  The items of all sequences stand in a row by
 // falling ct, the longest work (of causal attention) first, with no gaps for sequences that are shorter than others.
-// A warp finds the item: F(c), the number of items with ct >= c of one head, falls in c.
+// A warp finds the item: F(c), the number of items with ct >= c of one head, falls in c.  (kSorted sequences at most: the lanes hold
+// their lengths.)  Of more, sequence s has the places from first_row / rows + s on, enough for its items and its last one first;
+// thirty-two sequences are looked at at a time.
 __device__ __forceinline__ bool find_item(const Args& a, int i, Seq& q, int& s, int& ct, int& kvh) {
     const int lane = threadIdx.x & 31;
     kvh = i % a.nkv;
@@ -143,7 +146,24 @@ __device__ __forceinline__ bool find_item(const Args& a, int i, Seq& q, int& s, 
         ct = items(q.lq) - 1 - i;
         return ct >= 0;
     }
-    constexpr int HELD = 4;     // sequences a lane keeps (their loads run together); more are read again
+    if (a.S > kSorted) {
+        auto place = [&](int s) {
+            const int q0 = a.cu_q[s];
+            return (q0 < 0 ? 0 : (q0 > a.Tq ? a.Tq : q0)) / a.rows + s;
+        };
+        int lo = 0, hi = a.S;           // place(lo) <= i < place(hi)
+        while (hi - lo > 1) {
+            const int by = (hi - lo + 31) / 32, at = lo + (lane + 1) * by;
+            const int n = __popc(__ballot_sync(0xffffffffu, at < hi && place(at) <= i));
+            lo += n * by;
+            hi = lo + by < hi ? lo + by : hi;
+        }
+        s = lo;
+        q = sequence(a, lo);
+        ct = items(q.lq) - 1 - (i - place(lo));
+        return ct >= 0;
+    }
+    constexpr int HELD = kSorted / 32;      // (loads that run together)
     int held[HELD];
 #pragma unroll
     for (int b = 0; b < HELD; ++b) held[b] = 32 * b < a.S ? items(sequence(a, 32 * b + lane).lq) : 0;
@@ -151,10 +171,6 @@ __device__ __forceinline__ bool find_item(const Args& a, int i, Seq& q, int& s, 
         int sum = 0;
 #pragma unroll
         for (int b = 0; b < HELD; ++b) sum += held[b] > c ? held[b] - c : 0;
-        for (int b = 32 * HELD; b < a.S; b += 32) {
-            const int n = items(sequence(a, b + lane).lq);
-            sum += n > c ? n - c : 0;
-        }
         return __reduce_add_sync(0xffffffffu, sum);
     };
     if (from(0) <= i) return false;
@@ -873,7 +889,7 @@ static bool make_plan(const hxq_attn* p, Plan& plan) {
     plan.splits = room > 1 && steps > plan.alone ? (int)(parts < room ? parts : room) : 1;
     plan.rows = plan.splits > 1 || all >= kMany ? 2 * plan.tpg : plan.tpg;
     const int64_t n_ct = (max_q + plan.rows - 1) / plan.rows;
-    const int64_t some = (int64_t)p->Tq / plan.rows + p->S, most = n_ct * p->S, n = (some < most ? some : most) * p->nkv;
+    const int64_t some = (int64_t)p->Tq / plan.rows + p->S, most = n_ct * p->S, n = (some < most || p->S > kSorted ? some : most) * p->nkv;
     plan.n_ct = (int)n_ct;
     plan.items = (int)n;
     plan.groups = max_q > plan.tpg ? 8 : (int)((max_q * (p->nq / p->nkv) + 31) / 32);
@@ -922,7 +938,7 @@ static int run_tiles(const hxq_attn* p, const Plan& plan, void* workspace, int32
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return HXQ_E_DEVICE;
     if (!attr_set[dev]) {
         cudaFuncAttributes fa;        // the warps' exchange of registers counts on what the launch brings
-        if (cudaFuncGetAttributes(&fa, attn_prompt_kernel<DP, TILES>) != cudaSuccess || fa.numRegs < Z::kRegsLaunch) return HXQ_E_DEVICE;
+        if (cudaFuncGetAttributes(&fa, attn_prompt_kernel<DP, TILES>) != cudaSuccess || (fa.numRegs + 7) / 8 * 8 < Z::kRegsLaunch) return HXQ_E_DEVICE;
         if (cudaFuncSetAttribute(attn_prompt_kernel<DP, TILES>, cudaFuncAttributeMaxDynamicSharedMemorySize, Z::kSmem) != cudaSuccess) return HXQ_E_DEVICE;
         attr_set[dev] = true;
     }

@@ -315,12 +315,13 @@ def test_many_tiles(nq, nkv, D):
             assert torch.equal(alone.view(torch.int16), out[a:b].view(torch.int16)), (causal, a, b)
 
 
-def test_hundreds_of_sequences():
-    """More sequences than a warp's lanes hold at once, most of them short, one long, some empty."""
+@pytest.mark.parametrize("n", [31, 33, 128, 129, 1000, 3000])
+def test_many_sequences(n):
+    """Around the numbers that a warp's lanes hold, most of them short, one long, some empty."""
     from helix_substrate_b200.prompt_ops import attn_prompt
     dev, nq, nkv, D = _dev(), 6, 2, 64
-    lens = [(7 * s) % 23 for s in range(300)]
-    lens[170] = 500
+    lens = [(7 * s) % 23 for s in range(n)]
+    lens[n * 4 // 7] = 500
     T = sum(lens)
     g = torch.Generator(device=dev).manual_seed(3)
     q, k, v = (torch.randn(T, n, D, device=dev, generator=g).bfloat16() for n in (nq, nkv, nkv))
@@ -329,3 +330,43 @@ def test_hundreds_of_sequences():
     attn_prompt(q, k, v, out, torch.tensor(cu, dtype=torch.int32, device=dev), max(lens), 0.125)
     want = torch.cat([_want(q[a:b], k[a:b], v[a:b], 0.125, True) for a, b in zip(cu, cu[1:]) if b > a])
     _compare(out, want, "all")
+
+
+def test_one_slab_seen_by_all():
+    """Five sequences over the same 300 rows (a slab expanded, no copy), one query head's keys for both KV heads, outputs over the queries."""
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, S, n, D = _dev(), 5, 300, 64
+    g = torch.Generator(device=dev).manual_seed(8)
+    q = torch.randn(S * 7, 8, D, device=dev, generator=g).bfloat16()
+    k, v = (torch.randn(1, 1, n, D, device=dev, generator=g).bfloat16().expand(S, 2, n, D) for _ in range(2))
+    cu, k_len = torch.arange(S + 1, device=dev, dtype=torch.int32) * 7, torch.full((S,), n, device=dev)
+    want = torch.cat([_want(q[7 * s: 7 * s + 7], k[s].transpose(0, 1), v[s].transpose(0, 1), 0.1, True) for s in range(S)])
+    attn_prompt(q, k, v, q, cu, 7, 0.1, k_len=k_len)
+    _compare(q, want, "in place")
+
+
+def test_two_streams_at_once():
+    """Whole items and shared ones on two streams, again and again: the bits of a call alone."""
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, T = _dev(), 2000
+    g = torch.Generator(device=dev).manual_seed(9)
+    q, k, v = (torch.randn(T, n, 128, device=dev, generator=g).bfloat16() for n in (14, 2, 2))
+    kc = torch.randn(1, 2, 9000, 128, device=dev, generator=g).bfloat16()
+    cu, few, k_len = torch.tensor([0, T], dtype=torch.int32, device=dev), torch.tensor([0, 16], dtype=torch.int32, device=dev), torch.tensor([9000], device=dev)
+
+    def both():
+        a, b = torch.empty_like(q), torch.empty_like(q[:16])
+        attn_prompt(q, k, v, a, cu, T, 0.1)
+        attn_prompt(q[:16], kc, kc, b, few, 16, 0.1, k_len=k_len)
+        return a, b
+
+    want = both()
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append(both())
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for pair in got for x, y in zip(pair, want))
