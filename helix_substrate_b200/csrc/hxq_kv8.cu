@@ -297,12 +297,30 @@ __global__ void __launch_bounds__(kAppendThreads, STEP ? 1 : 2) append_kernel(co
         if (n == 0) return;
         blk = first = last = (int)(p0 / kBlock);
     } else {
-        int at = s, before = 0;
-        s = -1;
-        for (int s0 = 0; s0 < a.S && s < 0; s0 += 32) {
+        const int at = s;
+        if (a.S > 32) {
+            // Sequence s has the places from cu[s] / 64 + 2 s on, enough wherever its rows start.  Thirty-two are looked at at a time.
+            auto place = [&](int i) {
+                const int r0 = a.cu[i];
+                return (r0 < 0 ? 0 : (r0 > a.T ? a.T : r0)) / kBlock + 2 * i;
+            };
+            int lo = 0, hi = a.S;       // place(lo) <= at < place(hi)
+            while (hi - lo > 1) {
+                const int by = (hi - lo + 31) / 32, i = lo + (lane + 1) * by;
+                lo += __popc(__ballot_sync(0xffffffffu, i < hi && place(i) <= at)) * by;
+                hi = lo + by < hi ? lo + by : hi;
+            }
+            s = lo;
+            n = sequence(a, s, row0, p0);
+            if (n == 0) return;
+            first = (int)(p0 / kBlock);
+            last = (int)((p0 + n - 1) / kBlock);
+            blk = first + at - place(s);
+            if (blk > last) return;
+        } else {
             int rows = 0, r0 = 0, f = 0, l = -1;
             int64_t p = 0;
-            if (s0 + lane < a.S) rows = sequence(a, s0 + lane, r0, p);
+            if (lane < a.S) rows = sequence(a, lane, r0, p);
             if (rows > 0) { f = (int)(p / kBlock); l = (int)((p + rows - 1) / kBlock); }
             int incl = l - f + 1;
 #pragma unroll
@@ -310,20 +328,16 @@ __global__ void __launch_bounds__(kAppendThreads, STEP ? 1 : 2) append_kernel(co
                 const int v = __shfl_up_sync(0xffffffffu, incl, o);
                 if (lane >= o) incl += v;
             }
-            const uint32_t hit = __ballot_sync(0xffffffffu, before + incl > at);
-            if (hit != 0u) {
-                const int k = __ffs(hit) - 1;
-                s = s0 + k;
-                n = __shfl_sync(0xffffffffu, rows, k);
-                row0 = __shfl_sync(0xffffffffu, r0, k);
-                p0 = __shfl_sync(0xffffffffu, p, k);
-                first = __shfl_sync(0xffffffffu, f, k);
-                last = __shfl_sync(0xffffffffu, l, k);
-                blk = first + at - (before + __shfl_sync(0xffffffffu, incl - (l - f + 1), k));
-            }
-            before += __shfl_sync(0xffffffffu, incl, 31);
+            const uint32_t hit = __ballot_sync(0xffffffffu, incl > at);
+            if (hit == 0u) return;
+            s = __ffs(hit) - 1;
+            n = __shfl_sync(0xffffffffu, rows, s);
+            row0 = __shfl_sync(0xffffffffu, r0, s);
+            p0 = __shfl_sync(0xffffffffu, p, s);
+            first = __shfl_sync(0xffffffffu, f, s);
+            last = __shfl_sync(0xffffffffu, l, s);
+            blk = first + at - __shfl_sync(0xffffffffu, incl - (l - f + 1), s);
         }
-        if (s < 0) return;
     }
     if (role < roles - 2 * a.c.nkv) {
         if (STEP) {

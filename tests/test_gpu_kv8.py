@@ -83,16 +83,17 @@ def test_append_prompts_in_pieces(nq, nkv, D):
         _check_cache(cache, ref)
 
 
-def test_append_of_many_packed_prompts():
+@pytest.mark.parametrize("S", [75, 32, 33, 1100])
+def test_append_of_many_packed_prompts(S):
     """More sequences than a warp has lanes, most of them short or empty, one long: every block finds its CTA."""
     from helix_substrate_b200.kv8 import Kv8Cache, rope_append_prompt_kv8
-    dev, S, nq, nkv, D, max_len = _dev(), 75, 5, 1, 112, 1024
+    dev, nq, nkv, D, max_len = _dev(), 5, 1, 112, 1024
     g = torch.Generator().manual_seed(8)
     cache, ref = Kv8Cache.empty(S, nkv, max_len, D, dev), RefCache(S, nkv, D)
     cos, sin = tables(max_len, D, "cpu")
     for turn in range(2):
         lens = [int(x) for x in torch.randint(0, 30, (S,), generator=g)]
-        lens[3], lens[40], lens[74] = 500, 0, 64
+        lens[3], lens[20], lens[S - 1] = 500, 0, 64
         pos = [ref.length(s) for s in range(S)]
         cu = [sum(lens[:s]) for s in range(S + 1)]
         qkv = torch.randn(cu[-1], (nq + 2 * nkv) * D, generator=g).bfloat16()
