@@ -30,7 +30,7 @@
 // TFLOP/s), 1.80 in one of a second, at the 1.6 GHz that the power limit leaves.
 //
 // A CTA's start (finding its tokens 1 to 2 us, first loads and scores 1.3) and end (V's edge 0.7, outputs by way of shared memory
-// 2.5) cost as much as seven steps; of 2048 tokens and less they are half of the time.
+// 1.7) cost as much as six steps; of 2048 tokens and less they are half of the time.
 //
 // The reference point m moves only when the maximum has grown by more than 2^8: weights stay below 256, nothing
 // overflows, the result is the same, and O is rarely rescaled.
@@ -785,12 +785,20 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 __syncwarp();
                 constexpr int PER = DP / 8, AT_ONCE = 32 / PER;     // lanes to a row, rows to a store
                 const int64_t mine = live ? dst - a.out : -1;
-#pragma unroll 8
-                for (int i = 0; i < PER; ++i) {
-                    const int from = i * AT_ONCE + lane / PER, c = lane % PER;
-                    const int64_t off = __shfl_sync(0xffffffffu, mine, from);
-                    const uint4 w = *reinterpret_cast<const uint4*>(stage + from * (DP * 2) + (c ^ (from & 7)) * 16);
-                    if (off >= 0 && 8 * c < a.D) *reinterpret_cast<uint4*>(a.out + off + 8 * c) = w;
+#pragma unroll 1
+                for (int i0 = 0; i0 < PER; i0 += 8) {       // (all eight read before the first is written: nothing says that they differ)
+                    uint4 w[8];
+                    int64_t off[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int from = (i0 + i) * AT_ONCE + lane / PER, c = lane % PER;
+                        off[i] = __shfl_sync(0xffffffffu, mine, from);
+                        if (8 * c >= a.D) off[i] = -1;
+                        w[i] = *reinterpret_cast<const uint4*>(stage + from * (DP * 2) + (c ^ (from & 7)) * 16);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (off[i] >= 0) *reinterpret_cast<uint4*>(a.out + off[i] + 8 * (lane % PER)) = w[i];
                 }
             }
         }
