@@ -33,21 +33,22 @@ def _call(dev: torch.device, name: str, *args) -> None:
 
 
 def _rows(t: torch.Tensor, name: str, dev: torch.device, width: int) -> None:
-    if not (t.dtype is torch.bfloat16 and t.device == dev and t.ndim == 2 and t.stride(1) == 1 and t.shape[1] == width):
+    if not (t.dtype is torch.bfloat16 and t.device == dev and t.shape[1:] == (width,) and t.stride()[1] == 1):
         raise TypeError(f"{name}: expected a bf16 [rows, {width}] tensor on {dev}, contiguous along its rows, got "
                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def _ints(t: torch.Tensor, name: str, dev: torch.device, dtype: torch.dtype, n: int) -> None:
-    if not (t.dtype is dtype and t.device == dev and t.ndim == 1 and t.shape[0] == n and t.is_contiguous()):
+    if not (t.dtype is dtype and t.device == dev and t.shape == (n,) and t.is_contiguous()):
         raise TypeError(f"{name}: expected a contiguous {dtype} tensor of {n} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def _positions(t: torch.Tensor, name: str, dev: torch.device, n: int) -> int:
     """Checks int64 positions, one per sequence or one for all; returns their stride."""
-    if not (t.dtype is torch.int64 and t.device == dev and t.ndim == 1 and t.shape[0] in (1, n) and t.is_contiguous()):
+    shape = t.shape
+    if not (t.dtype is torch.int64 and t.device == dev and (shape == (n,) or shape == (1,)) and t.is_contiguous()):
         raise TypeError(f"{name}: expected a contiguous int64 tensor of 1 or {n} on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return int(t.shape[0] == n and n > 1)
+    return int(n > 1 and shape[0] == n)
 
 
 class Kv8Cache:
@@ -103,8 +104,8 @@ class Kv8Cache:
 
 def _tables(cos: torch.Tensor, sin: torch.Tensor, cache: Kv8Cache) -> None:
     for name, t in (("cos", cos), ("sin", sin)):
-        if not (t.dtype is torch.float32 and t.device == cache.device and t.ndim == 2 and t.shape[1] == cache.D
-                and t.shape[0] >= cache.max_len and t.is_contiguous()):
+        if not (t.dtype is torch.float32 and t.device == cache.device and t.shape[1:] == (cache.D,) and t.shape[0] >= cache.max_len
+                and t.is_contiguous()):
             raise TypeError(f"{name}: expected a contiguous fp32 [{cache.max_len} or more, {cache.D}] table on {cache.device}, got "
                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
 
@@ -189,18 +190,18 @@ def kv8_rows(cache: Kv8Cache, length: torch.Tensor, k_out: torch.Tensor, v_out: 
     """Rows 0 .. length - 1 of every slot as bf16, scale * code rounded once, into k_out and v_out [S, kv_heads,
     rows, D] (any strides over the first three); at most ``rows`` of them, the rest of the outputs is left as it is.
     ``length`` int64 on the device, one per sequence or one for all: how many positions each slot holds."""
-    dev = cache.device
-    S = k_out.shape[0]
+    dev, shape, strides = cache.device, k_out.shape, k_out.stride()
     for name, t in (("k_out", k_out), ("v_out", v_out)):
-        if not (t.dtype is torch.bfloat16 and t.device == dev and t.ndim == 4 and t.shape[1] == cache.kv_heads and t.shape[3] == cache.D
-                and t.stride(3) == 1 and t.shape == k_out.shape and t.stride() == k_out.stride()):
+        if not (t.dtype is torch.bfloat16 and t.device == dev and t.shape == shape and t.stride() == strides and len(shape) == 4
+                and shape[1] == cache.kv_heads and shape[3] == cache.D and strides[3] == 1):
             raise TypeError(f"{name}: expected a bf16 [slots, {cache.kv_heads}, rows, {cache.D}] tensor on {dev}, contiguous along D, both "
                             f"outputs alike, got {t.dtype} {tuple(t.shape)} {t.stride()} on {t.device}")
+    S = shape[0]
     if not 1 <= S <= cache.slots:
         raise ValueError(f"outputs of {S} sequences, {cache.slots} slots")
     stride = _positions(length, "length", dev, S)
-    if k_out.shape[2] == 0:
+    if shape[2] == 0:
         return k_out, v_out
-    _call(dev, "hxq_kv8_rows", cache._ref, length.data_ptr(), stride, S, k_out.shape[2], k_out.data_ptr(), v_out.data_ptr(),
-          k_out.stride(0), k_out.stride(1), k_out.stride(2))
+    _call(dev, "hxq_kv8_rows", cache._ref, length.data_ptr(), stride, S, shape[2], k_out.data_ptr(), v_out.data_ptr(), strides[0], strides[1],
+          strides[2])
     return k_out, v_out
