@@ -117,9 +117,9 @@ def lib() -> C.CDLL:
                                   C.c_void_p, C.c_size_t, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                   C.c_float, C.c_void_p]
     L.hxq_attn_prompt.restype = C.c_int
-    L.hxq_attn_prompt.argtypes = [C.POINTER(HxqAttn), C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]
+    L.hxq_attn_prompt.argtypes = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]       # (HxqAttn, or its bytes)
     L.hxq_attn_prompt_workspace_bytes.restype = C.c_size_t
-    L.hxq_attn_prompt_workspace_bytes.argtypes = [C.POINTER(HxqAttn)]
+    L.hxq_attn_prompt_workspace_bytes.argtypes = [C.c_void_p]
     K = C.POINTER(HxqKv8)
     L.hxq_rope_append_kv8.restype = C.c_int
     L.hxq_rope_append_kv8.argtypes = [K, C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
