@@ -126,6 +126,6 @@ def test_decoder_refuses():
     with pytest.raises(ValueError, match="kv_bits"):
         _pair(kv_bits=4)
     with pytest.raises(ValueError, match="prompt_attn"):
-        _pair(prompt_attn="flash")
+        _pair(prompt_attn="other")
     with pytest.raises(ValueError, match="8-bit"):
         _pair(kv_bits=8).make_graphed_step(2, fused=False)
