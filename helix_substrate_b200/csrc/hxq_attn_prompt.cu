@@ -26,8 +26,8 @@
 // scores are there when a warp comes for them.  (Products of 64 keys cost a third more, 670 cycles a step and tile instead of 512: a
 // Q tile is read from shared memory for half the work.  With 128 keys a step and one buffer, S of the next waiting for P V of
 // this one, a step took 3900 cycles, its products 2048.)  Both tiles' 64 keys take 1530 to 1750 cycles, their products 1345; a
-// tile by itself takes 1241, its softmax's latency.  16384 tokens of 28 + 4 heads of 128 take 1.54 ms in a short run (1250
-// TFLOP/s), 1.80 in one of a second, at the 1.6 GHz that the power limit leaves.
+// tile by itself takes 1241, its softmax's latency.  16384 tokens of 28 + 4 heads of 128 take 1.51 ms in a short run (1270
+// TFLOP/s), 1.76 in one of a second, at the 1.6 GHz that the power limit leaves.
 //
 // A CTA's start (finding its tokens 1 to 2 us, first loads and scores 1.3) and end (V's edge 0.7, outputs by way of shared memory
 // 1.7) cost as much as six steps; of 2048 tokens and less they are half of the time.
