@@ -752,7 +752,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                     tmem_ld_wait(r);
                 }
 #pragma unroll
-                for (int e = 0; e < 32; ++e) r[e] = nx == 0 || l == 0.f ? 0u : __float_as_uint(__uint_as_float(r[e]) * inv);
+                for (int e = 0; e < 32; ++e) r[e] = cnt <= 0 ? 0u : __float_as_uint(__uint_as_float(r[e]) * inv);     // (scores of -inf alone: NaN)
                 if (odd && live) {      // infinities and NaNs that were taken out of V, back to the rows that see them
                     const __nv_bfloat16* vp = a.v + (a.cu_k != nullptr ? 0 : (int64_t)job[5] * a.v_seq) + (int64_t)head * a.v_head + (int64_t)k0 * a.v_row;
                     for (int kk = seen_by_all; kk < cnt; ++kk)
@@ -871,9 +871,10 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a) {
         y0 += w * meet[p][2 + 2 * warp][lane];
         y1 += w * meet[p][3 + 2 * warp][lane];
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const bool none = reach(a, seq.lq, seq.lk, first + in / a.G) == 0;
+    const float inv = 1.f / sum;
     __nv_bfloat16* dst = a.out + (int64_t)(seq.q0 + first + in / a.G) * a.o_tok + (int64_t)(kvh * a.G + in % a.G) * a.o_head + d + 2 * warp;
-    *reinterpret_cast<uint32_t*>(dst) = sum == 0.f ? 0u : bf2(y0 * inv, y1 * inv);
+    *reinterpret_cast<uint32_t*>(dst) = none ? 0u : bf2(y0 * inv, y1 * inv);
 }
 
 // ---- host side ---------------------------------------------------------------------

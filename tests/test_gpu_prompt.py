@@ -370,3 +370,23 @@ def test_two_streams_at_once():
                 got.append(both())
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for pair in got for x, y in zip(pair, want))
+
+
+@pytest.mark.parametrize("lens,keys", [([40], [40]), ([6], [3006])])
+def test_scores_of_minus_infinity(lens, keys):
+    """A key whose scores are -inf has no weight; a row that sees such keys alone is NaN, as 0 / 0 is; keys whole and in shares."""
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, nq, nkv, D, T, n = _dev(), 4, 2, 64, lens[0], keys[0]
+    g = torch.Generator(device=dev).manual_seed(n)
+    q = torch.rand(T, nq, D, device=dev, generator=g).bfloat16() + 0.5
+    kc, vc = (torch.randn(1, nkv, n, D, device=dev, generator=g).bfloat16() for _ in range(2))
+    kc[0, 0, : n - T + 1, 5] = float("-inf")          # all that the first query sees, in one head
+    kc[0, 1, n - 3, 5] = float("-inf")
+    cu, k_len = torch.tensor([0, T], dtype=torch.int32, device=dev), torch.tensor([n], device=dev)
+    out = torch.empty(T, nq, D, device=dev, dtype=torch.bfloat16)
+    attn_prompt(q, kc, vc, out, cu, T, 0.1, k_len=k_len)
+    s = torch.einsum("thd,hkd->htk", q.double(), kc[0].double().repeat_interleave(nq // nkv, 0)) * 0.1
+    s = s.masked_fill(~torch.ones(T, n, device=dev).tril(n - T).bool(), float("-inf"))
+    want = torch.einsum("htk,hkd->thd", s.softmax(-1), vc[0].double().repeat_interleave(nq // nkv, 0))
+    assert bool(want[0, :2].isnan().all()) and int(want.isnan().sum()) == 2 * D
+    _compare(out, want, "-inf")
