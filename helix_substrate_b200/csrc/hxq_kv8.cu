@@ -77,7 +77,7 @@ __device__ __forceinline__ uint4 ld16(const void* p) { return *reinterpret_cast<
 // on.  Nearly always fp32 tells the same: r = fma(x, cos, fl(y sin)) is off by 2^-24 (|y sin| + |r|) at most and the
 // true sum's fp32 value by one more rounding, so where r - d and r + d, d = 2^-23 (|y sin| + |r|), round to the same bf16, that is
 // it.  One value in some 2^13 takes the 64-bit path.  (All in 64 bits, conversions alone filled half of the time: 86 us for 8191
-// tokens of 28 + 4 heads, 41 as it is; exact sums of products and their rests in packed fp32 took 42 to 48.)
+// tokens of 28 + 4 heads where this takes 41; exact sums of products and their rests in packed fp32 took 42 to 48.)
 __device__ __forceinline__ uint32_t turn(float x, float c, float y, float s, bool& sure) {
     const float p = y * s, r = fmaf(x, c, p);
     const float d = fmaf(fabsf(p) + fabsf(r), 1.0001f * 1.1920929e-7f, 2.8e-45f);
@@ -141,12 +141,12 @@ struct AppendArgs {
     const float *cos_t, *sin_t;
     __nv_bfloat16 *q_out, *k_out;
     int64_t ld_qkv, ld_q, ld_k;
-    int pos_stride, T, S, max_q, nq, groups;        // groups: of kHeadsEach query heads
+    int pos_stride, T, S, max_q, nq, groups;        // groups: of kHeadsPrompt or kHeadsStep query heads
 };
 
 constexpr int kAppendThreads = 256;
 constexpr int kMaxD = 128;
-constexpr int kHeadsEach = 4;       // query heads of a thread
+constexpr int kHeadsPrompt = 4, kHeadsStep = 2;       // query heads of a thread: few for a single token, whose time is one thread's
 constexpr int kUnits = 4 * kMaxD / kAppendThreads;      // pairs of eight-element pieces a thread holds of a block
 
 // Sequence s: its first row of qkv, the number of its new rows that have a place in the cache, its first position.
@@ -256,13 +256,14 @@ __device__ void append_block(const AppendArgs& a, bool is_k, int s, int h, int b
     }
 }
 
-// The query heads h0, h0 + groups, ... (up to kHeadsEach) of one row, the pieces at d and d + D / 2, under one set of angles.
+// The query heads h0, h0 + groups, ... (up to HEADS) of one row, the pieces at d and d + D / 2, under one set of angles.
+template <int HEADS>
 __device__ __forceinline__ void turn_queries(const AppendArgs& a, int64_t t, int64_t p, int h0, int d) {
     const int D = a.c.D, half = D >> 1;
     const __nv_bfloat16* src = a.qkv + t * a.ld_qkv + h0 * D + d;
-    uint4 lo[kHeadsEach], hi[kHeadsEach];
+    uint4 lo[HEADS], hi[HEADS];
 #pragma unroll
-    for (int k = 0; k < kHeadsEach; ++k)
+    for (int k = 0; k < HEADS; ++k)
         if (h0 + k * a.groups < a.nq) {
             lo[k] = ld16(src + k * a.groups * D);
             hi[k] = ld16(src + k * a.groups * D + half);
@@ -270,7 +271,7 @@ __device__ __forceinline__ void turn_queries(const AppendArgs& a, int64_t t, int
     const Angles angles(a.cos_t + p * D, a.sin_t + p * D, d, half);
     __nv_bfloat16* dst = a.q_out + t * a.ld_q + h0 * D + d;
 #pragma unroll
-    for (int k = 0; k < kHeadsEach; ++k)
+    for (int k = 0; k < HEADS; ++k)
         if (h0 + k * a.groups < a.nq) {
             rotate16(lo[k], hi[k], angles);
             *reinterpret_cast<uint4*>(dst + k * a.groups * D) = lo[k];
@@ -282,8 +283,10 @@ __device__ __forceinline__ void turn_queries(const AppendArgs& a, int64_t t, int
 // STEP: one token a sequence, the CTA's block being the token's; a CTA for all query heads.
 // Else the blocks that the sequences' new rows touch stand in a row, and every warp works out for itself where its CTA's lies.
 // Bound by HBM for prompts (and by instructions nearly as much), by one memory round trip and the launch for single tokens.
+// 8191 tokens of 28 + 4 heads: 36 us with three CTAs an SM and 4 heads a thread (a few registers spilled), 41 with two, 43 with four, 38
+// with 3 or 5 heads.  32 single tokens: 3.2 us with 2 heads a thread, 4.7 with 4.
 template <bool STEP>
-__global__ void __launch_bounds__(kAppendThreads, STEP ? 1 : 2) append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, STEP ? 1 : 3) append_kernel(const AppendArgs a) {
     __shared__ uint32_t red[kAppendThreads / 32];
     pdl_enter();
     const int D = a.c.D, pieces = D >> 4, lane = threadIdx.x & 31;
@@ -341,10 +344,10 @@ __global__ void __launch_bounds__(kAppendThreads, STEP ? 1 : 2) append_kernel(co
     }
     if (role < roles - 2 * a.c.nkv) {
         if (STEP) {
-            for (int u = threadIdx.x; u < a.groups * pieces; u += kAppendThreads) turn_queries(a, row0, p0, u / pieces, (u % pieces) * 8);
+            for (int u = threadIdx.x; u < a.groups * pieces; u += kAppendThreads) turn_queries<kHeadsStep>(a, row0, p0, u / pieces, (u % pieces) * 8);
         } else {
             const int64_t p = (int64_t)blk * kBlock + (role % parts) * (kBlock / parts) + threadIdx.x / pieces;
-            if ((int)threadIdx.x < kBlock / parts * pieces && p >= p0 && p < p0 + n) turn_queries(a, row0 + (p - p0), p, role / parts, (threadIdx.x % pieces) * 8);
+            if ((int)threadIdx.x < kBlock / parts * pieces && p >= p0 && p < p0 + n) turn_queries<kHeadsPrompt>(a, row0 + (p - p0), p, role / parts, (threadIdx.x % pieces) * 8);
         }
         return;
     }
@@ -1088,7 +1091,7 @@ static int run_append(const hxq_kv8* c, const void* qkv, int64_t ld_qkv, int32_t
     a.ld_qkv = ld_qkv; a.ld_q = ld_q; a.ld_k = ld_k;
     a.pos_stride = pos_stride; a.T = T; a.S = S; a.nq = nq;
     a.max_q = max_q < c->max_len ? max_q : c->max_len;
-    a.groups = (nq + kHeadsEach - 1) / kHeadsEach;
+    a.groups = cu ? (nq + kHeadsPrompt - 1) / kHeadsPrompt : (nq + kHeadsStep - 1) / kHeadsStep;
     // blocks that n rows touch: n / 64 and up to two more, wherever they start
     const int64_t blocks = cu ? (int64_t)T / kBlock + 2 * (int64_t)S : S, grid = blocks * ((cu ? a.groups * ((kBlock * (c->D / 16) + kAppendThreads - 1) / kAppendThreads) : 1) + 2 * c->nkv);
     if (grid > 0x7fffffffLL) return HXQ_E_SHAPE;
