@@ -16,18 +16,21 @@ from ._lib import HxqKv8
 BLOCK = 64      # positions that share one scale
 
 
-def _raw_stream(dev: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(dev.index)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_entries: dict = {}
 
 
 def _call(dev: torch.device, name: str, *args) -> None:
     """One C call on the current stream of ``dev`` (appended as its last argument), ``dev`` being current."""
-    f = getattr(_lib.lib(), name)
-    if torch.cuda.current_device() == dev.index:
-        st = f(*args, _raw_stream(dev))
+    f = _entries.get(name)
+    if f is None:
+        f = _entries[name] = getattr(_lib.lib(), name)
+    index = dev.index
+    if torch._C._cuda_getDevice() == index:
+        st = f(*args, _raw_stream(index))
     else:
         with torch.cuda.device(dev):
-            st = f(*args, _raw_stream(dev))
+            st = f(*args, _raw_stream(index))
     if st != _lib.HXQ_OK:
         _lib.check(st, name)
 
