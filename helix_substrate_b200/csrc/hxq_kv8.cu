@@ -486,31 +486,47 @@ __device__ __forceinline__ Share find(const DecodeArgs& a, int cta, int at, int6
     auto units = [&](int b) { return b < a.B ? units_of(a.pos[(int64_t)b * a.pos_stride], a.c.max_len) : 0; };
     Share r;
     const int first = units(lane);
-    int64_t sum = __reduce_add_sync(0xffffffffu, padded(first));
-    for (int b0 = 32; b0 < a.B; b0 += 32) sum += __reduce_add_sync(0xffffffffu, padded(units(b0 + lane)));
-    total = sum * a.c.nkv;
+    int sum = padded(first), pre = lane < at ? sum : 0;         // (what a cache can hold of units stays far below 2^31)
+#pragma unroll 4
+    for (int b = lane + 32; b < a.B; b += 32) {
+        const int u = padded(units(b));
+        sum += u;
+        pre += b < at ? u : 0;
+    }
+    total = (int64_t)__reduce_add_sync(0xffffffffu, sum) * a.c.nkv;
     r.per = (total + a.ctas - 1) / a.ctas;
     if (r.per < kWarps) r.per = kWarps;       // a unit for each warp at least
-    const int64_t place = r.per * cta;
     r.b = -1; r.before = 0; r.units = 0;
-    if (at < 0 && place >= total) return r;
+    if (at >= 0) {
+        r.b = at;
+        r.before = __reduce_add_sync(0xffffffffu, pre);
+        r.units = units(at);
+        return r;
+    }
+    const int64_t place = r.per * cta;
+    if (place >= total) return r;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
         const int u = b0 == 0 ? first : units(b0 + lane);
         int incl = padded(u);
+        if (b0 + 32 < a.B) {
+            const int all = __reduce_add_sync(0xffffffffu, incl);
+            if ((r.before + all) * a.c.nkv <= place) {
+                r.before += all;
+                continue;
+            }
+        }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += v;
         }
-        const uint32_t hit = at < 0 ? __ballot_sync(0xffffffffu, (r.before + incl) * a.c.nkv > place) : (at < b0 + 32 ? 1u << (at - b0) : 0u);
-        if (hit != 0u) {
-            const int l = __ffs(hit) - 1;
-            r.b = b0 + l;
-            r.units = __shfl_sync(0xffffffffu, u, l);
-            r.before += __shfl_sync(0xffffffffu, incl - padded(u), l);
-            return r;
-        }
-        r.before += __shfl_sync(0xffffffffu, incl, 31);
+        const uint32_t hit = __ballot_sync(0xffffffffu, (r.before + incl) * a.c.nkv > place);
+        if (hit == 0u) return r;        // (positions that change meanwhile)
+        const int l = __ffs(hit) - 1;
+        r.b = b0 + l;
+        r.units = __shfl_sync(0xffffffffu, u, l);
+        r.before += __shfl_sync(0xffffffffu, incl - padded(u), l);
+        return r;
     }
     return r;
 }
