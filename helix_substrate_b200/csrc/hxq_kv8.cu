@@ -466,6 +466,7 @@ struct DecodeArgs {
     float* part;            // [CTAs, 2, G, D + 2]: maximum, sum, un-normalised output
     int64_t ld_q, ld_out;
     int pos_stride, B, nq, G, ctas;
+    bool edges;             // more pairs than CTAs: see combine_kernel
     float scale_log2;       // scale * log2(e)
 };
 
@@ -585,6 +586,10 @@ __global__ void __launch_bounds__(32 * kWarps, kDecodeCtas) decode_kernel(const 
         flat = rank * per < units ? rank * per : units;
         flat_end = flat + per < units ? flat + per : units;
     } else {
+        if (a.edges)            // sequences with nothing to see: the joining launch does not come by
+            for (int i = blockIdx.x; i < a.B; i += gridDim.x)
+                if (units_of(a.pos[(int64_t)i * a.pos_stride], a.c.max_len) == 0)
+                    for (int d = threadIdx.x; d < a.nq * D; d += 32 * kWarps) a.out[(int64_t)i * a.ld_out + d] = __float2bfloat16_rn(0.f);
         int64_t total;
         const Share at = find(a, blockIdx.x, -1, total);
         if (at.b < 0) return;
@@ -978,19 +983,30 @@ __global__ void __launch_bounds__(32 * kWarps, kDecodeCtas) decode_kernel(const 
 // Joins the partial results of the pairs that more than one CTA had a segment of:
 // out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c; sequences with nothing to see get zeros.  kFew results are one round
 // trip to memory.  A long context has a hundred and more, and a large CTA.
+// With more pairs than CTAs (EDGES) there is a CTA for each place where a share starts instead, and the first in a pair joins it.
 // (32 sequences: 128 threads a CTA, so that all CTAs are there and have found their pairs when the last result is written, and
 // one round trip: 10 -> 3 us.)
 constexpr int kJoin = 8, kFew = 8, kHeld = 28;
 static_assert(kJoin * kMaxD >= kDecodeCtas * 148 + 1, "a thread to a result");
-__global__ void __launch_bounds__(kJoin * kMaxD) combine_kernel(const DecodeArgs a) {
+template <bool EDGES>
+__global__ void __launch_bounds__(EDGES ? kMaxD : kJoin * kMaxD) combine_kernel(const DecodeArgs a) {
     __shared__ float w_s[kDecodeCtas * 148 + 1], o_s[kJoin][kMaxD], red[2][kJoin * kMaxD / 32];
-    const int kvh = blockIdx.x, hd = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, D = a.c.D;
+    const int hd = blockIdx.y, tid = threadIdx.x, D = a.c.D;
+    int kvh = blockIdx.x, b = blockIdx.z;
     const int d = tid & (kMaxD - 1), j = tid / kMaxD, lane = tid & 31, warp = tid >> 5;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     int64_t total;
-    const Share at = find(a, 0, b, total);
-    const int64_t s = at.before * a.c.nkv + (int64_t)kvh * (at.units + kPad), e = s + at.units;
-    const int c0 = (int)(s / at.per), n = at.units == 0 ? 0 : (int)((e - 1) / at.per) - c0 + 1;
+    const Share at = EDGES ? find(a, blockIdx.x + 1, -1, total) : find(a, 0, b, total);
+    int64_t s = at.before * a.c.nkv;
+    if (EDGES) {
+        b = at.b;
+        kvh = b < 0 ? 0 : (int)((at.per * (blockIdx.x + 1) - s) / (at.units + kPad));
+    }
+    s += (int64_t)kvh * (at.units + kPad);
+    const int64_t e = s + at.units;
+    const int c0 = (int)(s / at.per);
+    int n = at.units == 0 ? 0 : (int)((e - 1) / at.per) - c0 + 1;
+    if (EDGES && (b < 0 || c0 != (int)blockIdx.x || n < 2)) n = 1;        // (c0 < the share that starts here <= the pair's last)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     __nv_bfloat16* out = a.out + (int64_t)b * a.ld_out + ((int64_t)kvh * a.G + hd) * D;
     if (n == 0) {
@@ -1224,12 +1240,14 @@ extern "C" int hxq_attn_decode_kv8(const hxq_kv8* cache, const void* q, int64_t 
     a.ld_q = ld_q; a.ld_out = ld_out;
     a.pos_stride = pos_stride; a.B = B; a.nq = nq; a.G = nq / cache->nkv;
     a.ctas = decode_ctas(B, cache->nkv, cache->max_len);
+    a.edges = (int64_t)B * cache->nkv > a.ctas && a.ctas > 1;
     a.scale_log2 = scale * 1.4426950408889634f;
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
     if (clustered) return run_decode<true>(a, stream) == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
     cudaError_t e = run_decode<false>(a, stream);
     // (about ctas / (B nkv) results a pair)
     const bool few = (int64_t)a.ctas <= (int64_t)B * cache->nkv * (kFew - 2);
-    if (e == cudaSuccess) e = launch_pdl(combine_kernel, dim3(cache->nkv, a.G, B), dim3(few ? kMaxD : kJoin * kMaxD), stream, 0, a);
+    if (e == cudaSuccess && a.edges) e = launch_pdl(combine_kernel<true>, dim3(a.ctas - 1, a.G), dim3(kMaxD), stream, 0, a);
+    else if (e == cudaSuccess) e = launch_pdl(combine_kernel<false>, dim3(cache->nkv, a.G, B), dim3(few ? kMaxD : kJoin * kMaxD), stream, 0, a);
     return e == cudaSuccess ? HXQ_OK : HXQ_E_LAUNCH;
 }

@@ -311,7 +311,7 @@ def test_attn_decode_kv8_values(case):
 
 
 @pytest.mark.parametrize("nq,nkv,D", [(4, 2, 64), (7, 1, 128), (2, 1, 112)])
-@pytest.mark.parametrize("B", [14, 33, 70, 130])
+@pytest.mark.parametrize("B", [14, 33, 70, 130, 300, 700])
 def test_attn_decode_kv8_many_sequences(nq, nkv, D, B):
     """More sequences than a warp has lanes, lengths from nothing to many blocks, idle slots in between and at both ends: every
     CTA finds its share; all at one position too."""
