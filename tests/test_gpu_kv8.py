@@ -449,3 +449,47 @@ def test_kv8_refuses_on_the_gpu():
         with pytest.raises(kind):
             call()
     assert rope_append_prompt_kv8(bf(0, 8 * D), i64(0, 0).int(), 5, i64(0), cos, sin, bf(0, nq * D), None, cache, nq).shape[0] == 0
+
+
+@pytest.mark.parametrize("B,max_len", [(500, 256), (40, 2048), (2, 32768)])
+def test_captured_attention_with_what_reads_it(B, max_len):
+    """Joined over borders between shares, over a few and over many results; idle slots among them; each call followed by a reader
+    that comes in early.  Replays leave the bits of calls one by one."""
+    from helix_substrate_b200.decode_ops import swiglu
+    from helix_substrate_b200.kv8 import Kv8Cache, attn_decode_kv8
+    dev, nq, nkv, D, N = _dev(), 4, 2, 64, 8
+    g = torch.Generator(device=dev).manual_seed(B)
+    cache = Kv8Cache.empty(B, nkv, max_len, D, dev)
+    for t in (cache.k, cache.v):
+        t.copy_(torch.randint(-127, 128, t.shape, device=dev, generator=g, dtype=torch.int8))
+    for t in (cache.k_scale, cache.v_scale):
+        t.uniform_(0.005, 0.02, generator=g)
+    for t in (cache.k_tail, cache.v_tail):
+        t.normal_(generator=g)
+    pos = torch.randint(-max_len // 16, max_len, (B,), device=dev, generator=g)
+    qs = [torch.randn(B, nq * D, device=dev, generator=g).bfloat16() for _ in range(N)]
+    gate = torch.full((B, nq * D), 20.0, device=dev, dtype=torch.bfloat16)
+    outs, reads = [torch.empty_like(q) for q in qs], [torch.empty_like(q) for q in qs]
+
+    def call(i, wait):
+        attn_decode_kv8(qs[i], cache, pos, outs[i], nq, 0.1)
+        if wait:
+            torch.cuda.synchronize()
+        swiglu(gate, outs[i], reads[i])
+
+    for i in range(N):
+        call(i, True)
+    assert not bool(outs[0][pos < 0].any()) and bool(outs[0][pos >= 0].any(1).all())
+    want = [t.clone() for t in outs + reads]
+    graph, st = torch.cuda.CUDAGraph(), torch.cuda.Stream(dev)
+    st.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(st), torch.cuda.graph(graph, stream=st):
+        for i in range(N):
+            call(i, False)
+    for _ in range(5):
+        for t in outs + reads:
+            t.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs + reads, want))

@@ -390,3 +390,37 @@ def test_scores_of_minus_infinity(lens, keys):
     want = torch.einsum("htk,hkd->thd", s.softmax(-1), vc[0].double().repeat_interleave(nq // nkv, 0))
     assert bool(want[0, :2].isnan().all()) and int(want.isnan().sum()) == 2 * D
     _compare(out, want, "-inf")
+
+
+def test_captured_with_what_reads_it():
+    """Calls that share their keys out, each followed by a reader that comes in early: replays leave the bits of calls one by one."""
+    from helix_substrate_b200.decode_ops import swiglu
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, nq, nkv, D, T, n, N = _dev(), 14, 2, 128, 12, 6000, 8
+    g = torch.Generator(device=dev).manual_seed(10)
+    k, v = (torch.randn(1, nkv, n, D, device=dev, generator=g).bfloat16() for _ in range(2))
+    qs = [torch.randn(T, nq, D, device=dev, generator=g).bfloat16() for _ in range(N)]
+    cu, k_len, gate = torch.tensor([0, T], dtype=torch.int32, device=dev), torch.tensor([n], device=dev), torch.full((T, nq * D), 20.0, device=dev, dtype=torch.bfloat16)
+    outs, reads = [torch.empty_like(q) for q in qs], [torch.empty_like(gate) for _ in qs]
+
+    def call(i, wait):
+        attn_prompt(qs[i], k, v, outs[i], cu, T, 0.1, k_len=k_len)
+        if wait:
+            torch.cuda.synchronize()
+        swiglu(gate, outs[i].view(T, -1), reads[i])
+
+    for i in range(N):
+        call(i, True)
+    want = [t.clone() for t in outs + reads]
+    graph, st = torch.cuda.CUDAGraph(), torch.cuda.Stream(dev)
+    st.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(st), torch.cuda.graph(graph, stream=st):
+        for i in range(N):
+            call(i, False)
+    for _ in range(5):
+        for t in outs + reads:
+            t.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs + reads, want))
