@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(kAppendThreads, STEP ? 1 : 3) append_kernel(co
             first = (int)(p0 / kBlock);
             last = (int)((p0 + n - 1) / kBlock);
             blk = first + at - place(s);
-            if (blk > last) return;
+            if (blk < first || blk > last) return;       // (below: a place before the first sequence's, where rows of no sequence precede it)
         } else {
             int rows = 0, r0 = 0, f = 0, l = -1;
             int64_t p = 0;

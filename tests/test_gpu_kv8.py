@@ -493,3 +493,39 @@ def test_captured_attention_with_what_reads_it(B, max_len):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs + reads, want))
+
+
+@pytest.mark.parametrize("S", [32, 33, 40, 1100])
+@pytest.mark.parametrize("lead", [64, 200])
+def test_append_behind_rows_of_no_sequence(S, lead):
+    """Packed prompts whose first one does not start at row 0, fresh slots and slots that hold finished blocks: these, the slots on
+    either side and the rows of no sequence stay as they are."""
+    from helix_substrate_b200.kv8 import Kv8Cache, rope_append_prompt_kv8
+    dev, nq, nkv, D, max_len = _dev(), 3, 1, 64, 256
+    g = torch.Generator().manual_seed(S + lead)
+    outer, ref = Kv8Cache.empty(S + 4, nkv, max_len, D, dev), RefCache(S, nkv, D)
+    cache = outer[2: S + 2]
+    cos, sin = tables(max_len, D, "cpu")
+    for turn in range(3):
+        lens = [int(x) for x in torch.randint(0, 80, (S,), generator=g)]
+        lens[0], lens[S - 1] = (10, 64) if turn else (70, 5)
+        pos = [ref.length(s) for s in range(S)]
+        cu = [lead + sum(lens[:s]) for s in range(S + 1)]
+        qkv = torch.randn(cu[-1], (nq + 2 * nkv) * D, generator=g).bfloat16()
+        qkv[:lead] = float("nan")
+        q_out = torch.full((cu[-1], nq * D), 7.0, device=dev, dtype=torch.bfloat16)
+        k_out = torch.full((cu[-1], nkv, D), 7.0, device=dev, dtype=torch.bfloat16)
+        rope_append_prompt_kv8(qkv.to(dev), torch.tensor(cu, dtype=torch.int32, device=dev), max(lens), torch.tensor(pos, device=dev), cos.to(dev), sin.to(dev),
+                               q_out, k_out, cache, nq)
+        x = qkv[lead:].view(-1, nq + 2 * nkv, D)
+        at = torch.tensor([p + i for p, n in zip(pos, lens) for i in range(n)])
+        turned = rotate(x[:, : nq + nkv], cos[at][:, None], sin[at][:, None])
+        assert torch.equal(q_out[lead:].cpu(), turned[:, :nq].flatten(1)) and torch.equal(k_out[lead:].cpu(), turned[:, nq:])
+        assert bool((q_out[:lead] == 7).all()) and bool((k_out[:lead] == 7).all())
+        for s in range(S):
+            a, b = cu[s] - lead, cu[s + 1] - lead
+            ref.append(s, turned[a:b, nq:], x[a:b, nq + nkv:])
+        _check_cache(cache, ref)
+        for name in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail"):
+            t = getattr(outer, name)
+            assert not bool(t[:2].any()) and not bool(t[S + 2:].any()), name
