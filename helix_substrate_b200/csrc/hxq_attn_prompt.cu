@@ -163,7 +163,7 @@ __device__ __forceinline__ bool find_item(const Args& a, int i, Seq& q, int& s, 
         s = lo;
         q = sequence(a, lo);
         ct = items(q.lq) - 1 - (i - place(lo));
-        return ct >= 0;
+        return ct >= 0 && i >= place(lo);       // (before the first sequence's places, where rows of no sequence precede it: none)
     }
     constexpr int HELD = kSorted / 32;      // (loads that run together)
     int held[HELD];

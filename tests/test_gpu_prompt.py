@@ -424,3 +424,39 @@ def test_captured_with_what_reads_it():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs + reads, want))
+
+
+@pytest.mark.parametrize("S", [128, 129, 1000])
+@pytest.mark.parametrize("lead", [64, 200, 5000])
+@pytest.mark.parametrize("slabs", [False, True])
+def test_rows_of_no_sequence_before_the_first(S, lead, slabs):
+    """Sequences whose first does not start at row 0 (it is empty, too, where keys lie in slabs): rows of none stay as they are, and
+    call after call gives the same bits."""
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, nq, nkv, D = _dev(), 14, 2, 64
+    lens = [(7 * s) % 11 for s in range(S)]
+    lens[0], lens[S // 2] = (0 if slabs else 3), 150
+    T = sum(lens)
+    g = torch.Generator(device=dev).manual_seed(S + lead)
+    q = torch.randn(lead + T + 2, nq, D, device=dev, generator=g).bfloat16()
+    q[:lead], q[lead + T:] = float("nan"), float("nan")
+    cu = [lead + sum(lens[:s]) for s in range(S + 1)]
+    cu_d = torch.tensor(cu, dtype=torch.int32, device=dev)
+    if slabs:
+        k, v = (torch.randn(S, nkv, 160, D, device=dev, generator=g).bfloat16() for _ in range(2))
+        n = [9 + s % 150 for s in range(S)]
+        kw = dict(k_len=torch.tensor(n, device=dev))
+        keys = lambda t, s: t[s, :, : n[s]].transpose(0, 1)        # noqa: E731
+    else:
+        k, v = (torch.randn(lead + T + 2, nkv, D, device=dev, generator=g).bfloat16() for _ in range(2))
+        k[:lead], v[:lead] = float("nan"), float("inf")
+        kw = {}
+        keys = lambda t, s: t[cu[s]: cu[s + 1]]        # noqa: E731
+    outs = [torch.full((lead + T + 2, nq, D), 7.0, device=dev, dtype=torch.bfloat16) for _ in range(10)]
+    for o in outs:
+        attn_prompt(q, k, v, o, cu_d, 150, 0.125, **kw)
+    out = outs[0]
+    assert bool((out[:lead] == 7).all()) and bool((out[lead + T:] == 7).all())
+    assert all(torch.equal(out, o) for o in outs)
+    want = torch.cat([_want(q[cu[s]: cu[s + 1]], keys(k, s), keys(v, s), 0.125, True) for s in range(S) if lens[s]])
+    _compare(out[lead: lead + T], want, "all")
