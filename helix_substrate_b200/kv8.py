@@ -155,9 +155,11 @@ def rope_append_prompt_kv8(qkv: torch.Tensor, cu: torch.Tensor, max_q: int, pos:
     ld_k, max_q = 0, min(max_q, T)
     if k_out is not None:
         if not (k_out.dtype is torch.bfloat16 and k_out.device == dev and tuple(k_out.shape) == (T, cache.kv_heads, cache.D)
-                and k_out.stride(2) == 1 and (cache.kv_heads == 1 or k_out.stride(1) == cache.D)):
-            raise TypeError(f"k_out: expected a bf16 [{T}, {cache.kv_heads}, {cache.D}] tensor on {dev}, contiguous along heads and D")
-        ld_k = max(k_out.stride(0), cache.kv_heads * cache.D)
+                and k_out.stride(2) == 1 and (cache.kv_heads == 1 or k_out.stride(1) == cache.D)
+                and (T <= 1 or k_out.stride(0) >= cache.kv_heads * cache.D)):
+            raise TypeError(f"k_out: expected a bf16 [{T}, {cache.kv_heads}, {cache.D}] tensor on {dev}, contiguous along heads and D, its "
+                            f"rows apart")
+        ld_k = k_out.stride(0) if T > 1 else cache.kv_heads * cache.D        # (a single row's stride says nothing)
     if T == 0:
         return q_out
     _call(dev, "hxq_rope_append_prompt_kv8", cache._ref, qkv.data_ptr(), qkv.stride(0), T, cu.data_ptr(), S, max_q, pos.data_ptr(), stride,

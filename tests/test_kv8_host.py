@@ -102,3 +102,30 @@ def test_reference_quantiser_bounds():
     back = codes.double() * s.repeat_interleave(64, 1)[..., None]
     assert codes.abs().max() == 127 or codes.abs().max() == 126
     assert float(((back - x.double()).abs() / s.repeat_interleave(64, 1)[..., None]).max()) <= 0.5
+
+
+@pytest.mark.parametrize("T", [1, 3])
+def test_prompt_append_takes_no_rows_that_lie_over_one_another(T, monkeypatch):
+    """k_out's rows are written by their stride: one expanded over the tokens, or with rows that overlap, is refused before the C entry
+    is called (whose stride could not stand for it); a single row may have any stride."""
+    from types import SimpleNamespace
+    from helix_substrate_b200 import kv8
+    calls = []
+    monkeypatch.setattr(kv8, "_call", lambda dev, name, *args: calls.append(args))
+    nq, nkv, D = 4, 2, 64
+    cache = SimpleNamespace(device=torch.device("cpu"), kv_heads=nkv, D=D, max_len=128, slots=2, _ref=None)
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)       # noqa: E731
+
+    def append(k_out):
+        kv8.rope_append_prompt_kv8(bf(T, (nq + 2 * nkv) * D), torch.tensor([0, T], dtype=torch.int32), T, torch.tensor([0]), torch.zeros(128, D),
+                                   torch.zeros(128, D), bf(T, nq * D), k_out, cache, nq)
+        return calls.pop()[-2]          # the stride that the C entry gets
+
+    assert append(bf(T, nkv, D)) == nkv * D and append(bf(T, nkv + 1, D)[:, :nkv]) >= nkv * D
+    for k_out in (bf(1, nkv, D).expand(T, nkv, D), bf(T * D + nkv * D).as_strided((T, nkv, D), (D, D, 1))):
+        if T == 1:
+            assert append(k_out) >= nkv * D
+        else:
+            with pytest.raises(TypeError, match="k_out"):
+                append(k_out)
+            assert not calls
