@@ -60,11 +60,27 @@ def _workspace(device: torch.device, nbytes: int, kind: str = "gemv", stream: Op
 
 
 def _status_word(device: torch.device) -> torch.Tensor:
+    """The device's int32 word in which a kernel whose bounded wait gave up leaves HXQ_E_TIMEOUT.  Made outside a
+    capture: inside one the clearing would be a node of the graph and hide at every replay what was raised before."""
     sw = _status_words.get(device.index)
     if sw is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(
+                "hxq kernels need their status word of this device made before a CUDA graph capture starts: "
+                "make one call outside the capture first, then capture")
         sw = torch.zeros(1, dtype=torch.int32, device=device)
+        torch.cuda.current_stream(device).synchronize()        # (cleared, whatever stream its first user runs on)
         _status_words[device.index] = sw
     return sw
+
+
+def check_status(device) -> int:
+    """0, or HXQ_E_TIMEOUT if a bounded wait inside a tensor-core kernel on ``device`` gave up since the process
+    started: outputs of that call are not to be used (synchronises)."""
+    device = torch.device(device)
+    index = torch.cuda.current_device() if device.index is None else device.index
+    sw = _status_words.get(index)
+    return 0 if sw is None else int(sw.item())
 
 
 def csr_from_positions(positions: torch.Tensor, out_features: int, in_features: int):
@@ -117,6 +133,8 @@ class HxqWeight:
             assert t is None or t.device == self.device, "all buffers of one weight live on one device"
         self.desc = self._fill()
         self._dref = C.byref(self.desc)
+        if not torch.cuda.is_current_stream_capturing():
+            _status_word(self.device)
         self._gemv_bytes: dict = {}     # tokens per call (1 .. 16) -> scratch bytes of hxq_gemv
         self._gemm_bytes: dict = {}     # tokens (1 .. GEMM_TS_MAX_M) -> workspace bytes of hxq_gemm
 
@@ -218,7 +236,7 @@ class HxqWeight:
     def gemm_status(self) -> int:
         """Non-zero if a bounded wait inside the tensor-core kernel gave up
         (synchronises the device)."""
-        return int(_status_word(self.device).item())
+        return check_status(self.device)
 
     def algorithmic_bytes(self, M: int, x_bytes: int, y_bytes: int) -> int:
         """Bytes one product has to move whatever the implementation: indices,

@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from .kv8 import _call, _ints
-from .packed import _status_word
+from .packed import _status_word, check_status        # noqa: F401  (check_status: whether a wait inside attn_prompt gave up)
 
 
 _ATTN = struct.Struct("@4P10q3P8if4x")       # HxqAttn as bytes, in half the time that its constructor takes
@@ -33,7 +33,8 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Te
     D]; or rows 0 .. ``k_len[s] - 1`` (int64) of slab s of k, v [S, nkv, rows, D].  Causal attention is aligned at the end:
     with more keys than queries the queries are the last ones.  A query that sees no key gets zeros, rows of ``out``
     [T, nq, D] of no sequence are left as they are, and what a query does not see may hold anything.  q, k, v and out may be
-    views (strides of whole 16 bytes)."""
+    views (strides of whole 16 bytes).  ``check_status(device)`` tells whether a bounded wait inside the kernel gave up.  The first
+    call on a device is not to be a captured one."""
     dev = q.device
     slabs = k_len is not None
     if slabs and cu_k is not None:

@@ -410,6 +410,11 @@ class Qwen2HxqDecoder(nn.Module):
             return decode_ops.dense_gemv(self.lm_head, x)
         return x @ self.lm_head.t()
 
+    def check_status(self) -> int:
+        """0, or HXQ_E_TIMEOUT if a wait inside a tensor-core kernel (projections, fused prompt attention) gave up since the
+        process started: what was generated meanwhile is not to be used (synchronises)."""
+        return prompt_ops.check_status(self.device)
+
     @torch.no_grad()
     def prefill(self, prompt: torch.Tensor, chunk: int = 2048) -> torch.Tensor:
         T = prompt.shape[1]
@@ -567,7 +572,7 @@ def run_decode(shape: str, batches, prompt: int, new_tokens: int, device, rank: 
         if world > 1 and getattr(model, "_ar", None) is not None:
             ar_status = model._ar.check_status()
         out.append({
-            "tok_s": batch * 1000.0 / ms_dec, "ms_per_step": ms_dec, "batch": batch, "context": prompt,
+            "kernel_status_word": model.check_status(), "tok_s": batch * 1000.0 / ms_dec, "ms_per_step": ms_dec, "batch": batch, "context": prompt,
             "new_tokens": new_tokens, "kv_bits": kv_bits, "prompt_attn": model.prompt_attn, "shape": shape, "layers": shp.layers, "n_gpus": world,
             "launch": "python" if run is None else "cuda_graph", "glue": "torch" if torch_glue else "fused",
             "projections": "qkv,o,gate_up,down" if fuse_proj else "q,k,v,o,gate,up,down",

@@ -129,3 +129,15 @@ def test_decoder_refuses():
         _pair(prompt_attn="other")
     with pytest.raises(ValueError, match="8-bit"):
         _pair(kv_bits=8).make_graphed_step(2, fused=False)
+
+
+def test_run_decode_reports_a_wait_that_gave_up():
+    from helix_substrate_b200 import _lib, packed
+    from helix_substrate_b200.qwen2_decode import run_decode
+    word = packed._status_word(_dev())
+    assert run_decode("tiny", [1], 70, 3, _dev(), prompt_attn="fused")[0]["kernel_status_word"] == 0
+    word.fill_(_lib.HXQ_E_TIMEOUT)
+    try:
+        assert run_decode("tiny", [1], 70, 3, _dev(), kv_bits=8)[0]["kernel_status_word"] == _lib.HXQ_E_TIMEOUT
+    finally:
+        word.zero_()

@@ -460,3 +460,27 @@ def test_rows_of_no_sequence_before_the_first(S, lead, slabs):
     assert all(torch.equal(out, o) for o in outs)
     want = torch.cat([_want(q[cu[s]: cu[s + 1]], keys(k, s), keys(v, s), 0.125, True) for s in range(S) if lens[s]])
     _compare(out[lead: lead + T], want, "all")
+
+
+def test_status_word_outlives_replays(monkeypatch):
+    """The word is made outside a capture (a first call under one is refused) and no replay clears it."""
+    from helix_substrate_b200 import packed
+    from helix_substrate_b200.prompt_ops import attn_prompt, check_status
+    monkeypatch.setattr(packed, "_status_words", {})
+    dev, T = _dev(), 40
+    q, k = (torch.randn(T, n, 64, device=dev).bfloat16() for n in (4, 2))
+    cu, out = torch.tensor([0, T], dtype=torch.int32, device=dev), torch.empty_like(q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            with pytest.raises(RuntimeError, match="capture"):
+                attn_prompt(q, k, k, out, cu, T, 0.1)
+        attn_prompt(q, k, k, out, cu, T, 0.1)
+        assert check_status(dev) == 0
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            attn_prompt(q, k, k, out, cu, T, 0.1)
+        packed._status_word(dev).fill_(-7)
+        graph.replay()
+        assert check_status(dev) == -7 == check_status("cuda:0")

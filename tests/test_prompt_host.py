@@ -70,3 +70,22 @@ def test_wrapper_refuses():
         attn_prompt(q, k, k, q, cu, 4, 0.1)
     with pytest.raises(ValueError, match="not both"):
         attn_prompt(q, k, k, q, cu, 4, 0.1, cu_k=cu, k_len=n)
+
+
+def test_first_use_under_capture_is_refused(monkeypatch):
+    """The device's status word is made and cleared outside a capture: as a node of a graph the clearing would run at every replay."""
+    from helix_substrate_b200 import packed
+    monkeypatch.setattr(packed, "_status_words", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="capture"):
+        packed._status_word(torch.device("cpu"))
+    assert not packed._status_words
+    word = packed._status_words[None] = torch.tensor([-7], dtype=torch.int32)
+    assert packed._status_word(torch.device("cpu")) is word
+
+
+def test_status_is_read_per_device(monkeypatch):
+    from helix_substrate_b200 import packed, prompt_ops
+    monkeypatch.setattr(packed, "_status_words", {3: torch.tensor([-7], dtype=torch.int32)})
+    assert prompt_ops.check_status(torch.device("cuda", 3)) == -7
+    assert prompt_ops.check_status("cuda:2") == 0 and 2 not in packed._status_words        # nothing has run there
