@@ -85,7 +85,7 @@ struct Args {
     int32_t* status;
     int64_t v_seq, v_head, v_row, o_tok, o_head;
     float* part;            // splits > 1: [items][splits][DP + 2][2 * BM]: reference point, sum, output before the division
-    int32_t Tq, Tk, S, nkv, G, D, tpg, rows, n_ct, causal, splits, alone, groups;     // rows: tokens of an item; alone: key tiles up to which a sequence's items are not shared; groups of 32 rows of an item that any token can fill
+    int32_t Tq, Tk, S, max_q, nkv, G, D, tpg, rows, n_ct, causal, splits, alone, groups;     // max_q: tokens of a sequence that are computed; rows: tokens of an item; alone: key tiles up to which a sequence's items are not shared; groups of 32 rows of an item that any token can fill
     float scale_log2;
 };
 
@@ -734,7 +734,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         if (ok) {
             sm100::tc_fence_after_sync();
             const int tok = job[6] + x * a.tpg + row / a.G, head = job[7];
-            const bool live = row < a.G * a.tpg && tok < job[2], shared = TILES == 2 && a.splits > 1 && find_share(a, job[2], job[4], job[6]).used > 1;
+            const bool live = row < a.G * a.tpg && tok < job[2] && tok < a.max_q, shared = TILES == 2 && a.splits > 1 && find_share(a, job[2], job[4], job[6]).used > 1;
             const float inv = shared ? 1.f : 1.f / l;
             const bool odd = nx > 0 && *odd_v != 0;
             __nv_bfloat16* dst = a.out + (int64_t)(job[1] + tok) * a.o_tok + (int64_t)(head * a.G + row % a.G) * a.o_head;
@@ -835,7 +835,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a) {
     if (!find_item(a, item, seq, s, ct, kvh)) return;
     const int used = find_share(a, seq.lq, seq.lk, ct * a.rows).used;
     if (used == 1) return;              // written already
-    const int x = group >> 2, first = (2 * ct + x) * a.tpg, left = seq.lq - first, rows = a.G * (left < a.tpg ? left : a.tpg);
+    const int x = group >> 2, first = (2 * ct + x) * a.tpg, left = (seq.lq < a.max_q ? seq.lq : a.max_q) - first, rows = a.G * (left < a.tpg ? left : a.tpg);
     const int in = (group & 3) * 32 + lane;
     float m = -INFINITY, l = 0.f, o[kJoin] = {};
     if (in < rows) {
@@ -919,7 +919,7 @@ static int run_tiles(const hxq_attn* p, const Plan& plan, void* workspace, int32
     a.out = reinterpret_cast<__nv_bfloat16*>(p->out);
     a.status = status;
     a.v_seq = p->v_seq; a.v_head = p->v_head; a.v_row = p->v_row; a.o_tok = p->o_tok; a.o_head = p->o_head;
-    a.Tq = p->Tq; a.Tk = p->Tk; a.S = p->S; a.nkv = p->nkv; a.G = p->nq / p->nkv; a.D = p->D; a.causal = p->causal != 0;
+    a.Tq = p->Tq; a.Tk = p->Tk; a.S = p->S; a.max_q = p->max_q; a.nkv = p->nkv; a.G = p->nq / p->nkv; a.D = p->D; a.causal = p->causal != 0;
     a.tpg = plan.tpg;
     a.rows = plan.rows;
     a.n_ct = plan.n_ct;

@@ -29,7 +29,7 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Te
                 scale: float, *, cu_k: Optional[torch.Tensor] = None, k_len: Optional[torch.Tensor] = None,
                 causal: bool = True) -> torch.Tensor:
     """Sequence s has the queries ``q[cu_q[s]: cu_q[s + 1]]`` of q [T, nq, D] (int32 offsets on the device, none longer
-    than ``max_q``).  Its keys and values are the same rows of k, v [T, nkv, D]; or rows ``cu_k[s]`` .. of k, v [Tk, nkv,
+    than ``max_q``: queries past it are not computed and their rows of ``out`` left as they are).  Its keys and values are the same rows of k, v [T, nkv, D]; or rows ``cu_k[s]`` .. of k, v [Tk, nkv,
     D]; or rows 0 .. ``k_len[s] - 1`` (int64) of slab s of k, v [S, nkv, rows, D].  Causal attention is aligned at the end:
     with more keys than queries the queries are the last ones.  A query that sees no key gets zeros, rows of ``out``
     [T, nq, D] of no sequence are left as they are, and what a query does not see may hold anything.  q, k, v and out may be

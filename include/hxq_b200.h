@@ -243,8 +243,8 @@ int32_t hxq_attn_decode_span(int32_t B, int32_t nkv, int32_t max_len);
  * 0 .. k_len[s] - 1 of slab s of k, v [S, nkv, Tk, D] (a cache).  causal: query i of lq sees keys 0 .. lk - lq + i, so the
  * last query sees all; a query that sees none gets zeros.  What a query does not see may hold anything, NaN too.
  * cu_q, cu_k (int32 [S + 1], ascending) and k_len (int64 [S]) are DEVICE arrays, exactly one of cu_k and k_len given;
- * max_q: no sequence has more queries (those past it are not computed).  Rows of out that belong to no sequence are
- * left as they are.  Strides in elements, multiples of 8; pointers 16-byte aligned; D % 8 == 0, 8 <= D <= 128;
+ * max_q: no sequence has more queries (of a longer one the first max_q are computed, as the first of all).  Rows of out that
+ * belong to no sequence, or to queries past max_q, are left as they are.  Strides in elements, multiples of 8; pointers 16-byte aligned; D % 8 == 0, 8 <= D <= 128;
  * nq / nkv <= 64; Tq, Tk <= 2^30; scale > 0.  status_word as in hxq_gemm.  Few queries before many keys split the keys among
  * thread blocks: workspace is hxq_attn_prompt_workspace_bytes() of 8-byte aligned scratch (0: none needed).
  */

@@ -484,3 +484,29 @@ def test_status_word_outlives_replays(monkeypatch):
         packed._status_word(dev).fill_(-7)
         graph.replay()
         assert check_status(dev) == -7 == check_status("cuda:0")
+
+
+@pytest.mark.parametrize("nq,nkv,D,lens,keys", [(28, 4, 128, [50, 3, 30], None), (128, 4, 64, [700, 37, 300, 900], None), (14, 2, 128, [40, 5], [6000, 5]),
+                                                (8, 8, 64, [200], [9000])])
+@pytest.mark.parametrize("max_q", [1, 4, 33])
+def test_queries_past_max_q_are_left_alone(nq, nkv, D, lens, keys, max_q):
+    """Sequences longer than max_q, tiles one to a thread block, two, and with their keys shared out: of each the first max_q queries are
+    computed, as the first of all its queries, and no other row of out is touched."""
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, T, S = _dev(), sum(lens), len(lens)
+    g = torch.Generator(device=dev).manual_seed(T + max_q)
+    q = torch.randn(T, nq, D, device=dev, generator=g).bfloat16()
+    cu = [sum(lens[:s]) for s in range(S + 1)]
+    if keys is None:
+        k, v = (torch.randn(T, nkv, D, device=dev, generator=g).bfloat16() for _ in range(2))
+        kw, of = {}, lambda t, s: t[cu[s]: cu[s + 1]]
+    else:
+        k, v = (torch.randn(S, nkv, max(keys), D, device=dev, generator=g).bfloat16() for _ in range(2))
+        kw, of = dict(k_len=torch.tensor(keys, device=dev)), lambda t, s: t[s, :, : keys[s]].transpose(0, 1)
+    for causal in (True, False):
+        out = torch.full((T, nq, D), 7.0, device=dev, dtype=torch.bfloat16)
+        attn_prompt(q, k, v, out, torch.tensor(cu, dtype=torch.int32, device=dev), max_q, 0.15, causal=causal, **kw)
+        for s, (a, b) in enumerate(zip(cu, cu[1:])):
+            m = min(max_q, b - a)
+            _compare(out[a: a + m], _want(q[a:b], of(k, s), of(v, s), 0.15, causal)[:m], (causal, s))
+            assert bool((out[a + m: b] == 7).all()), (causal, s)
