@@ -434,6 +434,13 @@ __device__ __forceinline__ uint32_t bf2_of(float lo, float hi) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+// A pair of bf16 numbers, infinities and NaNs replaced by bf16's largest.
+__device__ __forceinline__ uint32_t finite2(uint32_t x) {
+    uint32_t r;
+    asm("min.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x7f7f7f7fu));
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(x) : "r"(r), "r"(0xff7fff7fu));
+    return x;
+}
 // Two biased bytes (code + 128), picked by sel out of x, as two fp16 numbers 1024 + byte (0x64nn): the code + 1152, exactly.
 template <uint32_t SEL>
 __device__ __forceinline__ uint32_t codes2(uint32_t x) { return __byte_perm(x, 0x64646464u, SEL); }
@@ -555,6 +562,7 @@ __device__ __forceinline__ Share find(const DecodeArgs& a, int cta, int at, int6
 //     took every sector twice and stopped at 4.3 TB/s).  The next unit's keys are fetched as soon as this one's are used, its values likewise:
 //     8 to 16 KB a warp are in flight.
 //   * the tail's products run in bf16, 16 positions to a warp, with each probability as the sum of two bf16 numbers (2^-17).
+//     Infinities and NaNs of its values reach the result, by the first of the two alone.
 template <int DP>
 struct DecodeSmem { static constexpr int bytes = kWarps * 128 * DP; };
 
@@ -751,7 +759,8 @@ __global__ void __launch_bounds__(32 * kWarps, kDecodeCtas) decode_kernel(const 
                     const uint32_t a0 = __byte_perm(x0, x1, 0x5410), a1 = __byte_perm(x0, x1, 0x7632);
                     const uint32_t a2 = __byte_perm(x2, x3, 0x5410), a3 = __byte_perm(x2, x3, 0x7632);
                     mma_bf16(o[n0 / 2 + e], a0, a1, a2, a3, hi[0], hi[1]);
-                    mma_bf16(o[n0 / 2 + e], a0, a1, a2, a3, lo[0], lo[1]);
+                    // (an infinity is the high part's alone: the low one, zero or of the other sign, would make a NaN of it)
+                    mma_bf16(o[n0 / 2 + e], finite2(a0), finite2(a1), finite2(a2), finite2(a3), lo[0], lo[1]);
                 }
             }
         }

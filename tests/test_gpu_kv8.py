@@ -529,3 +529,42 @@ def test_append_behind_rows_of_no_sequence(S, lead):
         for name in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail"):
             t = getattr(outer, name)
             assert not bool(t[:2].any()) and not bool(t[S + 2:].any()), name
+
+
+@pytest.mark.parametrize("max_len,n", [(128, 36), (512, 300), (512, 257), (1 << 15, 20000), (1 << 15, 30)])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_bad_values_in_the_tail(max_len, n, bad):
+    """An infinity or a NaN in a row of V of the unfinished block is that dimension's result, for the heads that read it; in a row of K
+    it makes its scores infinite or none.  Clusters and shares, a tail alone and behind blocks."""
+    from helix_substrate_b200.kv8 import attn_decode_kv8
+    dev, nq, nkv, D = _dev(), 14, 2, 64
+    cache, ref = _filled(1, nkv, max_len, D, [n], seed=n)
+    g = torch.Generator().manual_seed(n)
+    q = torch.rand(1, nq, D, generator=g).bfloat16() + 0.25          # (of one sign: what an infinite key's score is)
+    out = torch.empty(1, nq * D, device=dev, dtype=torch.bfloat16)
+    pos = torch.tensor([n - 1], device=dev)
+
+    def check(what):
+        attn_decode_kv8(q.flatten(1).to(dev), cache, pos, out, nq, 0.1)
+        got = out.cpu().double().view(nq, D)
+        k, v = (ref.values(x, 0).repeat_interleave(nq // nkv, 0) for x in ("k", "v"))
+        s = torch.einsum("hd,hjd->hj", q[0].double(), k) * 0.1
+        want = torch.einsum("hj,hjd->hd", s.softmax(-1), v)          # (a key of -inf with a value of inf: 0 * inf, none)
+        assert torch.equal(want.isnan(), got.isnan()), what
+        assert torch.equal(want.isinf(), got.isinf()) and torch.equal(want[want.isinf()], got[got.isinf()]), what
+        fine = want.isfinite()
+        assert not bool(fine.any()) or rel_l2(got[fine], want[fine]) < TOL, what
+
+    first, last = n // BLOCK * BLOCK, n - 1
+    for name in ("v", "k"):
+        tail, rows = getattr(cache, name + "_tail"), ref.rows[name][0]
+        for row, h, d in ((first, 0, 3), (last, 1, 62)):
+            keep = rows[h, row, d].clone()
+            rows[h, row, d] = bad
+            tail[0, h, row % BLOCK, d] = bad
+            check((name, row))
+            if row == last:
+                break
+            rows[h, row, d] = keep
+            tail[0, h, row % BLOCK, d] = keep
+        rows[1, last, 62], tail[0, 1, last % BLOCK, 62] = 0.5, 0.5
