@@ -638,8 +638,8 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
         const uint32_t to = t_lane + 128u * TILES + 128u * x;
         const float sc = a.scale_log2;
         float ref = -INFINITY, l = 0.f;         // in units of S
-        float first = 0.f, bias = 0.f;
-        bool far = false;
+        float first = 0.f, bias = 0.f;          // weights are 2^((S - first) sc + bias)
+        bool far = false;                       // first is not zero in some lane
         for (int j = 0; j < nx; ++j) {
             const int buf = j & 1;
             const uint32_t ts = t_lane + 128u * x + 64u * buf;
@@ -673,11 +673,13 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_const
                 const float corr = move ? ex2((ref - mx) * sc) : 1.f;
                 if (move) ref = mx;
                 l *= corr;
-                // 2^(S sc - ref sc) in one multiply-add: the rounding of ref sc shifts a whole row and divides out, unless
-                // scores are so large that it is itself large; then the difference is taken first
-                far = __any_sync(0xffffffffu, ref != -INFINITY && fabsf(ref * sc) > 65536.f);
-                first = ref == -INFINITY ? 0.f : ref;
-                bias = far ? 0.f : -first * sc;
+                // 2^(S sc - ref sc) in one multiply-add.  The rounding of ref sc divides out only among the keys of one reference point;
+                // up to 1024 it is 2^-15 at most, 2.1e-5 of a weight (P's own rounding is 2^-8), beyond, the difference is taken
+                // first.  A row by itself: its neighbours in the warp may be other sequences' and have no say in its bits.
+                const bool large = ref != -INFINITY && fabsf(ref * sc) > 1024.f;
+                far = __any_sync(0xffffffffu, large);
+                first = large ? ref : 0.f;
+                bias = large || ref == -INFINITY ? 0.f : -ref * sc;
                 if (j > 0) {
                     // the product before has retired: the next step's scores come after it, or, at the end, its own signal does
                     const bool next = j + 1 < nx;

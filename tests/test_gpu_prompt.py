@@ -510,3 +510,52 @@ def test_queries_past_max_q_are_left_alone(nq, nkv, D, lens, keys, max_q):
             m = min(max_q, b - a)
             _compare(out[a: a + m], _want(q[a:b], of(k, s), of(v, s), 0.15, causal)[:m], (causal, s))
             assert bool((out[a + m: b] == 7).all()), (causal, s)
+
+
+@pytest.mark.parametrize("lens,keys", [([61, 9], None), ([700, 400], None), ([9, 3], [3000, 2])])
+@pytest.mark.parametrize("loud", [30.0, 3e4])
+def test_a_neighbours_scores_change_no_bit(lens, keys, loud):
+    """Rows of one tile are other heads', other tokens' and other sequences': whatever the size of theirs, a row's bits stay."""
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, nq, nkv, D, T, S = _dev(), 8, 1, 64, sum(lens), len(lens)
+    g = torch.Generator(device=dev).manual_seed(T)
+    q = torch.randn(T, nq, D, device=dev, generator=g).bfloat16() * 3
+    rows = T if keys is None else max(keys)
+    k, v = (torch.randn(*((rows,) if keys is None else (S, nkv, rows)), *((nkv, D) if keys is None else (D,)), device=dev, generator=g).bfloat16() for _ in range(2))
+    kw = {} if keys is None else dict(k_len=torch.tensor(keys, device=dev))
+    cu = torch.tensor([0, lens[0], T], dtype=torch.int32, device=dev)
+    out, other = torch.empty_like(q), torch.empty_like(q)
+    attn_prompt(q, k, v, out, cu, max(lens), 1.0, **kw)
+    q2 = q.clone()
+    q2[:, 0] *= loud             # a head
+    q2[::5] *= loud              # tokens
+    q2[lens[0]:] *= loud         # the next sequence
+    attn_prompt(q2, k, v, other, cu, max(lens), 1.0, **kw)
+    same = (q2 == q).all(-1)
+    assert bool(same.any()) and torch.equal(out[same], other[same])
+
+
+@pytest.mark.parametrize("n", [2000, 6000])
+@pytest.mark.parametrize("size", [500.0, 2000.0, 20000.0, 60000.0])
+def test_reference_points_that_move_among_large_scores(n, size):
+    """Scores about `size`, sixteen keys of them as heavy together as half of all, values that nearly cancel: weights count across a move
+    of the reference point and across shares of the keys."""
+    from math import log
+    from helix_substrate_b200.prompt_ops import attn_prompt
+    dev, D, T = _dev(), 64, 8
+    g = torch.Generator(device=dev).manual_seed(n)
+    q = torch.zeros(T, 1, D, device=dev)
+    q[:, :, 0] = 256.0
+    q[:, :, 1] = 1.0
+    big = torch.tensor(size / 256, device=dev).bfloat16()
+    k, v = torch.zeros(n, 1, D, device=dev), torch.randn(n, 1, D, device=dev, generator=g) * 0.01
+    k[:, :, 0] = big.float()
+    k[n // 2: n // 2 + 16, :, 1] = log(n / 2 / 16)
+    v[: n // 2] += 1.0
+    v[n // 2: n // 2 + 16] -= 1.0
+    q, k, v = q.bfloat16(), k.bfloat16(), v.bfloat16()
+    out = torch.empty_like(q)
+    attn_prompt(q, k, v, out, torch.tensor([0, T], dtype=torch.int32, device=dev), T, 1.0, cu_k=torch.tensor([0, n], dtype=torch.int32, device=dev), causal=False)
+    want = _want(q, k, v, 1.0, False)
+    # fp32 holds a score of `size` to 2^-24 size; weights are rounded to bf16 (2^-8), the output too; sums of |w v| / w are below 1.1
+    assert float((out.double() - want).abs().max()) <= 1.1 * (2.0 ** -8 + size * 2.0 ** -23) + 2.0 ** -8
