@@ -5,10 +5,10 @@
 // Per (sequence, KV head) the positions form blocks of 64.  A finished block holds codes x = s * code with
 //     s = max(up(max |x| / 127), 2^-126),   code = rint(x / s) in -127 .. 127,
 // up() rounding up to bf16.  x and s then both have 8 significant bits, so x / s is a tie exactly or at least
-// 1/510 off one: the fp32 division decides every code as exact arithmetic would.  A block with an infinity or a
-// NaN gets s = NaN and reads back as NaN.  The rows of the last, unfinished block stay bf16 in the tail
-// (row = position mod 64) and are quantised once, when the 64th arrives: no row is ever rounded twice, and what a
-// cache holds does not depend on how a prompt was cut into calls.
+// 1/510 off one: x times the rounded reciprocal, snapped to multiples of 1/1024, decides every code as exact arithmetic
+// would.  A block with an infinity or a NaN gets s = NaN and reads back as NaN.  The rows of the last, unfinished
+// block stay bf16 in the tail (row = position mod 64) and are quantised once, when the 64th arrives: no row is ever
+// rounded twice, and what a cache holds does not depend on how a prompt was cut into calls.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -234,7 +234,7 @@ __device__ void append_block(const AppendArgs& a, bool is_k, int s, int h, int b
     scale = fmaxf(scale, 1.17549435e-38f);
     int8_t* codes = (is_k ? a.c.k : a.c.v) + (head * a.c.max_len + b0) * D;
     if (threadIdx.x == 0) (is_k ? a.c.ks : a.c.vs)[head * (a.c.max_len / kBlock) + blk] = bad ? __uint_as_float(0x7fc00000u) : scale;
-    // x / s is a tie exactly or at least 1/512 off one (both have 8 significant bits): x * fl(1 / s), off by 2^-16 at most, is
+    // x / s is a tie exactly or at least 1/510 off one (both have 8 significant bits): x * fl(1 / s), off by 2^-16 at most, is
     // snapped to multiples of 1/1024, where ties are ties again, and then rounded; the code is the low byte of 1.5 * 2^23 + it.
     const float inv = bad ? 0.f : __fdiv_rn(1.f, scale);
     auto code = [&](float x) {

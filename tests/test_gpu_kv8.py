@@ -568,3 +568,29 @@ def test_bad_values_in_the_tail(max_len, n, bad):
             rows[h, row, d] = keep
             tail[0, h, row % BLOCK, d] = keep
         rows[1, last, 62], tail[0, 1, last % BLOCK, 62] = 0.5, 0.5
+
+
+@pytest.mark.parametrize("e", [-126, -124, -100, -10, 0, 1, 60, 120])
+def test_codes_of_every_mantissa(e):
+    """Blocks under every mantissa of the largest element (scales clamped to 2^-126 among them), each holding every mantissa in nine
+    octaves below it, both signs, ties in plenty: exactly the codes of exact arithmetic."""
+    from helix_substrate_b200.kv8 import Kv8Cache, rope_append_prompt_kv8
+    dev, D = _dev(), 128
+    m = torch.arange(128, 256, dtype=torch.float64)
+    x = torch.cat([m * 2.0 ** (e - 7 - d) for d in range(9)])                          # [9 * 128]
+    rows = torch.zeros(128, BLOCK * D, dtype=torch.float64)
+    for i, a in enumerate(m.tolist()):
+        y = x.where(x <= a * 2.0 ** (e - 7), -x / 2)
+        rows[i, : 2 * y.numel()] = torch.cat([y, -y])
+        rows[i, 2 * y.numel()] = a * 2.0 ** (e - 7)
+    rows = rows.view(128 * BLOCK, D).bfloat16()
+    n = rows.shape[0]
+    qkv = torch.zeros(n, 3, D, dtype=torch.bfloat16)
+    qkv[:, 2] = rows
+    cache, cos = Kv8Cache.empty(1, 1, n, D, dev), torch.zeros(n, D, device=dev)
+    rope_append_prompt_kv8(qkv.flatten(1).to(dev), torch.tensor([0, n], dtype=torch.int32, device=dev), n, torch.zeros(1, dtype=torch.int64, device=dev),
+                           cos, cos, torch.empty(n, D, device=dev, dtype=torch.bfloat16), None, cache, 1)
+    codes, s = quantise(rows[None])
+    assert torch.equal(cache.v_scale[0, 0].cpu().double(), s[0])
+    assert torch.equal(cache.v[0, 0].cpu(), codes[0])
+    assert bool(codes.any())

@@ -129,3 +129,25 @@ def test_prompt_append_takes_no_rows_that_lie_over_one_another(T, monkeypatch):
             with pytest.raises(TypeError, match="k_out"):
                 append(k_out)
             assert not calls
+
+
+@pytest.mark.parametrize("e", [-126, -124, -118, -100, -10, 0, 1, 60, 120, 127])
+def test_reciprocal_and_snapping_give_the_exact_codes(e):
+    """The append's arithmetic, step by step in fp32: x fl(1 / s) added to 12288 in one rounding and taken off again (multiples of 1/1024),
+    the code from the low byte of that + 1.5 * 2^23.  Under every mantissa of max|x|, for every mantissa of x in ten octaves, both signs.
+    x / s is a tie or 1/510 and more off one, so its fp64 quotient, off by 2^-46 at most, rounds as exact arithmetic does."""
+    f32 = np.float32
+    m = np.arange(128, 256) * 2.0 ** (e - 7)
+    m = m[m < 3.39e38].astype(f32)
+    s = ((m / f32(127)).view(np.uint32) + np.uint32(0xffff) & np.uint32(0xffff0000)).view(f32)
+    s = np.maximum(s, f32(2.0 ** -126))[:, None]
+    x = np.concatenate([np.arange(128, 256) * 2.0 ** (e - 7 - d) for d in range(10)])
+    x = torch.from_numpy(np.concatenate([x, -x, [0.0]])).bfloat16().double().numpy()          # (some below 2^-133: none)
+    x = np.where(np.abs(x) <= m[:, None].astype(np.float64), x, 0.0)
+    want = np.rint(x / s.astype(np.float64))
+    inv = f32(1) / s
+    # (the product has 32 bits, 12288 is 2^13.6 and x inv at least 2^-12 where it can matter: fp64 holds the sum, one rounding follows)
+    q = (x * inv.astype(np.float64) + 12288.0).astype(f32) - f32(12288)
+    assert np.array_equal(np.abs(q - np.floor(q)) == 0.5, np.abs(x / s.astype(np.float64) - np.floor(x / s.astype(np.float64))) == 0.5), "ties are ties"
+    code = ((q + f32(12582912)).view(np.uint32) & np.uint32(0xff)).astype(np.uint8).view(np.int8)
+    assert np.array_equal(code, want) and np.abs(want).max() <= 127
