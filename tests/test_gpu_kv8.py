@@ -575,6 +575,7 @@ def test_codes_of_every_mantissa(e):
     """Blocks under every mantissa of the largest element (scales clamped to 2^-126 among them), each holding every mantissa in nine
     octaves below it, both signs, ties in plenty: exactly the codes of exact arithmetic."""
     from helix_substrate_b200.kv8 import Kv8Cache, rope_append_prompt_kv8
+    from kv8_ref import quantise
     dev, D = _dev(), 128
     m = torch.arange(128, 256, dtype=torch.float64)
     x = torch.cat([m * 2.0 ** (e - 7 - d) for d in range(9)])                          # [9 * 128]
