@@ -17,7 +17,7 @@
 //                     tensor memory for the whole row
 //
 // Roles: four warps a tile are its softmax and epilogue, one warp feeds K and V through a ring, one issues the MMAs, two
-// clean V tiles.  P is rounded to bf16, V's type (the MMA takes no other beside it): 2^-9 at most per weight, as much as
+// clean V tiles.  P is rounded to bf16, V's type (the MMA takes no other beside it): 2^-8 at most per weight, as much as
 // the output's own rounding; the sum that divides takes the weights before rounding.
 //
 // Bound by the tensor cores for long prompts, by each CTA's start and end for short ones.  A step's products, its softmax
@@ -321,7 +321,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {       // NaN 
     return r;
 }
 // 2^x of a pair on the multiply-add units: x = n + f with n whole, |f| <= 1/2 (adding and taking off 1.5 * 2^23 leaves n, in
-// the low bits too); 2^f by a polynomial of least largest relative error, 1.0e-4 (a twentieth of P's rounding), with the
+// the low bits too); 2^f by a polynomial of least largest relative error, 1.0e-4 (a fortieth of P's rounding), with the
 // constant term 1; n added to the exponent.  From x = -127 down, and at -inf, it is 0 (there f = 0, and 1's exponent is
 // 127).  x <= 127.
 __device__ __forceinline__ f2 ex2_pair(f2 x) {

@@ -77,7 +77,7 @@ __device__ __forceinline__ uint4 ld16(const void* p) { return *reinterpret_cast<
 // on.  Nearly always fp32 tells the same: r = fma(x, cos, fl(y sin)) is off by 2^-24 (|y sin| + |r|) at most and the
 // true sum's fp32 value by one more rounding, so where r - d and r + d, d = 2^-23 (|y sin| + |r|), round to the same bf16, that is
 // it.  One value in some 2^13 takes the 64-bit path.  (All in 64 bits, conversions alone filled half of the time: 86 us for 8191
-// tokens of 28 + 4 heads where this takes 41; exact sums of products and their rests in packed fp32 took 42 to 48.)
+// tokens of 28 + 4 heads where this takes 36; exact sums of products and their rests in packed fp32 took 42 to 48 when this took 41.)
 __device__ __forceinline__ uint32_t turn(float x, float c, float y, float s, bool& sure) {
     const float p = y * s, r = fmaf(x, c, p);
     const float d = fmaf(fabsf(p) + fabsf(r), 1.0001f * 1.1920929e-7f, 2.8e-45f);
@@ -548,20 +548,22 @@ __device__ __forceinline__ Share find(const DecodeArgs& a, int cta, int at, int6
 // Bound by HBM: each code is read once, 2 D bytes a position and KV head.  On the CUDA cores G query heads cost G
 // multiply-adds a code, more than the cores have at the memory's pace from G = 5 on, so both products go through
 // mma.sync (a tcgen05 tile would want 128 rows of queries; there are eight).
-//   * Q K^T runs in int8, the codes as they are.  A query row is rounded to 16 bits, a step of 2^-16 of its largest element
-//     (bf16 itself has steps of 2^-9 of each), as two int8 planes q = 256 hi + lo: heads' high parts are rows 0-7 of the
+//   * Q K^T runs in int8, the codes as they are.  A query row is rounded to 16 bits, off by 2^-16 of its largest element at
+//     most (bf16's rounding is 2^-8 of each: elements below 2^-8 of the largest lose more here), as two int8 planes q = 256 hi + lo: heads' high parts are rows 0-7 of the
 //     MMA, low parts rows 8-15, and both sums of a score end in one lane.  They are exact; scales multiply in fp32.
 //   * P V runs in fp16 with fp32 sums: a code becomes the fp16 number code + 1152 (byte permutes alone), the sum starts at
-//     -1152 times the sum of the probabilities (32 positions at a time: it costs a hundredth of the output's rounding).
+//     -1152 times the sum of the probabilities, 32 positions at a time.  The tensor cores cut sums, not round them: that leaves
+//     -5e-5 of a code's step in every output, at any length (random values: a hundredth of the output's rounding at 4096 positions
+//     of equal weight, a sixteenth at 131072).
 //     Dimensions are the MMA's rows and heads its columns, which is how the scores' layout already holds P.  Probabilities are scaled by
-//     2^10 and rounded to fp16: 2^-12 relative (a sixteenth of the output's own rounding) down to 2^-24 of the largest, 2^-35
+//     2^10 and rounded to fp16: 2^-11 relative (an eighth of the output's own rounding) down to 2^-24 of the largest, 2^-35
 //     of it absolute below that; the sum that divides takes them in fp32.
 //   * the order of a contraction's index is free, so it is chosen such that every lane's operands are 16 consecutive
 //     bytes of a cache row, read without bank conflicts.  Rows pass through a ring in shared memory, one per warp, filled by
 //     asynchronous copies of whole rows: pieces of 16 bytes trade places only within 128 (spread over a slot per lane, the copies
 //     took every sector twice and stopped at 4.3 TB/s).  The next unit's keys are fetched as soon as this one's are used, its values likewise:
-//     8 to 16 KB a warp are in flight.
-//   * the tail's products run in bf16, 16 positions to a warp, with each probability as the sum of two bf16 numbers (2^-17).
+//     8 to 16 KB a warp are in flight.  (168 registers are what three CTAs an SM leave; of D > 64 a few are spilled, 12 to 148 bytes a thread.)
+//   * the tail's products run in bf16, 16 positions to a warp, with each probability as the sum of two bf16 numbers (2^-16).
 //     Infinities and NaNs of its values reach the result, by the first of the two alone.
 template <int DP>
 struct DecodeSmem { static constexpr int bytes = kWarps * 128 * DP; };

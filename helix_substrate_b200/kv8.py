@@ -173,7 +173,7 @@ _ws_bytes: dict = {}
 def attn_decode_kv8(q: torch.Tensor, cache: Kv8Cache, pos: torch.Tensor, out: torch.Tensor, nq: int, scale: float) -> torch.Tensor:
     """Attention of one query token per slot over positions 0..pos of the cache (pos int64 on the device, one per
     sequence or one for all; a negative one, or one past the cache, gives zeros).  At most eight query heads per KV
-    head.  The scratch comes from the caching allocator for the call alone, so captured graphs do not share it."""
+    head.  A query row is held in 16 bits: off by 2^-16 of its largest element, whatever the size of the others.  The scratch comes from the caching allocator for the call alone, so captured graphs do not share it."""
     _groups(nq, cache)
     dev, B = cache.device, q.shape[0]
     _rows(q, "q", dev, nq * cache.D)

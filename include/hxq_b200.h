@@ -286,8 +286,8 @@ typedef struct hxq_kv8 {
 } hxq_kv8;
 
 /* hxq_rope_append for an 8-bit cache.  qkv[b, :] is one new token of the sequence in slot b at position pos[b]
- * (int64 on the DEVICE; pos_stride 1: one per sequence, 0: pos[0] for all).  q and k are rotated (products and sum
- * in fp64, rounded once to bf16), q goes to q_out, k and v to the tail, or, when their row is the 64th of its block,
+ * (int64 on the DEVICE; pos_stride 1: one per sequence, 0: pos[0] for all).  q and k are rotated (as products and sum
+ * in fp64 give them, rounded to fp32 and then to bf16), q goes to q_out, k and v to the tail, or, when their row is the 64th of its block,
  * the block's codes and scales are written from the tail and that row.  A position < 0 or >= max_len leaves that
  * sequence's q_out and cache as they are.  Rows of qkv and q_out 16-byte aligned, tables [max_len, D] too. */
 int hxq_rope_append_kv8(const hxq_kv8* cache, const void* qkv, int64_t ld_qkv, const int64_t* pos, int32_t pos_stride,
@@ -304,7 +304,9 @@ int hxq_rope_append_prompt_kv8(const hxq_kv8* cache, const void* qkv, int64_t ld
                                hxq_stream_t stream);
 
 /* hxq_attn_decode over an 8-bit cache: positions 0 .. pos[b] of slot b, the finished blocks from their codes, the
- * last one from the tail.  A position < 0 or >= max_len gives zeros.  nq / nkv <= 8.  workspace:
+ * last one from the tail.  A position < 0 or >= max_len gives zeros.  nq / nkv <= 8.  Over finished blocks a query row is
+ * held in 16 bits (off by 2^-16 of its largest element at most, also where elements are far smaller) and weights in fp16
+ * (2^-11; below 2^-24 of the largest, 2^-35 of it); sums are exact or fp32.  workspace:
  * hxq_attn_decode_kv8_workspace_bytes() of 8-byte aligned scratch (0: none needed). */
 size_t hxq_attn_decode_kv8_workspace_bytes(int32_t B, int32_t nq, int32_t nkv, int32_t D, int32_t max_len);
 int hxq_attn_decode_kv8(const hxq_kv8* cache, const void* q, int64_t ld_q, const int64_t* pos, int32_t pos_stride,

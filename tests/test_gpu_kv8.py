@@ -595,3 +595,24 @@ def test_codes_of_every_mantissa(e):
     assert torch.equal(cache.v_scale[0, 0].cpu().double(), s[0])
     assert torch.equal(cache.v[0, 0].cpu(), codes[0])
     assert bool(codes.any())
+
+
+@pytest.mark.parametrize("n", [1 << 10, 1 << 17, 1 << 20])
+@pytest.mark.parametrize("spread", [0.01, 1.0])
+def test_values_that_cancel(n, spread):
+    """Pairs of positions with the same key and values of opposite sign: the result is what the arithmetic leaves.  Codes enter as
+    1152 + code, and 1152 times the sum of the weights is taken off: three sums (the weights', two products') that hold numbers of up to
+    1279 times it, each cut to 24 bits, 3 * 2^-23 * 1279 < 2^-11 of a code's step, whatever the length; fp32 sums over the blocks and the
+    output's rounding add 2^-8 of that at most."""
+    from helix_substrate_b200.kv8 import Kv8Cache, attn_decode_kv8
+    dev, nq, D = _dev(), 8, 128
+    cache = Kv8Cache.empty(1, 1, n, D, dev)
+    g = torch.Generator(device=dev).manual_seed(n)
+    v, k = (torch.randint(-127, 128, (n // 2, D), device=dev, generator=g, dtype=torch.int8) for _ in range(2))
+    cache.v[0, 0, 0::2], cache.v[0, 0, 1::2] = v, -v
+    cache.k[0, 0, 0::2], cache.k[0, 0, 1::2] = k, k
+    cache.v_scale.fill_(1.0)
+    cache.k_scale.fill_(1.0)
+    q, out = torch.randn(1, nq * D, device=dev, generator=g).bfloat16(), torch.empty(1, nq * D, device=dev, dtype=torch.bfloat16)
+    attn_decode_kv8(q, cache, torch.tensor([n - 1], device=dev), out, nq, spread / 73 / D ** 0.5)         # (scores of that size)
+    assert float(out.double().abs().max()) <= 2.0 ** -11 * (1 + 2.0 ** -8)
